@@ -229,6 +229,97 @@ int needle2_attention_prefill_device(void *kv, const int *session_ids, const int
  * int8, scales [capacity][kvheads], capacity = window ? window + prefix_len : max_seq. */
 int needle2_kv_export(void *kv, int session, int8_t *keys, int8_t *values, float *k_scales, float *v_scales);
 
+/* ---- additive: attention of a batch behind a shared prefix, key weights, eviction ---- */
+/*
+ * Stateless forms for caches that the caller owns, in device memory: INT8 rows
+ * with one FP32 scale per key and KV head (queries and output FP32), or bf16 or
+ * f16 rows (queries and output of that type).  No counterpart in the reference,
+ * whose attention (needle2/csrc/engine.cpp:898-967) serves one sequence.
+ *
+ * Query token t of sequence b stands at the sequence's own index
+ * i = lengths[b] - tokens[b] + t and sees every prefix key and the own keys j with
+ * j <= i and, where window > 0, j > i - window (the new tokens' own keys are in
+ * the cache before the call).  With z_j = scale * q.k_j over what it sees,
+ * out = sum_j softmax(z)_j v_j and lse = log sum_j e^z_j; a query that sees
+ * nothing gets out 0 and lse -inf.  weights_out = weights + the softmax weights
+ * that each own key received, summed over the queries and over the query heads
+ * of the KV head (every slot of the capacity is written; behind the length the
+ * weight is copied).  Rows of out and lse for t >= tokens[b] are left as they were.
+ *
+ * Strides are in elements; the last axis of q, out, k, v and the prefix is
+ * contiguous, and their pointers and strides are multiples of 16 bytes.
+ * Lengths are clamped to [0, capacity], token counts to [0, tokens].  Own keys at
+ * and behind the length are never used, whatever they hold; every key that any
+ * query of its sequence sees must be finite.
+ */
+typedef struct {
+    int batch, tokens, heads, kvheads, head_dim;   /* head_dim 64 or 128; heads a multiple of kvheads */
+    int prefix, capacity;                          /* keys of the prefix, slots of a sequence's own keys */
+    int window;                                    /* 0: every own key up to the query */
+    int cache_type;                                /* 0 INT8 with scales, 1 bf16, 2 f16 */
+    float scale;                                   /* softmax scale, positive */
+    const void *q;                                 /* [batch][tokens][heads][head_dim] */
+    long long q_stride[3];                         /* batch, token, head */
+    void *out;                                     /* like q; not overlapping the inputs */
+    long long out_stride[3];
+    const void *k, *v;                             /* [batch][kvheads][capacity][head_dim] */
+    long long k_stride[3], v_stride[3];            /* batch, KV head, key */
+    const float *k_scales, *v_scales;              /* [batch][kvheads][capacity], INT8 only */
+    long long k_scale_stride[3], v_scale_stride[3];
+    const void *prefix_k, *prefix_v;               /* [kvheads][prefix][head_dim] */
+    long long prefix_k_stride[2], prefix_v_stride[2];
+    const float *prefix_k_scales, *prefix_v_scales; /* [kvheads][prefix], INT8 only */
+    long long prefix_k_scale_stride[2], prefix_v_scale_stride[2];
+    const int *lengths;                            /* [batch] own keys */
+    const int *token_counts;                       /* [batch] queries, or NULL: `tokens` each */
+    const int *cache_rows;                         /* [batch] row of k, v and scales, or NULL: the sequence's index */
+    float *lse;                                    /* [batch][tokens][heads], or NULL */
+    const float *weights;                          /* [batch][kvheads][capacity], or NULL: no weights */
+    long long weights_stride[3];
+    float *weights_out;                            /* may be `weights` itself, with the same strides */
+    long long weights_out_stride[3];
+} needle2_prefix_attention_args;
+
+/* Bytes of device workspace of a call with these sizes (pointers are not read;
+ * lse and weights count as given or not), or -1.  The workspace needs no
+ * initial contents; calls that may overlap in time need one each. */
+long long needle2_prefix_attention_workspace(const needle2_prefix_attention_args *args);
+/* The call on `stream`; no host synchronisation, no allocation.  `workspace` is
+ * 16-byte aligned and may be NULL where 0 bytes are asked for. */
+int needle2_prefix_attention_device(const needle2_prefix_attention_args *args, void *workspace,
+                                    long long workspace_bytes, void *stream);
+
+/* Eviction by accumulated attention weight.  Of a sequence's n own keys
+ * (lengths, clamped to [0, capacity]) `keep` stay per KV head where n > keep, all
+ * of them otherwise: the first `first`, the last `recent`, and of those between
+ * them the keep - first - recent of the largest weight, the lower index of equal
+ * ones (NaN counts as -inf).  K and V rows, scales and weights of the keys that
+ * stay are packed in their order into the front of the outputs; indices
+ * [batch][kvheads][keep] are theirs, -1 behind them; lengths_out[b] = min(n, keep).
+ * Weights behind the kept ones become 0 up to out_capacity; rows and scales there
+ * are left as they were.  In place (every output its input, with its strides and
+ * out_capacity = capacity) or to memory that overlaps no input; lengths_out
+ * overlaps lengths in neither case.  Enqueued on `stream`. */
+typedef struct {
+    int batch, kvheads, head_dim, capacity, out_capacity, keep, first, recent;
+    int cache_type;
+    const void *k, *v;
+    long long k_stride[3], v_stride[3];
+    const float *k_scales, *v_scales;
+    long long k_scale_stride[3], v_scale_stride[3];
+    const float *weights;
+    long long weights_stride[3];
+    const int *lengths;
+    void *k_out, *v_out;
+    long long k_out_stride[3], v_out_stride[3];
+    float *k_scales_out, *v_scales_out;
+    long long k_scale_out_stride[3], v_scale_out_stride[3];
+    float *weights_out;
+    long long weights_out_stride[3];
+    int *indices, *lengths_out;
+} needle2_evict_args;
+int needle2_evict_device(const needle2_evict_args *args, void *stream);
+
 /* ---- reference-compatible engine ABI (whole Needle-2 forward on the GPU) -- */
 /*
  * Layouts of needle2/csrc/engine.cpp:14-19 and :327-339 (bound from Python by

@@ -10,6 +10,9 @@ CUDA tensors and do not synchronise.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
+import struct
+from typing import NamedTuple
 
 import numpy as np
 
@@ -175,3 +178,288 @@ class KVCache:
         _check(self._lib.needle2_attention_prefill_device(self._handle, ids.ctypes.data, pos.ctypes.data, int(tokens),
                                                           q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                                           ids.size, _stream_ptr(stream)), "attention_prefill_device")
+
+
+# ---- stateless operators on caches that the caller owns ---------------------------
+#
+# These take torch CUDA tensors with any strides whose last axis is contiguous
+# (rows on 16-byte boundaries), run on torch's current stream or on `stream`
+# without synchronising, allocate through torch (results and workspace belong to
+# that stream, so captured graphs each keep their own) and have no gradients.
+
+# needle2_prefix_attention_args and needle2_evict_args, field by field
+_ATTENTION_ARGS = struct.Struct("@9i f P 3q P 3q 2P 6q 2P 6q 2P 4q 2P 4q 3P P P 3q P 3q")
+_EVICT_ARGS = struct.Struct("@9i 0q 2P 6q 2P 6q P 3q P 2P 6q 2P 6q P 3q 2P")
+_NO_STRIDES2, _NO_STRIDES3 = (0, 0), (0, 0, 0)
+
+
+class Evicted(NamedTuple):
+    """What ``evict`` leaves: the packed cache, and which keys stayed."""
+    k: object
+    v: object
+    weights: object
+    lengths: object
+    indices: object
+    k_scales: object = None
+    v_scales: object = None
+
+
+@functools.lru_cache(maxsize=1)
+def _bind_operators():
+    lib = _library()
+    lib.needle2_prefix_attention_workspace.argtypes = [ct.c_char_p]
+    lib.needle2_prefix_attention_workspace.restype = ct.c_longlong
+    lib.needle2_prefix_attention_device.argtypes = [ct.c_char_p, _p, ct.c_longlong, _p]
+    lib.needle2_prefix_attention_device.restype = _i
+    lib.needle2_evict_device.argtypes = [ct.c_char_p, _p]
+    lib.needle2_evict_device.restype = _i
+    import torch
+    types = {torch.int8: (0, torch.float32), torch.bfloat16: (1, torch.bfloat16), torch.float16: (2, torch.float16)}
+    return lib, torch, types
+
+
+def _on_stream(torch, device, stream):
+    """The context in which torch allocates and launches for `device` and `stream` (None: the current one)."""
+    if device.type != "cuda":
+        raise ValueError("the operators run on CUDA tensors")
+    if stream is None:
+        return torch.cuda.device(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = _stream_ptr(stream)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    if stream.device != device:
+        raise ValueError("the stream belongs to another device than the tensors")
+    return torch.cuda.stream(stream)
+
+
+def _want(x, name, shape, dtype, device, last=True):
+    if x.dtype != dtype or x.device != device or x.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}, got {x.dtype} "
+                         f"{tuple(x.shape)} on {x.device}")
+    if last and x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+
+
+def _span(x):
+    """First and past-the-last byte that a tensor's elements take."""
+    if not x.numel():
+        return 0, 0
+    a = x.data_ptr()
+    return a, a + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+
+
+def _apart(out, inputs, name):
+    """Refuse an output that shares memory with an input, or with itself."""
+    if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{name} must not be expanded")
+    a0, a1 = _span(out)
+    for x in inputs:
+        if x is not None:
+            b0, b1 = _span(x)
+            if a0 < b1 and b0 < a1:
+                raise ValueError(f"{name} overlaps an input")
+
+
+def _no_gradients(torch, *tensors):
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+        raise ValueError("these operators have no gradients: detach the inputs or call them under torch.no_grad()")
+
+
+def _cache_operands(torch, types, k, v, k_scales, v_scales, lead, keys, head_dim, name):
+    """Check K, V and their scales of a cache [*lead, keys, head_dim]; their pointers and strides."""
+    dtype, device, shape = k.dtype, k.device, (*lead, keys, head_dim)
+    _want(k, name + "k", shape, dtype, device)
+    _want(v, name + "v", shape, dtype, device)
+    if dtype == torch.int8:
+        if k_scales is None or v_scales is None:
+            raise ValueError(f"an INT8 cache needs {name}k_scales and {name}v_scales")
+        _want(k_scales, name + "k_scales", shape[:-1], torch.float32, device, last=False)
+        _want(v_scales, name + "v_scales", shape[:-1], torch.float32, device, last=False)
+        return (k.data_ptr(), v.data_ptr(), *k.stride()[:-1], *v.stride()[:-1],
+                k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(), *v_scales.stride())
+    if k_scales is not None or v_scales is not None:
+        raise ValueError(f"{name}k_scales and {name}v_scales belong to INT8 caches only")
+    return (k.data_ptr(), v.data_ptr(), *k.stride()[:-1], *v.stride()[:-1], 0, 0, *([0] * (2 * len(lead) + 2)))
+
+
+def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
+            prefix_v_scales, tokens, window, scale, out, return_lse, stream):
+    lib, torch, types = _bind_operators()
+    if k.dim() != 4 or k.dtype not in types:
+        raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
+    batch, kvheads, capacity, head_dim = k.shape
+    device = k.device
+    cache_type, qtype = types[k.dtype]
+    single = q.dim() == 3                              # one token per sequence
+    if q.dim() not in (3, 4):
+        raise ValueError("q must be [batch, tokens, heads, head_dim], or [batch, heads, head_dim] for one token")
+    q4 = q.unsqueeze(1) if single else q
+    count, heads = q4.shape[1], q4.shape[2]
+    _want(q4, "q", (batch, count, heads, head_dim), qtype, device)
+    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights)
+    own = _cache_operands(torch, types, k, v, k_scales, v_scales, (batch, kvheads), capacity, head_dim, "")
+    prefix = 0
+    shared = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    if (prefix_k is None) != (prefix_v is None):
+        raise ValueError("prefix_k and prefix_v go together")
+    if prefix_k is not None:
+        prefix = prefix_k.shape[1] if prefix_k.dim() == 3 else -1
+        if prefix_k.dtype != k.dtype or prefix_k.device != device or prefix < 0:
+            raise ValueError("prefix_k and prefix_v must be [kvheads, prefix, head_dim] of the cache's type and device")
+        shared = _cache_operands(torch, types, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales, (kvheads,),
+                                 prefix, head_dim, "prefix_")
+    elif prefix_k_scales is not None or prefix_v_scales is not None:
+        raise ValueError("prefix scales without a prefix")
+    _want(lengths, "lengths", (batch,), torch.int32, device)
+    if tokens is not None:
+        _want(tokens, "tokens", (batch,), torch.int32, device)
+    window = int(window)
+    if window < 0:
+        raise ValueError("window must not be negative")
+    window = 0 if window >= capacity else window
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if weights is not None:
+        _want(weights, "weights", (batch, kvheads, capacity), torch.float32, device, last=False)
+    if out is not None:
+        _want(out, "out", q.shape, qtype, device)
+        _apart(out, (q, k, v, prefix_k, prefix_v, lengths, tokens, weights, k_scales, v_scales, prefix_k_scales,
+                     prefix_v_scales, weights_out), "out")
+    if weights_out is not None:
+        _want(weights_out, "weights_out", (batch, kvheads, capacity), torch.float32, device, last=False)
+        same = weights_out.data_ptr() == weights.data_ptr() and weights_out.stride() == weights.stride()
+        _apart(weights_out, (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales,
+                             prefix_v_scales, None if same else weights), "weights_out")
+    with _on_stream(torch, device, stream):
+        if out is None:
+            out = torch.empty(q.shape, dtype=qtype, device=device)
+        lse = torch.empty((batch, count, heads), dtype=torch.float32, device=device) if return_lse else None
+        if weights is not None and weights_out is None:
+            weights_out = torch.empty((batch, kvheads, capacity), dtype=torch.float32, device=device)
+        weigh = weights is not None and capacity > 0
+        o = out.stride()
+        o3 = (o[0], 0, o[1]) if single else o[:3]
+        args = _ATTENTION_ARGS.pack(
+            batch, count, heads, kvheads, head_dim, prefix, capacity, window, cache_type, scale,
+            q4.data_ptr(), *q4.stride()[:3], out.data_ptr(), *o3, *own, *shared, lengths.data_ptr(),
+            0 if tokens is None else tokens.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
+            weights.data_ptr() if weigh else 0, *(weights.stride() if weigh else _NO_STRIDES3),
+            weights_out.data_ptr() if weigh else 0, *(weights_out.stride() if weigh else _NO_STRIDES3))
+        size = lib.needle2_prefix_attention_workspace(args)
+        if size < 0:
+            raise ValueError(last_error())
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _check(lib.needle2_prefix_attention_device(args, workspace.data_ptr() if size else None, size,
+                                                   torch.cuda.current_stream(device).cuda_stream),
+               "prefix_attention")
+    if return_lse and single:
+        lse = lse.squeeze(1)
+    return out, lse, weights_out
+
+
+def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, *, k_scales=None, v_scales=None,
+                     prefix_k_scales=None, prefix_v_scales=None, tokens=None, window=0, scale=None, out=None,
+                     return_lse=False, stream=None):
+    """Attention of a batch of sequences that share one prefix, whose part is
+    computed once for all of them.
+
+    ``q`` [batch, tokens, heads, head_dim] ([batch, heads, head_dim] for one
+    token each); ``k``, ``v`` [batch, kvheads, capacity, head_dim] the
+    sequences' own keys, of which sequence b has ``lengths[b]`` (int32), those of
+    the new tokens among them; ``prefix_k``, ``prefix_v`` [kvheads, prefix,
+    head_dim].  Caches are bfloat16 or float16 (q and the result too), or int8
+    with float32 scales [.., capacity] / [kvheads, prefix] (q and the result
+    float32).  head_dim is 64 or 128.
+
+    Token t of sequence b stands at own index ``lengths[b] - tokens[b] + t`` and
+    sees the whole prefix and its own keys up to there, the last ``window`` of
+    them if window > 0.  ``tokens`` (int32 [batch]) says how many of q's tokens a
+    sequence has; rows behind them are left as they were in ``out``.  A query
+    that sees nothing gets zeros.  With ``return_lse`` also the natural logarithm
+    of the softmax's denominators, float32 [batch, tokens, heads]."""
+    out, lse, _ = _attend(q, k, v, lengths, None, None, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
+                          prefix_v_scales, tokens, window, scale, out, return_lse, stream)
+    return (out, lse) if return_lse else out
+
+
+def accumulate_attention(q, k, v, lengths, weights, prefix_k=None, prefix_v=None, *, k_scales=None, v_scales=None,
+                         prefix_k_scales=None, prefix_v_scales=None, tokens=None, window=0, scale=None, out=None,
+                         weights_out=None, stream=None):
+    """``prefix_attention``, which also adds to each own key the softmax weights
+    that the call gave it: ``weights_out[b, g, j] = weights[b, g, j] + `` the sum
+    over the sequence's queries and the query heads of KV head g.  ``weights`` is
+    float32 [batch, kvheads, capacity]; ``weights_out`` may be ``weights``.
+    Returns (out, weights_out)."""
+    if weights is None:
+        raise ValueError("accumulate_attention needs weights")
+    out, _, weights_out = _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales,
+                                  prefix_k_scales, prefix_v_scales, tokens, window, scale, out, False, stream)
+    return out, weights_out
+
+
+def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_scales=None, out=None, in_place=False,
+          stream=None):
+    """Thin out a cache by the weights that ``accumulate_attention`` gathered.
+
+    Of a sequence's ``lengths[b]`` keys, ``keep`` stay per KV head where there
+    are more: the first ``first``, the last ``recent`` and, of those between
+    them, the ones of the largest weight (the lower index of equal ones, NaN
+    last).  They are packed in their order into the front of the result, an
+    ``Evicted`` of k, v, weights [batch, kvheads, n, ..], lengths, indices
+    [batch, kvheads, keep] (-1 behind the kept) and an INT8 cache's scales.
+    Slots behind the kept keys have weight 0 and otherwise stay as they were.
+
+    The result goes to ``out`` (an ``Evicted`` of tensors with n >= keep slots),
+    to the inputs themselves (``in_place``; lengths and indices are new), or to
+    new tensors of ``keep`` slots, zero behind the kept keys."""
+    lib, torch, types = _bind_operators()
+    if k.dim() != 4 or k.dtype not in types:
+        raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
+    batch, kvheads, capacity, head_dim = k.shape
+    device, keep, first, recent = k.device, int(keep), int(first), int(recent)
+    if keep < 0 or first < 0 or recent < 0 or first + recent > keep:
+        raise ValueError("first and recent must not be negative, nor exceed keep together")
+    _no_gradients(torch, k, v, weights)
+    cache = _cache_operands(torch, types, k, v, k_scales, v_scales, (batch, kvheads), capacity, head_dim, "")
+    _want(weights, "weights", (batch, kvheads, capacity), torch.float32, device, last=False)
+    _want(lengths, "lengths", (batch,), torch.int32, device)
+    int8 = k.dtype == torch.int8
+    with _on_stream(torch, device, stream):
+        if in_place:
+            if out is not None:
+                raise ValueError("evict: out and in_place exclude each other")
+            if keep > capacity:
+                raise ValueError("evict: in place, keep must not exceed the capacity")
+            for x in (k, v, weights, k_scales, v_scales):
+                if x is not None:
+                    _apart(x, [y for y in (k, v, weights, lengths, k_scales, v_scales) if y is not x], "the cache")
+            out = Evicted(k, v, weights, torch.empty(batch, dtype=torch.int32, device=device),
+                          torch.empty((batch, kvheads, keep), dtype=torch.int32, device=device), k_scales, v_scales)
+        elif out is None:
+            shape = (batch, kvheads, keep)
+            f32 = {"dtype": torch.float32, "device": device}
+            out = Evicted(torch.zeros((*shape, head_dim), dtype=k.dtype, device=device),
+                          torch.zeros((*shape, head_dim), dtype=k.dtype, device=device), torch.empty(shape, **f32),
+                          torch.empty(batch, dtype=torch.int32, device=device),
+                          torch.empty(shape, dtype=torch.int32, device=device),
+                          torch.zeros(shape, **f32) if int8 else None, torch.zeros(shape, **f32) if int8 else None)
+        else:
+            out = Evicted(*out)
+            if out.k.dim() != 4 or out.k.shape[2] < keep or out.k.dtype != k.dtype or out.k.device != device:
+                raise ValueError("evict: out.k must be a cache of the input's type with at least keep slots")
+            _want(out.weights, "out.weights", (batch, kvheads, out.k.shape[2]), torch.float32, device, last=False)
+            _want(out.lengths, "out.lengths", (batch,), torch.int32, device)
+            _want(out.indices, "out.indices", (batch, kvheads, keep), torch.int32, device)
+            if not out.indices.is_contiguous():
+                raise ValueError("out.indices must be contiguous")
+            outs = [x for x in out if x is not None]
+            for i, x in enumerate(outs):
+                _apart(x, [k, v, weights, lengths, k_scales, v_scales, *outs[:i]], "out")
+        slots = out.k.shape[2]
+        packed = _cache_operands(torch, types, out.k, out.v, out.k_scales, out.v_scales, (batch, kvheads), slots,
+                                 head_dim, "out.")
+        args = _EVICT_ARGS.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
+                                *cache, weights.data_ptr(), *weights.stride(), lengths.data_ptr(), *packed,
+                                out.weights.data_ptr(), *out.weights.stride(), out.indices.data_ptr(),
+                                out.lengths.data_ptr())
+        _check(lib.needle2_evict_device(args, torch.cuda.current_stream(device).cuda_stream), "evict")
+    return out

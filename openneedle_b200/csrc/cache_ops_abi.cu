@@ -1,0 +1,266 @@
+// C ABI of the stateless cache operators: attention behind a shared prefix,
+// accumulated key weights, eviction.  Argument checks, the split of the work
+// into key ranges, and the workspace.
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <initializer_list>
+#include <string>
+
+#include "../../include/needle2_b200.h"
+#include "common.cuh"
+#include "evict.cuh"
+#include "prefix_attention.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr long long kMaxUnits = 0x7fffffff;
+
+bool refuse(const char *msg) {
+    set_error(msg);
+    return false;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Pointer and strides (of axes longer than one) of rows read 16 bytes at a time.
+bool rows_ok(const void *p, const long long *stride, std::initializer_list<int> extent, int size, const char *what) {
+    if (!p) return refuse((std::string(what) + " is null").c_str());
+    bool ok = aligned16(p);
+    for (int n : extent) ok = ok && (n <= 1 || (*stride * size) % 16 == 0), ++stride;
+    return ok ? true : refuse((std::string(what) + ": the pointer and the strides must be multiples of 16 bytes").c_str());
+}
+
+bool sizes_ok(const needle2_prefix_attention_args &a) {
+    if (a.batch < 0 || a.tokens < 0 || a.heads < 1 || a.kvheads < 1 || a.prefix < 0 || a.capacity < 0 || a.window < 0)
+        return refuse("prefix attention: negative size");
+    if (a.heads % a.kvheads) return refuse("prefix attention: heads must be a multiple of kvheads");
+    if (a.head_dim != 64 && a.head_dim != 128) return refuse("prefix attention: head_dim must be 64 or 128");
+    if (a.cache_type < 0 || a.cache_type > 2) return refuse("prefix attention: unknown cache type");
+    if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return refuse("prefix attention: scale must be positive and finite");
+    const long long rows = (long long)a.batch * a.tokens;
+    // units of work and row numbers are 32-bit
+    if (rows * a.heads > kMaxUnits / 64 || (long long)a.batch * a.kvheads > kMaxUnits / 64 ||
+        (long long)a.batch * a.kvheads * ((a.capacity + 63) / 64) > kMaxUnits || a.capacity > 0x7fffff00 ||
+        a.prefix > 0x7fffff00)
+        return refuse("prefix attention: the call is too large");
+    return true;
+}
+
+constexpr int kLogitRows = 16;   // query rows of a KV head up to which logits are kept for the weights
+
+struct Plan {
+    int prefix_slots, own_slots;
+    bool logits, row_lse;
+    long long part_o, part_lse, row_lse_at, logits_at, bytes;
+};
+
+int sm_count() {
+    static int count[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < 0 || dev >= 64) return 148;
+    if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        count[dev] = 148;
+    return count[dev];
+}
+
+Plan plan_of(const needle2_prefix_attention_args &a) {
+    Plan p{};
+    const int sms = sm_count();
+    const int R = a.heads / a.kvheads, tile = a.cache_type == kCacheI8 ? 8 : 16;
+    const long long rows = (long long)a.batch * a.tokens * a.heads;
+    auto slots = [&](long long units, int keys) {
+        const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
+        return (int)std::max(1LL, std::min({want, (long long)(keys + 127) / 128, 64LL}));
+    };
+    const long long own_units = (long long)a.batch * a.kvheads * ((a.tokens * R + tile - 1) / tile);
+    const long long prefix_units = (long long)a.kvheads * (((long long)a.batch * a.tokens * R + tile - 1) / tile);
+    const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
+    p.own_slots = a.capacity || !a.prefix ? slots(own_units, span) : 0;
+    p.prefix_slots = a.prefix ? slots(prefix_units, a.prefix) : 0;
+    p.logits = a.weights && a.tokens > 0 && a.tokens * R <= kLogitRows;
+    p.row_lse = a.weights != nullptr;
+    long long at = 0;
+    auto take = [&](long long bytes) {
+        const long long r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    const int n = p.own_slots + p.prefix_slots;
+    if (n > 1) {
+        p.part_o = take(rows * n * a.head_dim * 4);
+        p.part_lse = take(rows * n * 4);
+    }
+    if (p.row_lse) p.row_lse_at = take(rows * 4);
+    if (p.logits) p.logits_at = take((long long)a.batch * a.kvheads * a.tokens * R * a.capacity * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <int N>
+void copy(long long (&to)[N], const long long (&from)[N]) {
+    for (int i = 0; i < N; ++i) to[i] = from[i];
+}
+
+bool attention(const needle2_prefix_attention_args &a, void *workspace, long long bytes, cudaStream_t st) {
+    if (!sizes_ok(a)) return false;
+    if (a.batch == 0) return true;
+    const int size = a.cache_type == kCacheI8 ? 1 : 2, qsize = a.cache_type == kCacheI8 ? 4 : 2;
+    const bool i8 = a.cache_type == kCacheI8;
+    if (a.tokens > 0) {
+        if (!rows_ok(a.q, a.q_stride, {a.batch, a.tokens, a.heads}, qsize, "q") ||
+            !rows_ok(a.out, a.out_stride, {a.batch, a.tokens, a.heads}, qsize, "out"))
+            return false;
+    }
+    if (a.capacity) {
+        // (with cache_rows the first axis is the cache's, which this call does not know)
+        const int lead = a.cache_rows ? 2 : a.batch;
+        if (!rows_ok(a.k, a.k_stride, {lead, a.kvheads, a.capacity}, size, "k") ||
+            !rows_ok(a.v, a.v_stride, {lead, a.kvheads, a.capacity}, size, "v"))
+            return false;
+        if (i8 && (!a.k_scales || !a.v_scales)) return refuse("an INT8 cache needs its scales");
+    }
+    if (a.prefix) {
+        if (!rows_ok(a.prefix_k, a.prefix_k_stride, {a.kvheads, a.prefix}, size, "prefix_k") ||
+            !rows_ok(a.prefix_v, a.prefix_v_stride, {a.kvheads, a.prefix}, size, "prefix_v"))
+            return false;
+        if (i8 && (!a.prefix_k_scales || !a.prefix_v_scales)) return refuse("an INT8 prefix needs its scales");
+    }
+    if (!a.lengths) return refuse("lengths is null");
+    if ((a.weights != nullptr) != (a.weights_out != nullptr))
+        return refuse("weights and weights_out go together");
+    const Plan plan = plan_of(a);
+    if (bytes < plan.bytes || (plan.bytes && (!workspace || !aligned16(workspace))))
+        return refuse("prefix attention: the workspace is too small or not 16-byte aligned");
+    PrefixAttn p{};
+    p.batch = a.batch; p.tokens = a.tokens; p.heads = a.heads; p.kvheads = a.kvheads;
+    p.group = a.heads / a.kvheads; p.hd = a.head_dim;
+    p.prefix = a.prefix; p.capacity = a.capacity; p.type = a.cache_type;
+    p.window = a.window >= a.capacity ? 0 : a.window;   // own indexes are below the capacity
+    p.scale2 = a.scale * 1.4426950408889634f;
+    p.q = a.q; p.out = a.out; p.k = a.k; p.v = a.v; p.pk = a.prefix_k; p.pv = a.prefix_v;
+    p.kscale = a.k_scales; p.vscale = a.v_scales; p.pkscale = a.prefix_k_scales; p.pvscale = a.prefix_v_scales;
+    copy(p.qs, a.q_stride); copy(p.os, a.out_stride); copy(p.ks, a.k_stride); copy(p.vs, a.v_stride);
+    copy(p.kss, a.k_scale_stride); copy(p.vss, a.v_scale_stride);
+    copy(p.pks, a.prefix_k_stride); copy(p.pvs, a.prefix_v_stride);
+    copy(p.pkss, a.prefix_k_scale_stride); copy(p.pvss, a.prefix_v_scale_stride);
+    p.lengths = a.lengths; p.ntokens = a.token_counts; p.cache_row = a.cache_rows;
+    p.lse = a.lse;
+    p.weights = a.weights; p.weights_out = a.weights_out;
+    copy(p.ws, a.weights_stride); copy(p.wos, a.weights_out_stride);
+    p.prefix_slots = plan.prefix_slots;
+    p.own_slots = plan.own_slots;
+    char *base = static_cast<char *>(workspace);
+    const int n = plan.own_slots + plan.prefix_slots;
+    if (n > 1) {
+        p.part_o = reinterpret_cast<float *>(base + plan.part_o);
+        p.part_lse = reinterpret_cast<float *>(base + plan.part_lse);
+    }
+    if (plan.row_lse) p.row_lse = reinterpret_cast<float *>(base + plan.row_lse_at);
+    if (plan.logits) p.logits = reinterpret_cast<float *>(base + plan.logits_at);
+    if (a.tokens > 0 && !launch_prefix_stream(p, plan.prefix_slots > 0, plan.own_slots > 0, st)) return false;
+    if (!launch_prefix_finish(p, st)) return false;
+    return !a.weights || plan.logits || launch_key_weights(p, st);
+}
+
+bool evict(const needle2_evict_args &a, cudaStream_t st) {
+    if (a.batch < 0 || a.kvheads < 1 || a.capacity < 0 || a.keep < 0 || a.first < 0 || a.recent < 0)
+        return refuse("evict: negative size");
+    if (a.head_dim != 64 && a.head_dim != 128) return refuse("evict: head_dim must be 64 or 128");
+    if (a.cache_type < 0 || a.cache_type > 2) return refuse("evict: unknown cache type");
+    if ((long long)a.first + a.recent > a.keep) return refuse("evict: first + recent must not exceed keep");
+    if (a.out_capacity < a.keep) return refuse("evict: the output holds fewer than keep slots");
+    if ((long long)a.batch * a.kvheads > kMaxUnits / 64 ||
+        (long long)a.batch * a.kvheads * ((a.keep + 15) / 16) > kMaxUnits || a.capacity > 0x7fffff00 ||
+        a.out_capacity > 0x7fffff00)
+        return refuse("evict: the call is too large");
+    if (a.batch == 0) return true;
+    const int size = a.cache_type == kCacheI8 ? 1 : 2;
+    if (!a.lengths || !a.lengths_out || (a.keep && !a.indices)) return refuse("evict: null pointer");
+    if (a.lengths == a.lengths_out) return refuse("evict: lengths_out must not be lengths");
+    if (a.capacity && (!rows_ok(a.k, a.k_stride, {a.batch, a.kvheads, a.capacity}, size, "k") || !rows_ok(a.v, a.v_stride, {a.batch, a.kvheads, a.capacity}, size, "v") || !a.weights))
+        return a.weights ? false : refuse("evict: weights is null");
+    if (a.out_capacity && (!rows_ok(a.k_out, a.k_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "k_out") ||
+                           !rows_ok(a.v_out, a.v_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "v_out") || !a.weights_out))
+        return a.weights_out ? false : refuse("evict: weights_out is null");
+    const bool i8 = a.cache_type == kCacheI8;
+    if (i8 && ((a.capacity && (!a.k_scales || !a.v_scales)) ||
+               (a.out_capacity && (!a.k_scales_out || !a.v_scales_out))))
+        return refuse("evict: an INT8 cache needs its scales");
+    auto same = [](const long long *x, const long long *y) { return x[0] == y[0] && x[1] == y[1] && x[2] == y[2]; };
+    const bool in_place = a.k == a.k_out;
+    if (in_place && a.capacity) {
+        bool ok = a.v == a.v_out && a.weights == a.weights_out && a.out_capacity == a.capacity &&
+                  same(a.k_stride, a.k_out_stride) && same(a.v_stride, a.v_out_stride) &&
+                  same(a.weights_stride, a.weights_out_stride);
+        if (i8)
+            ok = ok && a.k_scales == a.k_scales_out && a.v_scales == a.v_scales_out &&
+                 same(a.k_scale_stride, a.k_scale_out_stride) && same(a.v_scale_stride, a.v_scale_out_stride);
+        if (!ok) return refuse("evict: in place, every output must be its input");
+    }
+    Evict e{};
+    e.batch = a.batch; e.kvheads = a.kvheads; e.capacity = a.capacity; e.out_capacity = a.out_capacity;
+    e.keep = a.keep; e.first = a.first; e.recent = a.recent;
+    e.row_bytes = a.head_dim * size;
+    e.k = (const char *)a.k; e.v = (const char *)a.v; e.ko = (char *)a.k_out; e.vo = (char *)a.v_out;
+    for (int i = 0; i < 3; ++i) {
+        e.ks[i] = a.k_stride[i] * size; e.vs[i] = a.v_stride[i] * size;
+        e.kos[i] = a.k_out_stride[i] * size; e.vos[i] = a.v_out_stride[i] * size;
+    }
+    if (i8) {
+        e.kscale = a.k_scales; e.vscale = a.v_scales; e.kscale_o = a.k_scales_out; e.vscale_o = a.v_scales_out;
+    }
+    copy(e.kss, a.k_scale_stride); copy(e.vss, a.v_scale_stride);
+    copy(e.ksos, a.k_scale_out_stride); copy(e.vsos, a.v_scale_out_stride);
+    e.weights = a.weights; e.weights_o = a.weights_out;
+    copy(e.ws, a.weights_stride); copy(e.wos, a.weights_out_stride);
+    e.lengths = a.lengths; e.lengths_o = a.lengths_out; e.indices = a.indices;
+    e.in_place = in_place;
+    return launch_evict(e, st);
+}
+
+}  // namespace
+}  // namespace nb200
+
+namespace {
+
+// No exception leaves a C entry.
+template <typename F>
+long long entry(const void *args, F f) {
+    nb200::clear_error();
+    if (!args) {
+        nb200::set_error("null arguments");
+        return -1;
+    }
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        nb200::set_error(e.what());
+    }
+    return -1;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long needle2_prefix_attention_workspace(const needle2_prefix_attention_args *args) {
+    return entry(args, [&]() -> long long { return nb200::sizes_ok(*args) ? nb200::plan_of(*args).bytes : -1; });
+}
+
+int needle2_prefix_attention_device(const needle2_prefix_attention_args *args, void *workspace,
+                                    long long workspace_bytes, void *stream) {
+    return (int)entry(args, [&]() -> long long {
+        return nb200::attention(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? 0 : -1;
+    });
+}
+
+int needle2_evict_device(const needle2_evict_args *args, void *stream) {
+    return (int)entry(args, [&]() -> long long {
+        return nb200::evict(*args, static_cast<cudaStream_t>(stream)) ? 0 : -1;
+    });
+}
+
+}  // extern "C"

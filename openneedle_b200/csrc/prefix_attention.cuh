@@ -1,0 +1,70 @@
+// Attention of a batch that shares a prefix, over caches of INT8 rows with FP32
+// scales or of 16-bit values, and the softmax weights its own keys receive:
+// parameters and launches shared by prefix_attention.cu (streaming kernel for
+// few rows, the merge of partial results, key weights), prefix_attention_tc.cu
+// (tcgen05 tiles for many rows) and the C ABI.
+//
+// Rows.  For one KV head, row m = (b * tokens + t) * R + r stands for query
+// token t of sequence b and query head g * R + r (R = heads / kvheads).  The
+// prefix takes all B * tokens * R rows as one matrix; a sequence's own keys
+// take its tokens * R consecutive rows.
+//
+// Partial results.  Disjoint key ranges of one row are attended separately;
+// each yields o = sum_j e^(z_j - lse) v_j and lse = log2 sum_j 2^(z_j) over its
+// range (z in log2 units; -inf and unwritten o for an empty range), and
+// out = sum_i 2^(lse_i - L) o_i with L = log2 sum_i 2^(lse_i).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace nb200 {
+
+enum CacheType { kCacheI8 = 0, kCacheBF16 = 1, kCacheF16 = 2 };
+
+struct PrefixAttn {
+    int batch, tokens, heads, kvheads, group, hd;   // group = heads / kvheads
+    int prefix, capacity, window, type;
+    float scale2;                                    // softmax scale * log2(e)
+    const void *q;                                   // f32 (INT8 cache) or the cache's type
+    long long qs[3];                                 // strides in elements: batch, token, head
+    void *out;
+    long long os[3];
+    const void *k, *v;
+    long long ks[3], vs[3];                          // batch, KV head, key
+    const float *kscale, *vscale;
+    long long kss[3], vss[3];
+    const void *pk, *pv;
+    long long pks[2], pvs[2];                        // KV head, key
+    const float *pkscale, *pvscale;
+    long long pkss[2], pvss[2];
+    const int *lengths;                              // own keys of each sequence, the new tokens' among them
+    const int *ntokens;                              // queries of each sequence (null: `tokens`)
+    const int *cache_row;                            // row of k, v and scales of each sequence (null: its own index)
+    float *lse;                                      // [B][tokens][heads], natural log (null: not written)
+    const float *weights;
+    long long ws[3];
+    float *weights_out;
+    long long wos[3];
+    // partial results, in the caller's workspace
+    int prefix_slots, own_slots;                     // key ranges of the prefix and of the own keys
+    float *part_o;                                   // [slots][rows][hd], rows = B * tokens * heads as out's
+    float *part_lse;                                 // [slots][rows]
+    float *row_lse;                                  // [rows], log2 (null: not needed)
+    float *logits;                                   // [B * kvheads][tokens * R][capacity], log2 (null: not kept)
+};
+
+__device__ __forceinline__ int own_length(const PrefixAttn &p, int b) {
+    return max(0, min(p.lengths[b], p.capacity));
+}
+__device__ __forceinline__ int own_tokens(const PrefixAttn &p, int b) {
+    return p.ntokens ? max(0, min(p.ntokens[b], p.tokens)) : p.tokens;
+}
+
+// The merge of the partial results, weights of few rows from kept logits, and
+// weights of any number of rows from row_lse.
+bool launch_prefix_finish(const PrefixAttn &p, cudaStream_t st);
+bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
+// Streaming kernel: `prefix` / `own` say which key sets it takes.
+bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream_t st);
+
+}  // namespace nb200

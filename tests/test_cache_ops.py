@@ -1,0 +1,158 @@
+"""The cache operators' argument checks (CPU only): what the Python entry points
+refuse before they touch a GPU, and the C ABI's own refusals."""
+import ctypes as ct
+
+import pytest
+import torch
+
+import cache_ops_reference as R
+from openneedle_b200 import attention, build
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    build.build()
+
+
+def inputs(cache="int8", t=1):
+    return R.make_inputs(cache, 2, t, 8, 4, 64, 20, 30, [30, 10])
+
+
+def attend(c, weigh=False, **more):
+    args = {n: c.get(n) for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales",
+                                  "prefix_v_scales")}
+    args.update(more)
+    if weigh:
+        return attention.accumulate_attention(c["q"], c["k"], c["v"], c["lengths"], c["weights"], **args)
+    return attention.prefix_attention(c["q"], c["k"], c["v"], c["lengths"], **args)
+
+
+def evict(c, keep=8, **more):
+    return attention.evict(c["k"], c["v"], c["weights"], c["lengths"], keep,
+                           **{"k_scales": c["k_scales"], "v_scales": c["v_scales"], **more})
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"q": lambda x: x.half()}, "q must be"),
+    ({"q": lambda x: x[:1]}, "q must be"),
+    ({"q": lambda x: x[0, 0]}, "q must be"),
+    ({"q": lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)}, "last axis"),
+    ({"k": lambda x: x.int()}, "int8, bfloat16 or float16"),
+    ({"k": lambda x: x[0]}, "int8, bfloat16 or float16"),
+    ({"v": lambda x: x[:, :, :-1]}, "v must be"),
+    ({"k_scales": lambda x: None}, "needs k_scales"),
+    ({"v_scales": lambda x: x.double()}, "v_scales must be"),
+    ({"prefix_k": lambda x: None}, "go together"),
+    ({"prefix_k": lambda x: x.half()}, "prefix_k and prefix_v must be"),
+    ({"prefix_v": lambda x: x[:, :5]}, "prefix_v must be"),
+    ({"prefix_v_scales": lambda x: None}, "needs prefix_k_scales"),
+    ({"lengths": lambda x: x.long()}, "lengths must be"),
+    ({"weights": lambda x: x[:, :, :3]}, "weights must be"),
+    ({"weights": lambda x: None}, "needs weights"),
+    ({"q": lambda x: x.requires_grad_()}, "no gradients"),
+    ({}, "CUDA tensors")])
+def test_attention_refuses(change, message):
+    c = inputs()
+    for n, f in change.items():
+        c[n] = f(c[n])
+    with pytest.raises(ValueError, match=message):
+        attend(c, weigh=True)
+
+
+@pytest.mark.parametrize("more,message", [
+    ({"window": -1}, "window"),
+    ({"tokens": torch.zeros(3, dtype=torch.int32)}, "tokens must be"),
+    ({"out": torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16)}, "out must be"),
+    ({"out": torch.zeros(2, 1, 1, 64).expand(2, 1, 8, 64)}, "expanded"),
+    ({"weights_out": torch.zeros(2, 4, 29)}, "weights_out must be")])
+def test_attention_refuses_options(more, message):
+    with pytest.raises(ValueError, match=message):
+        attend(inputs(), weigh=True, **more)
+
+
+def test_outputs_must_not_overlap_inputs():
+    c = inputs()
+    with pytest.raises(ValueError, match="out overlaps"):
+        attend(c, out=c["q"])
+    with pytest.raises(ValueError, match="weights_out overlaps"):
+        whole = torch.zeros(2, 5, 30)
+        c["weights"] = whole[:, :4]
+        attend(c, weigh=True, weights_out=whole[:, 1:])
+    c = inputs("bf16")
+    with pytest.raises(ValueError, match="scales belong to INT8"):
+        attend(c, k_scales=torch.zeros(2, 4, 30), v_scales=torch.zeros(2, 4, 30))
+    c = inputs()
+    e = attention.Evicted(c["k"][:, :, :8], c["v"], c["weights"], c["lengths"], None)
+    with pytest.raises(ValueError):
+        evict(c, out=e)
+
+
+@pytest.mark.parametrize("more,message", [
+    ({"keep": -1}, "must not"), ({"first": 5, "recent": 4}, "exceed keep"), ({"first": -1}, "must not"),
+    ({"in_place": True, "out": ()}, "exclude"), ({"in_place": True, "keep": 31}, "capacity"),
+    ({"k_scales": None}, "needs k_scales"), ({}, "CUDA tensors")])
+def test_evict_refuses(more, message):
+    if message in ("exclude", "capacity"):
+        if not torch.cuda.is_available():
+            message = "CUDA tensors"                        # (the stream's device is looked at first)
+    with pytest.raises(ValueError, match=message):
+        evict(inputs(), **{"keep": 8, **more})
+
+
+# ---- the C ABI ------------------------------------------------------------------
+
+def pack(**change):
+    """A valid call of two sequences on an INT8 cache; addresses that nothing reads."""
+    a = dict(batch=2, tokens=1, heads=8, kvheads=4, head_dim=64, prefix=16, capacity=32, window=0, cache_type=0,
+             scale=0.125, q=4096, out=8192, k=4096, v=4096, ks=4096, vs=4096, pk=4096, pv=4096, pks=4096, pvs=4096,
+             lengths=4096, counts=0, rows=0, lse=0, weights=0, weights_out=0, kstride=64)
+    a.update(change)
+    return attention._ATTENTION_ARGS.pack(
+        a["batch"], a["tokens"], a["heads"], a["kvheads"], a["head_dim"], a["prefix"], a["capacity"], a["window"],
+        a["cache_type"], a["scale"], a["q"], 512, 512, 64, a["out"], 512, 512, 64,
+        a["k"], a["v"], 8192, 2048, a["kstride"], 8192, 2048, 64, a["ks"], a["vs"], 128, 32, 1, 128, 32, 1,
+        a["pk"], a["pv"], 1024, 64, 1024, 64, a["pks"], a["pvs"], 16, 1, 16, 1,
+        a["lengths"], a["counts"], a["rows"], a["lse"], a["weights"], 128, 32, 1, a["weights_out"], 128, 32, 1)
+
+
+def test_workspace_grows_with_what_is_asked():
+    lib = attention._bind_operators()[0]
+    plain = lib.needle2_prefix_attention_workspace(pack())
+    assert 0 < plain < lib.needle2_prefix_attention_workspace(pack(weights=4096, weights_out=4096))
+    assert lib.needle2_prefix_attention_workspace(pack(batch=0)) >= 0
+    assert lib.needle2_prefix_attention_workspace(None) == -1
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"batch": -1}, "negative size"), ({"tokens": -1}, "negative size"), ({"prefix": -1}, "negative size"),
+    ({"capacity": -1}, "negative size"), ({"window": -2}, "negative size"), ({"kvheads": 0}, "negative size"),
+    ({"heads": 6}, "multiple of kvheads"), ({"head_dim": 96}, "head_dim"), ({"cache_type": 3}, "cache type"),
+    ({"scale": 0.0}, "scale"), ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"),
+    ({"batch": 1 << 30}, "too large"), ({"tokens": 1 << 28}, "too large"),
+    ({"q": 0}, "q is null"), ({"q": 4104}, "q: the pointer"), ({"out": 4100}, "out: the pointer"),
+    ({"k": 4097}, "k: the pointer"), ({"kstride": 72}, "k: the pointer"), ({"v": 0}, "v is null"),
+    ({"ks": 0}, "needs its scales"), ({"pks": 0}, "needs its scales"), ({"pv": 0}, "prefix_v is null"),
+    ({"lengths": 0}, "lengths is null"), ({"weights": 4096}, "go together"), ({}, "workspace")])
+def test_c_abi_refuses(change, message):
+    lib = attention._bind_operators()[0]
+    assert lib.needle2_prefix_attention_device(pack(**change), None, 0, None) == -1
+    assert message in attention.last_error()
+
+
+@pytest.mark.parametrize("index,value,message", [
+    (0, -1, "negative size"), (2, 80, "head_dim"), (8, 7, "cache type"), (5, 3, "exceed keep"), (4, 7, "fewer than keep"),
+    (9, 0, "k is null"), (9, 4100, "multiples of 16"), (13, 72, "multiples of 16"), (17, 0, "needs its scales"),
+    (25, 0, "weights is null"), (29, 0, "null pointer"), (29, 65536, "must not be lengths"), (30, 4096, "in place")])
+def test_c_abi_refuses_evictions(index, value, message):
+    lib = attention._bind_operators()[0]
+    three = (8192, 2048, 64)
+    flat = (128, 32, 1)
+    a = [2, 4, 64, 32, 32, 8, 2, 2, 0, 4096, 4096, *three, *three, 4096, 4096, *flat, *flat, 4096, *flat, 4096,
+         16384, 16384, *three, *three, 16384, 16384, *flat, *flat, 16384, *flat, 16384, 65536]
+    if message == "must not be lengths":
+        a[29] = a[-1]
+    else:
+        a[index] = value
+    assert lib.needle2_evict_device(attention._EVICT_ARGS.pack(*a), None) == -1
+    assert message in attention.last_error()
+    assert lib.needle2_evict_device(None, None) == -1

@@ -1,0 +1,398 @@
+"""Attention behind a shared prefix, accumulated key weights and eviction on the
+GPU against their definitions in 64 bits (cache_ops_reference.py, whose bounds
+follow from the roundings of each step)."""
+import math
+
+import pytest
+import torch
+
+import cache_ops_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from openneedle_b200 import attention, build
+    build.build()
+    return attention
+
+
+def cuda(c):
+    return {n: None if x is None else x.cuda() for n, x in c.items()}
+
+
+def call(ops, c, weigh=False, **more):
+    d = cuda(c)
+    args = {n: d.get(n) for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales",
+                                  "prefix_v_scales")}
+    if weigh:
+        return ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], **args, **more)
+    return ops.prefix_attention(d["q"], d["k"], d["v"], d["lengths"], return_lse=True, **args, **more)
+
+
+def both(ops, c, **more):
+    """out and lse of prefix_attention and out and weights of accumulate_attention within their bounds."""
+    ref = R.attention(c, **{n: x for n, x in more.items() if n in ("window", "scale")})
+    bound = R.bounds(c, ref)
+    out, lse = call(ops, c, **more)
+    R.check(out, ref["out"], bound["out"], "out")
+    R.check(lse, ref["lse"], bound["lse"], "lse")
+    out2, weights = call(ops, c, weigh=True, **more)
+    R.check(out2, ref["out"], bound["out"], "out of accumulate_attention")
+    R.check(weights, ref["weights"], bound["weights"], "weights")
+    return out, lse, weights
+
+
+CACHES = ("int8", "bf16", "f16")
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("d", (64, 128))
+@pytest.mark.parametrize("b,heads,kv,p,s,lengths", [
+    (1, 8, 4, 0, 1, [1]),                                   # one key
+    (1, 8, 4, 1, 1, [0]),                                   # one prefix key, no own
+    (3, 8, 4, 48, 64, [17, 0, 64]),
+    (2, 4, 1, 33, 97, [97, 50]),                            # one KV head
+    (2, 16, 2, 130, 31, [31, 1]),                           # eight query heads a KV head
+    (5, 6, 6, 257, 200, [200, 33, 0, 1, 129]),              # one query head a KV head
+    (40, 8, 4, 300, 40, [(7 * i) % 41 for i in range(40)]),  # more prefix rows than one tile
+    (1, 32, 1, 70, 90, [90])])                              # more query heads than a tile's rows
+def test_one_token(ops, cache, d, b, heads, kv, p, s, lengths):
+    both(ops, R.make_inputs(cache, b, 1, heads, kv, d, p, s, lengths, seed=b + p))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("d", (64, 128))
+@pytest.mark.parametrize("b,t,heads,kv,p,s,lengths,window", [
+    (2, 2, 8, 4, 5, 20, [20, 2], 0),
+    (2, 7, 4, 2, 0, 40, [40, 9], 0),
+    (1, 33, 8, 4, 65, 150, [150], 0),
+    (2, 33, 8, 4, 65, 150, [150, 33], 16),
+    (2, 5, 4, 4, 3, 50, [50, 3], 4),                        # fewer own keys than tokens: the first see the prefix only
+    (2, 5, 4, 4, 0, 50, [50, 3], 4),                        # ... or nothing
+    (1, 150, 2, 1, 0, 150, [150], 0),
+    (1, 140, 3, 1, 129, 300, [300], 37),
+    (2, 1, 8, 4, 17, 70, [70, 20], 16),                     # decode in a window
+    (2, 1, 8, 4, 17, 70, [70, 20], 1)])
+def test_several_tokens(ops, cache, d, b, t, heads, kv, p, s, lengths, window):
+    both(ops, R.make_inputs(cache, b, t, heads, kv, d, p, s, lengths, seed=t + p), window=window)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_rows_that_see_nothing(ops, cache):
+    c = R.make_inputs(cache, 3, 1, 8, 4, 64, 0, 16, [0, 5, 0])
+    out, lse, weights = both(ops, c)
+    assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and (out[2] == 0).all()
+    assert torch.equal(weights[0].cpu(), c["weights"][0])
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t", (1, 40))
+def test_padded_tokens_are_left_alone(ops, cache, t):
+    c = R.make_inputs(cache, 4, t, 8, 4, 64, 20, 80, [80, 70, 60, 50], seed=9)
+    tokens = torch.tensor([t, 0, t // 2, 1], dtype=torch.int32)
+    c["q"][3, 1:] = math.nan
+    ref = R.attention(c, tokens=tokens)
+    bound = R.bounds(c, {n: x.nan_to_num() for n, x in ref.items()})
+    out = torch.full_like(c["q"].nan_to_num(), 7.0).cuda()
+    call(ops, c, tokens=tokens.cuda(), out=out)
+    for i in range(4):
+        n = int(tokens[i])
+        R.check(out[i, :n], ref["out"][i, :n], bound["out"][i, :n], "out")
+        assert (out[i, n:] == 7.0).all()
+    out2 = torch.full_like(out, 7.0)
+    _, weights = call(ops, c, weigh=True, tokens=tokens.cuda(), out=out2)
+    assert torch.equal(out2, out)
+    R.check(weights, ref["weights"], bound["weights"].nan_to_num(), "weights")
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t", (1, 40))
+def test_what_lies_behind_the_length_is_not_used(ops, cache, t):
+    lengths = [t + 3, t, 90]
+    c = R.make_inputs(cache, 3, t, 8, 4, 128, 50, 100, lengths, seed=3)
+    clean = call(ops, c)
+    clean_w = call(ops, c, weigh=True)
+    for i, n in enumerate(lengths):
+        if cache == "int8":
+            c["k_scales"][i, :, n:] = math.nan
+            c["v_scales"][i, :, n:] = math.inf
+        else:
+            c["k"][i, :, n:] = math.nan
+            c["v"][i, :, n:] = math.inf
+    for x, y in zip(clean + clean_w, call(ops, c) + call(ops, c, weigh=True)):
+        assert torch.equal(x, y)
+    # ... nor before every query's window
+    c = R.make_inputs(cache, 1, t, 8, 4, 128, 50, 100, [95], seed=4)
+    clean = call(ops, c, window=6) + call(ops, c, weigh=True, window=6)
+    n = 95 - t - 5
+    if cache == "int8":
+        c["v_scales"][0, :, :n] = math.nan
+    else:
+        c["v"][0, :, :n] = math.nan
+    for x, y in zip(clean, call(ops, c, window=6) + call(ops, c, weigh=True, window=6)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t", (1, 40))
+def test_a_row_of_nan_stays_alone(ops, cache, t):
+    c = R.make_inputs(cache, 3, t, 8, 4, 64, 50, 100, [100, 80, 60], seed=5)
+    clean = call(ops, c)
+    c["q"][1, 0, 3, 5] = math.nan
+    out, lse = call(ops, c)
+    assert out[1, 0, 3].isnan().all() and lse[1, 0, 3].isnan()
+    hit = torch.zeros(3, t, 8, dtype=torch.bool, device="cuda")
+    hit[1, 0, 3] = True
+    assert torch.equal(out[~hit], clean[0][~hit]) and torch.equal(lse[~hit], clean[1][~hit])
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t", (1, 24))
+def test_large_and_small_logits(ops, cache, t):
+    """Softmax weights from one key to all keys alike, scales over many powers of two."""
+    for sharp, scale in ((30.0, None), (0.0, None), (1.0, 1e-3)):
+        both(ops, R.make_inputs(cache, 2, t, 8, 4, 64, 37, 60, [60, 24], seed=6, sharp=sharp), scale=scale)
+    c = R.make_inputs(cache, 2, t, 8, 4, 64, 37, 60, [60, 24], seed=7)
+    if cache == "int8":                                     # V scales from row to row, rising and falling
+        c["v_scales"] *= 2.0 ** (torch.arange(60) % 23 - 11.0)
+        c["prefix_v_scales"] *= 2.0 ** torch.arange(37).flip(0)
+        c["v_scales"][:, :, 3] = 0.0
+        c["q"][:, :, 1] *= 1e-20
+        c["q"][:, :, 2] = 0.0
+    both(ops, c)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t", (1, 40))
+def test_strides(ops, cache, t):
+    """Caches laid out [B, S, KV, D], a slice of a longer cache, queries inside a fused projection."""
+    c = R.make_inputs(cache, 3, t, 8, 4, 64, 50, 100, [100, 80, 60], seed=8)
+    plain = call(ops, c) + call(ops, c, weigh=True)
+    d = cuda(c)
+    fused = torch.zeros(3, t, 16, 64, dtype=d["q"].dtype, device="cuda")
+    fused[:, :, 4:12] = d["q"]
+    d["q"] = fused[:, :, 4:12]
+    for n in ("k", "v"):
+        d[n] = d[n].transpose(1, 2).contiguous().transpose(1, 2)
+        longer = torch.zeros(4, 60, 64, dtype=d[n].dtype, device="cuda")
+        longer[:, 7:57] = d["prefix_" + n]
+        d["prefix_" + n] = longer[:, 7:57]
+        if cache == "int8":
+            s = n + "_scales"
+            d[s] = d[s].permute(2, 0, 1).contiguous().permute(1, 2, 0)
+            d["prefix_" + s] = d["prefix_" + s].t().contiguous().t()
+    d["weights"] = d["weights"].transpose(1, 2).contiguous().transpose(1, 2)
+    args = {n: d.get(n) for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales",
+                                  "prefix_v_scales")}
+    wide = torch.zeros(3, t, 10, 64, dtype=plain[0].dtype, device="cuda")
+    got = ops.prefix_attention(d["q"], d["k"], d["v"], d["lengths"], out=wide[:, :, 1:9], return_lse=True, **args)
+    assert got[0].data_ptr() == wide[:, :, 1:9].data_ptr()
+    assert (wide[:, :, 0] == 0).all() and (wide[:, :, 9] == 0).all()
+    more = ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], weights_out=d["weights"],
+                                    **args)
+    assert more[1] is d["weights"]
+    for x, y in zip(plain, got + more):
+        assert torch.equal(x, y)
+
+
+def test_one_token_without_its_axis(ops):
+    c = R.make_inputs("bf16", 3, 1, 8, 4, 64, 50, 100, [100, 80, 60], seed=8)
+    out, lse = call(ops, c)
+    c["q"] = c["q"][:, 0]
+    out2, lse2 = call(ops, c)
+    assert torch.equal(out[:, 0], out2) and torch.equal(lse[:, 0], lse2)
+
+
+def test_empty_calls(ops):
+    c = R.make_inputs("f16", 2, 1, 8, 4, 64, 50, 100, [100, 80], seed=8)
+    d = cuda(c)
+    out = ops.prefix_attention(d["q"][:0], d["k"][:0], d["v"][:0], d["lengths"][:0])
+    assert out.shape == (0, 1, 8, 64)
+    out, w = ops.accumulate_attention(d["q"][:, :0], d["k"], d["v"], d["lengths"], d["weights"])
+    assert out.shape == (2, 0, 8, 64) and torch.equal(w, d["weights"])
+    # no own slots: the prefix alone
+    ref = R.attention({**c, "lengths": torch.zeros(2, dtype=torch.int32)})
+    out = ops.prefix_attention(d["q"], d["k"][:, :, :0], d["v"][:, :, :0], d["lengths"], d["prefix_k"], d["prefix_v"])
+    R.check(out, ref["out"], R.bounds(c, ref)["out"], "out")
+
+
+# ---- eviction -----------------------------------------------------------------
+
+def evicted(ops, c, keep, first, recent, **more):
+    d = cuda(c)
+    return ops.evict(d["k"], d["v"], d["weights"], d["lengths"], keep, first=first, recent=recent,
+                     k_scales=d["k_scales"], v_scales=d["v_scales"], **more), d
+
+
+def check_evicted(e, c, keep, first, recent, behind=None):
+    for i, row in enumerate(R.evict(c, keep, first, recent)):
+        for g, at in enumerate(row):
+            n = len(at)
+            assert int(e.lengths[i]) == n
+            assert e.indices[i, g].tolist() == at + [-1] * (keep - n)
+            for name in ("k", "v", "k_scales", "v_scales"):
+                if c[name] is not None:
+                    got = getattr(e, name)[i, g].cpu()
+                    assert torch.equal(got[:n], c[name][i, g][at]), name
+                    if behind is not None:
+                        assert torch.equal(got[n:], behind[name][i, g, n:got.shape[0]]), name
+            w = e.weights[i, g].cpu()
+            assert torch.equal(w[:n].nan_to_num(nan=-5.0), c["weights"][i, g][at].nan_to_num(nan=-5.0))
+            assert (w[n:] == 0).all()
+
+
+def evict_inputs(cache, b, kv, d, s, lengths, seed=0):
+    c = R.make_inputs(cache, b, 1, kv, kv, d, 0, s, lengths, seed)
+    g = torch.Generator().manual_seed(seed)
+    # ties, among them zeros of both signs, and weights over many powers of two
+    c["weights"] = torch.exp(4 * torch.randn(b, kv, s, generator=g))
+    c["weights"] = torch.where(torch.rand(b, kv, s, generator=g) < 0.3, torch.zeros(()), c["weights"])
+    c["weights"] = torch.where(torch.rand(b, kv, s, generator=g) < 0.1, -torch.zeros(()), c["weights"])
+    c["weights"] = torch.where(torch.rand(b, kv, s, generator=g) < 0.2, c["weights"].round(), c["weights"])
+    return c
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("b,kv,d,s,lengths,keep,first,recent", [
+    (1, 1, 64, 1, [1], 1, 0, 0),
+    (2, 4, 64, 50, [50, 20], 20, 4, 8),
+    (3, 2, 128, 1500, [1500, 0, 1025], 333, 0, 0),
+    (2, 2, 64, 2100, [2100, 1024], 1024, 1000, 24),         # nothing to choose
+    (2, 2, 128, 700, [700, 699], 699, 1, 1),
+    (2, 1, 64, 30, [30, 9], 64, 4, 4),                      # keep above the capacity
+    (2, 2, 64, 300, [300, 150], 0, 0, 0),                   # nothing stays
+    (2, 3, 64, 9000, [9000, 8999], 1, 0, 1)])
+def test_evict(ops, cache, b, kv, d, s, lengths, keep, first, recent):
+    c = evict_inputs(cache, b, kv, d, s, lengths, seed=s)
+    e, _ = evicted(ops, c, keep, first, recent)
+    check_evicted(e, c, keep, first, recent)
+    if keep <= s:
+        before = {n: None if c[n] is None else c[n].clone() for n in c}
+        e, d = evicted(ops, c, keep, first, recent, in_place=True)
+        assert e.k is d["k"] and e.weights is d["weights"]
+        # rows behind the kept ones may hold what was there or nothing else: unchanged
+        check_evicted(e, c, keep, first, recent, behind=before)
+
+
+@pytest.mark.parametrize("value", (0.0, -0.0, math.nan, -math.inf, math.inf, -3.0))
+def test_evict_equal_weights(ops, value):
+    c = evict_inputs("bf16", 2, 2, 64, 5000, [5000, 4097], seed=1)
+    c["weights"][0] = value
+    c["weights"][1, :, ::3] = value
+    for keep, first, recent in ((100, 0, 0), (4096, 3, 1000)):
+        e, _ = evicted(ops, c, keep, first, recent)
+        check_evicted(e, c, keep, first, recent)
+
+
+def test_evict_into_strided_outputs(ops):
+    c = evict_inputs("int8", 2, 4, 64, 600, [600, 77], seed=2)
+    d = cuda(c)
+    whole = torch.full((2, 200, 4, 64), 9, dtype=torch.int8, device="cuda")
+    f = lambda: torch.full((2, 200, 4), 9.0, device="cuda")      # noqa: E731
+    w, ks, vs = f(), f(), f()
+    other = whole.clone()
+    out = ops.Evicted(whole.transpose(1, 2), other.transpose(1, 2), w.transpose(1, 2),
+                      torch.zeros(2, dtype=torch.int32, device="cuda"),
+                      torch.zeros(2, 4, 150, dtype=torch.int32, device="cuda"), ks.transpose(1, 2), vs.transpose(1, 2))
+    e = ops.evict(d["k"], d["v"], d["weights"], d["lengths"], 150, first=5, recent=10, k_scales=d["k_scales"],
+                  v_scales=d["v_scales"], out=out)
+    behind = {"k": torch.full((2, 4, 200, 64), 9, dtype=torch.int8), "v": torch.full((2, 4, 200, 64), 9, dtype=torch.int8),
+              "k_scales": torch.full((2, 4, 200), 9.0), "v_scales": torch.full((2, 4, 200), 9.0)}
+    check_evicted(e, c, 150, 5, 10, behind=behind)
+
+
+# ---- a run of them together, streams and graphs -------------------------------------
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_prefill_evict_decode(ops, cache):
+    """A prompt behind a shared prefix, its cache thinned out in place, then decoded on: the operators as a
+    generation loop uses them, against the same steps on the definitions."""
+    b, kv, heads, d, p, s, t, keep = 3, 2, 4, 64, 40, 128, 60, 48
+    lengths = [60, 90, 75]
+    c = R.make_inputs(cache, b, t, heads, kv, d, p, s, lengths, seed=12)
+    c["weights"] = torch.zeros(b, kv, s)
+    dev = cuda(c)
+    args = {n: dev.get(n) for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales",
+                                    "prefix_v_scales")}
+    scales = {n: dev[n] for n in ("k_scales", "v_scales")}
+    ref = R.attention(c)
+    out, w = ops.accumulate_attention(dev["q"], dev["k"], dev["v"], dev["lengths"], dev["weights"],
+                                      weights_out=dev["weights"], **args)
+    R.check(out, ref["out"], R.bounds(c, ref)["out"], "prefill")
+    c["weights"] = w.cpu()                                      # the same weights decide on both sides
+    kept = R.evict(c, keep, 2, 8)
+    e = ops.evict(dev["k"], dev["v"], w, dev["lengths"], keep, first=2, recent=8, in_place=True, **scales)
+    check_evicted(e, c, keep, 2, 8)
+    for i in range(b):
+        for g in range(kv):
+            n = len(kept[i][g])
+            for name in ("k", "v", "weights", "k_scales", "v_scales"):
+                if c[name] is not None:
+                    c[name][i, g, :n] = c[name][i, g][kept[i][g]].clone()
+            c["weights"][i, g, n:] = 0
+    lengths = e.lengths.clone()
+    for step in range(3):
+        new = R.make_inputs(cache, b, 1, heads, kv, d, 0, 1, [1] * b, seed=20 + step)
+        c["lengths"] = lengths.cpu() + 1
+        for i in range(b):
+            at = int(lengths[i])
+            for name in ("k", "v", "k_scales", "v_scales"):
+                if c[name] is not None:
+                    c[name][i, :, at] = new[name][i, :, 0]
+                    dev[name][i, :, at] = new[name][i, :, 0].cuda()
+        lengths += 1
+        c["q"] = new["q"]
+        ref = R.attention(c)
+        bound = R.bounds(c, ref)
+        out, w = ops.accumulate_attention(new["q"].cuda(), dev["k"], dev["v"], lengths, dev["weights"],
+                                          weights_out=dev["weights"], **args)
+        R.check(out, ref["out"], bound["out"], f"step {step}")
+        R.check(w, ref["weights"], bound["weights"], f"weights of step {step}")
+        c["weights"] = w.cpu()
+
+
+@pytest.mark.parametrize("t", (1, 40))
+def test_streams_and_graphs(ops, t):
+    """Calls on a side stream, and two captured graphs replayed in turn with new inputs: each keeps its own
+    workspace."""
+    cs = [R.make_inputs("int8", 3, t, 8, 4, 64, 300, 100, [100, 80, 60], seed=30 + i) for i in range(3)]
+    plain = [call(ops, c, weigh=True) for c in cs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    ds = [cuda(c) for c in cs]
+    names = ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales", "prefix_v_scales")
+
+    def run(d, **more):
+        out, w = ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"],
+                                          **{n: d[n] for n in names}, **more)
+        e = ops.evict(d["k"], d["v"], w, d["lengths"], 50, recent=5, k_scales=d["k_scales"], v_scales=d["v_scales"],
+                      **more)
+        return out, w, e
+
+    torch.cuda.synchronize()
+    for given in (side, side.cuda_stream):
+        out, w, _ = run(ds[0], stream=given)
+        side.synchronize()
+        assert torch.equal(out, plain[0][0]) and torch.equal(w, plain[0][1])
+    eager = [run(d)[2] for d in ds]
+    live = [{n: None if x is None else x.clone() for n, x in ds[i].items()} for i in range(2)]
+    graphs, results = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(run(live[i]))
+        graphs.append(graph)
+    for a, b in ((0, 1), (2, 0), (1, 2)):
+        for i, j in ((0, a), (1, b)):
+            for n, x in ds[j].items():
+                if x is not None:
+                    live[i][n].copy_(x)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for i, j in ((0, a), (1, b)):
+            assert torch.equal(results[i][0], plain[j][0]) and torch.equal(results[i][1], plain[j][1])
+            for x, y in zip(results[i][2], eager[j]):
+                assert torch.equal(x, y)
