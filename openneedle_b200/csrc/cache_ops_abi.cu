@@ -48,10 +48,8 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
     return true;
 }
 
-constexpr int kLogitRows = 16;   // query rows of a KV head up to which logits are kept for the weights
-
 struct Plan {
-    int prefix_slots, own_slots;
+    PrefixSplit prefix, own;
     bool logits, row_lse;
     long long part_o, part_lse, row_lse_at, logits_at, bytes;
 };
@@ -71,16 +69,30 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     const int sms = sm_count();
     const int R = a.heads / a.kvheads, tile = a.cache_type == kCacheI8 ? 8 : 16;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
-    auto slots = [&](long long units, int keys) {
-        const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
-        return (int)std::max(1LL, std::min({want, (long long)(keys + 127) / 128, 64LL}));
+    // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys
+    auto split = [&](long long groups, long long group_rows, long long keys) {
+        PrefixSplit s;
+        s.tiles = group_rows > tile;
+        if (s.tiles) {
+            s.alt = group_rows <= 128 || (a.cache_type == kCacheI8 && a.head_dim == 128);
+            const long long units = groups * ((group_rows + (s.alt ? 127 : 255)) / (s.alt ? 128 : 256));
+            const long long most = (keys + (s.alt ? 511 : 255)) / (s.alt ? 512 : 256);
+            s.ranges = (int)std::max(1LL, std::min({sms / std::max(1LL, units), most, 32LL}));
+        } else {
+            const long long units = groups * ((group_rows + tile - 1) / tile);
+            const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
+            s.ranges = (int)std::max(1LL, std::min({want, (keys + 127) / 128, 64LL}));
+        }
+        return s;
     };
-    const long long own_units = (long long)a.batch * a.kvheads * ((a.tokens * R + tile - 1) / tile);
-    const long long prefix_units = (long long)a.kvheads * (((long long)a.batch * a.tokens * R + tile - 1) / tile);
     const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
-    p.own_slots = a.capacity || !a.prefix ? slots(own_units, span) : 0;
-    p.prefix_slots = a.prefix ? slots(prefix_units, a.prefix) : 0;
-    p.logits = a.weights && a.tokens > 0 && a.tokens * R <= kLogitRows;
+    if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span);
+    if (a.prefix) p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix);
+    if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros
+        p.own = PrefixSplit{};
+        p.own.ranges = 1;
+    }
+    p.logits = a.weights && a.tokens > 0 && !p.own.tiles;     // (the tile kernel's rows are too many to keep)
     p.row_lse = a.weights != nullptr;
     long long at = 0;
     auto take = [&](long long bytes) {
@@ -88,7 +100,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    const int n = p.own_slots + p.prefix_slots;
+    const int n = p.own.slots() + p.prefix.slots();
     if (n > 1) {
         p.part_o = take(rows * n * a.head_dim * 4);
         p.part_lse = take(rows * n * 4);
@@ -150,17 +162,25 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
     p.lse = a.lse;
     p.weights = a.weights; p.weights_out = a.weights_out;
     copy(p.ws, a.weights_stride); copy(p.wos, a.weights_out_stride);
-    p.prefix_slots = plan.prefix_slots;
-    p.own_slots = plan.own_slots;
+    p.prefix_slots = plan.prefix.slots();
+    p.own_slots = plan.own.slots();
     char *base = static_cast<char *>(workspace);
-    const int n = plan.own_slots + plan.prefix_slots;
+    const int n = p.own_slots + p.prefix_slots;
     if (n > 1) {
         p.part_o = reinterpret_cast<float *>(base + plan.part_o);
         p.part_lse = reinterpret_cast<float *>(base + plan.part_lse);
     }
     if (plan.row_lse) p.row_lse = reinterpret_cast<float *>(base + plan.row_lse_at);
     if (plan.logits) p.logits = reinterpret_cast<float *>(base + plan.logits_at);
-    if (a.tokens > 0 && !launch_prefix_stream(p, plan.prefix_slots > 0, plan.own_slots > 0, st)) return false;
+    if (a.tokens > 0) {
+        const bool stream_prefix = plan.prefix.ranges && !plan.prefix.tiles;
+        const bool stream_own = plan.own.ranges && !plan.own.tiles;
+        if ((stream_prefix || stream_own) && !launch_prefix_stream(p, stream_prefix, stream_own, st)) return false;
+        // the first axis of a cache addressed by cache_rows has an extent that only the caller knows
+        if ((plan.prefix.tiles || plan.own.tiles) &&
+            !launch_prefix_tiles(p, plan.prefix, plan.own, a.cache_rows ? 1LL << 30 : a.batch, st))
+            return false;
+    }
     if (!launch_prefix_finish(p, st)) return false;
     return !a.weights || plan.logits || launch_key_weights(p, st);
 }

@@ -60,11 +60,24 @@ __device__ __forceinline__ int own_tokens(const PrefixAttn &p, int b) {
     return p.ntokens ? max(0, min(p.ntokens[b], p.tokens)) : p.tokens;
 }
 
+// How one set of keys is attended: by the streaming kernel or by tiles, in how
+// many key ranges; `alt`: both row tiles of a CTA on the same rows and alternate
+// key tiles, each with its partial result.
+struct PrefixSplit {
+    bool tiles = false, alt = false;
+    int ranges = 0;
+    int slots() const { return alt ? 2 * ranges : ranges; }
+};
+
 // The merge of the partial results, weights of few rows from kept logits, and
 // weights of any number of rows from row_lse.
 bool launch_prefix_finish(const PrefixAttn &p, cudaStream_t st);
 bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
 // Streaming kernel: `prefix` / `own` say which key sets it takes.
 bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream_t st);
+// Tile kernel for the sets whose split says `tiles`; cache_rows: extent of the
+// first axis of k and v.
+bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
+                         cudaStream_t st);
 
 }  // namespace nb200

@@ -1,0 +1,774 @@
+// Shared-prefix attention on the sm_100a tensor cores, for many query rows per
+// KV head: the whole batch's rows against the prefix, a sequence's rows of a
+// chunk or prompt against its own keys.  Formulas and the row and
+// partial-result conventions: prefix_attention.cuh.
+//
+// One CTA attends up to 256 rows (two tiles of 128) to one key range, 128 keys
+// at a time.  A warp feeds K and V by TMA, one thread issues the products
+// S = Q K^T (into TMEM) and O += P V (P from TMEM, V from shared memory), and
+// each tile has a warpgroup whose thread i owns row i: it reads its 128 logits
+// back, keeps the row's maximum and sum in registers, writes the weights over
+// the logits and, where the maximum grew by more than 2^8, rescales its row of
+// O.  While one tile is in its softmax the tensor core works for the other.
+// Up to 128 rows run with both warpgroups on the same rows and alternate key
+// tiles, as two key ranges.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+#include "pdl.cuh"
+#include "prefix_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace nb200 {
+
+extern __device__ int g_gemv_fault;
+
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kTile = 128;                       // rows of a tile, keys of a step
+constexpr float kGrow = 8.f;                     // log2 growth of a maximum that is left to the weights
+constexpr uint32_t kWaitLimit = 1u << 22;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Bounded wait; on its end the CTA gives up and raises the device fault flag.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    const uint32_t a = smem_addr(bar);
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 255) == 255 && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(&g_gemv_fault, 1);
+    return false;
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// 128-byte swizzled operands: rows of 128 bytes in atoms of 8 rows.  K-major
+// (Q, K): SBO = 1024 between 8-row groups.  MN-major (V, whose keys are the rows
+// and whose dimensions run along them): SBO = 1024 between groups of 8 keys,
+// LBO between chunks of 64 dimensions.
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(kTile * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16, f32 accumulator: types at bits 7 and 10 (0 f16, 1 bf16), B
+// MN-major at bit 16, N / 8 at bit 17, M / 16 at bit 24.
+__host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int n) {
+    return (1u << 4) | ((uint32_t)bf << 7) | ((uint32_t)bf << 10) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(desc), "r"(acc)
+        : "memory");
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    } else {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+}
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t i8x2_to_f16(uint32_t u) {
+    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+template <int TYPE, int HD>
+struct TileGeom {
+    static constexpr bool I8 = TYPE == kCacheI8;
+    static constexpr int kPieces = I8 ? 2 : 1;                    // FP32 queries and weights as FP16 pairs
+    static constexpr int kTileBytes = kTile * HD * 2;             // a Q, K or V tile of 16-bit values
+    // the FP32 queries' pairs of two 128-dimension tiles would fill the shared memory
+    static constexpr int kQTiles = I8 && HD == 128 ? 1 : 2;
+    static constexpr int kStages = HD == 64 ? (I8 ? 4 : 6) : (I8 ? 3 : 4);
+    static constexpr int kRaw = I8 ? (HD == 64 ? 4 : 2) : 0;      // INT8 tiles on their way
+    static constexpr int kRawBytes = kTile * HD;
+    static constexpr int kScaleRing = 4;
+    static constexpr int kRing = kQTiles * kPieces * kTileBytes;
+    static constexpr int kRawAt = kRing + kStages * kTileBytes;
+    static constexpr int kScaleAt = kRawAt + kRaw * kRawBytes;
+    static constexpr int kSmem = kScaleAt + (I8 ? kScaleRing * 2 * kTile * 4 : 0) + 1024;
+    static constexpr int kConverters = I8 ? 2 : 0;                // warps
+    static constexpr int kThreads = 320 + 32 * kConverters;
+    static_assert(kSmem <= 232448 - 2048, "shared memory of a CTA");
+};
+
+// Units of work: (range, row tiles, KV head[, sequence]).
+struct TileGrid {
+    int own_units, own_tiles, own_ranges, own_alt, own_rows;          // rows of a unit
+    int prefix_units, prefix_tiles, prefix_ranges, prefix_alt, prefix_rows;
+    // whether the cache's head and sequence axes advance in the tensor maps
+    int k_head, k_seq, v_head, v_seq, pk_head, pv_head;
+};
+
+template <int TYPE, int HD>
+__global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_kernel(
+    const PrefixAttn p, const TileGrid grid, const __grid_constant__ CUtensorMap mk,
+    const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mpk,
+    const __grid_constant__ CUtensorMap mpv) {
+    using G = TileGeom<TYPE, HD>;
+    constexpr bool I8 = G::I8, BF = TYPE == kCacheBF16;
+    constexpr int kStages = G::kStages;
+    extern __shared__ __align__(16) char smem_raw[];
+    char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    char *ring = smem + G::kRing;
+    float *scales = (float *)(smem + G::kScaleAt);               // [kScaleRing][K, V][kTile]
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], raw_full[4], raw_empty[4];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
+    __shared__ float qscale[I8 ? 256 : 1];
+    __shared__ float vmost[G::kScaleRing][2];
+    __shared__ uint32_t tmem_at;
+    __shared__ int abort_at;
+    volatile int *abort_flag = &abort_at;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // the unit
+    const int R = p.group, TR = p.tokens * R;
+    int unit = blockIdx.x, g, m0, rows, lo, hi, slot, seq = -1, len = 0, nq = 0, alt;
+    const float *ksc = nullptr, *vsc = nullptr;
+    long long ksc_step = 0, vsc_step = 0;
+    int kz, kw, vz, vw;
+    const CUtensorMap *km, *vm;
+    if (unit < grid.own_units) {
+        alt = grid.own_alt;
+        slot = unit % grid.own_ranges;
+        unit /= grid.own_ranges;
+        // later tokens see more keys: their units first
+        const int tile = grid.own_tiles - 1 - unit % grid.own_tiles;
+        unit /= grid.own_tiles;
+        g = unit % p.kvheads;
+        seq = unit / p.kvheads;
+        m0 = seq * TR + tile * grid.own_rows;
+        rows = min(grid.own_rows, TR - tile * grid.own_rows);
+        len = own_length(p, seq);
+        nq = own_tokens(p, seq);
+        const int t0 = tile * grid.own_rows / R, t1 = min((tile * grid.own_rows + rows - 1) / R, nq - 1);
+        hi = max(0, min(len, len - nq + t1 + 1));
+        lo = p.window ? max(0, len - nq + t0 - p.window + 1) : 0;
+        if (t0 >= nq) rows = 0;
+        const int n = max(0, hi - lo), each = (ceil_div(n, grid.own_ranges) + kTile - 1) / kTile * kTile;
+        const int a = min(hi, lo + slot * each);
+        hi = min(hi, a + each);
+        lo = a;
+        slot = p.prefix_slots + (alt ? 2 * slot : slot);
+        const int row = p.cache_row ? p.cache_row[seq] : seq;
+        km = &mk;
+        vm = &mv;
+        kz = g * grid.k_head; kw = row * grid.k_seq; vz = g * grid.v_head; vw = row * grid.v_seq;
+        if constexpr (I8) {
+            ksc = p.kscale + (long long)row * p.kss[0] + g * p.kss[1];
+            vsc = p.vscale + (long long)row * p.vss[0] + g * p.vss[1];
+            ksc_step = p.kss[2];
+            vsc_step = p.vss[2];
+        }
+    } else {
+        alt = grid.prefix_alt;
+        unit -= grid.own_units;
+        slot = unit % grid.prefix_ranges;
+        unit /= grid.prefix_ranges;
+        const int tile = unit % grid.prefix_tiles;
+        g = unit / grid.prefix_tiles;
+        m0 = tile * grid.prefix_rows;
+        rows = min(grid.prefix_rows, p.batch * TR - m0);
+        const int each = (ceil_div(p.prefix, grid.prefix_ranges) + kTile - 1) / kTile * kTile;
+        lo = min(p.prefix, slot * each);
+        hi = min(p.prefix, lo + each);
+        slot = alt ? 2 * slot : slot;
+        km = &mpk;
+        vm = &mpv;
+        kz = g * grid.pk_head; kw = 0; vz = g * grid.pv_head; vw = 0;
+        if constexpr (I8) {
+            ksc = p.pkscale + g * p.pkss[0];
+            vsc = p.pvscale + g * p.pvss[0];
+            ksc_step = p.pkss[1];
+            vsc_step = p.pvss[1];
+        }
+    }
+    if (rows <= 0) return;                        // the whole CTA
+    const int n = ceil_div(max(0, hi - lo), kTile);              // key tiles
+    const int tiles = alt ? 1 : (rows > kTile ? 2 : 1);          // row tiles
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], I8 ? 32 * G::kConverters : 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < G::kRaw; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], 32 * G::kConverters);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], kTile);
+            mbar_init(&o_full[i], 1);
+        }
+        abort_at = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8) tc::alloc(&tmem_at, 512);
+
+    // the queries, in the products' layout; rows that do not exist are zeros
+    if constexpr (I8) {
+        for (int r = warp; r < tiles * kTile; r += G::kThreads / 32) {
+            float x[HD / 32], most = 0.f;
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) x[e] = 0.f;
+            if (r < rows) {
+                const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
+                const float *q = (const float *)p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2] + lane * (HD / 32);
+#pragma unroll
+                for (int e = 0; e < HD / 32; ++e) {
+                    x[e] = q[e];
+                    most = fmaxf(most, fabsf(x[e]));
+                }
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            // a power of two that brings the row's largest value to [2^12, 2^13)
+            const int ex = most > 0.f ? min(max((int)((__float_as_uint(most) >> 23) & 255) - 127, -100), 100) : 0;
+            const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
+            if (lane == 0) qscale[r] = p.scale2 * __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+            char *q0 = smem + (r / kTile) * 2 * G::kTileBytes;
+#pragma unroll
+            for (int e = 0; e < HD / 32; e += 2) {
+                uint32_t h, l;
+                split2(x[e] * up, x[e + 1] * up, h, l);
+                const int d = lane * (HD / 32) + e, rr = r % kTile;
+                const int at = (d / 64) * (kTile * 128) + rr * 128 + (((d % 64) / 8) ^ (rr & 7)) * 16 + (d % 8) * 2;
+                *(uint32_t *)(q0 + at) = h;
+                *(uint32_t *)(q0 + G::kTileBytes + at) = l;
+            }
+        }
+    } else {
+        constexpr int kChunks = HD / 8;
+        for (int i = threadIdx.x; i < tiles * kTile * kChunks; i += G::kThreads) {
+            const int r = i / kChunks, c = i % kChunks, rr = r % kTile;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows) {
+                const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
+                v = *(const uint4 *)((const char *)p.q + (b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) * 2 + c * 16);
+            }
+            *(uint4 *)(smem + (r / kTile) * G::kTileBytes + (c / 8) * (kTile * 128) + rr * 128 +
+                       (((c % 8) ^ (rr & 7)) << 4)) = v;
+        }
+    }
+    fence_proxy_async();
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == 9) {
+        // ---- copies: tile j's K, then its V
+        if (lane == 0) {
+            int issued = 0;
+            for (int i = 0; i < 2 * n; ++i) {
+                const CUtensorMap *map = i & 1 ? vm : km;
+                const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kTile;
+                if constexpr (I8) {
+                    const int s = i % G::kRaw;
+                    if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
+                    mbar_arrive_expect_tx(&raw_full[s], G::kRawBytes);
+                    tma_load_4d(smem + G::kRawAt + s * G::kRawBytes, map, 0, key, z, w, &raw_full[s]);
+                } else {
+                    const int s = i % kStages;
+                    if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+                    mbar_arrive_expect_tx(&full[s], G::kTileBytes);
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c)
+                        tma_load_4d(ring + s * G::kTileBytes + c * (kTile * 128), map, 64 * c, key, z, w, &full[s]);
+                }
+                ++issued;
+            }
+            // no copy is in flight when the CTA ends, whatever became of its consumers
+            constexpr int kDepth = I8 ? G::kRaw : kStages;
+            for (int i = max(0, issued - kDepth); i < issued; ++i)
+                mbar_wait(I8 ? &raw_full[i % kDepth] : &full[i % kDepth], (uint32_t)(i / kDepth) & 1);
+        }
+        __syncwarp();
+    } else if (warp == 8) {
+        // ---- products
+        const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring);
+        constexpr uint32_t ids = idesc(BF, false, kTile), ido = idesc(BF, true, HD);
+        auto logits = [&](int w, int j) {             // S_w = Q_w K_j^T
+            const uint32_t k = r0 + ((2 * j) % kStages) * G::kTileBytes;
+            const uint32_t q = q0 + (alt ? 0 : w) * (G::kPieces * G::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < G::kPieces; ++x)
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
+                    tc::mma_bf16_ss(tmem + w * kTile, desc_k(q + x * G::kTileBytes + at), desc_k(k + at), ids,
+                                    x + c > 0);
+                }
+            tc::commit(&s_full[w]);
+        };
+        auto values = [&](int w, int j, bool first) {  // O_w += P_w V_j
+            const uint32_t v = r0 + ((2 * j + 1) % kStages) * G::kTileBytes;
+#pragma unroll
+            for (int x = 0; x < G::kPieces; ++x)
+#pragma unroll
+                for (int c = 0; c < kTile / 16; ++c)
+                    mma_ts(tmem + 2 * kTile + w * HD, tmem + w * kTile + x * (kTile / 2) + c * 8, desc_mn(v + c * 2048),
+                           ido, !first || x + c > 0);
+        };
+        auto have = [&](int i) { return wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
+        auto have_v = [&](int j) {
+            if (!have(2 * j + 1)) return false;
+            const int valid = hi - lo - j * kTile;
+            if (!I8 && valid < kTile) {               // rows behind the range: whatever they hold, zeros
+                char *v = ring + ((2 * j + 1) % kStages) * G::kTileBytes;
+                for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c)
+                        *(uint4 *)(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+                __syncwarp();
+            }
+            return true;
+        };
+        bool ok = n > 0;
+        if (alt) {
+            for (int j = 0; ok && j < min(n, 2); ++j) {
+                ok = have(2 * j);
+                if (ok && lane == 0) {
+                    tc::fence_after();
+                    logits(j, j);
+                    tc::commit(&empty[(2 * j) % kStages]);
+                }
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                const int w = j & 1;
+                ok = have_v(j) && wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
+                if (!ok) break;
+                if (lane == 0) {
+                    tc::fence_after();
+                    values(w, j, j < 2);
+                    tc::commit(&empty[(2 * j + 1) % kStages]);
+                    if (j + 2 >= n) tc::commit(&o_full[w]);
+                }
+                if (j + 2 < n) {
+                    ok = have(2 * j + 4);
+                    if (ok && lane == 0) {
+                        tc::fence_after();
+                        logits(w, j + 2);
+                        tc::commit(&empty[(2 * j + 4) % kStages]);
+                    }
+                }
+            }
+        } else {
+            ok = ok && have(0);
+            if (ok && lane == 0) {
+                tc::fence_after();
+                for (int w = 0; w < tiles; ++w) logits(w, 0);
+                tc::commit(&empty[0]);
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                ok = have_v(j);
+                for (int w = 0; ok && w < tiles; ++w) {
+                    ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        tc::fence_after();
+                        values(w, j, j == 0);
+                        if (w == tiles - 1) tc::commit(&empty[(2 * j + 1) % kStages]);
+                        if (j == n - 1) tc::commit(&o_full[w]);
+                    }
+                    if (j + 1 < n) {
+                        ok = w > 0 || have(2 * j + 2);
+                        if (ok && lane == 0) {
+                            tc::fence_after();
+                            logits(w, j + 1);
+                            if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 10) {
+        // ---- INT8 tiles to FP16, exactly
+        if constexpr (I8) {
+            const int me = threadIdx.x - 320;
+            constexpr int kN = 32 * G::kConverters, kChunks = HD / 16;
+            for (int i = 0; i < 2 * n; ++i) {
+                const int s = i % kStages, rs = i % G::kRaw, j = i >> 1;
+                if (!(i & 1)) {
+                    // both scales of the tile's keys (V's zero behind the range), and V's largest
+                    float *sk = scales + (j % G::kScaleRing) * 2 * kTile, most = 0.f;
+                    float kx[kTile / kN], vx[kTile / kN];
+#pragma unroll
+                    for (int e = 0; e < kTile / kN; ++e) {
+                        const int key = lo + j * kTile + me + e * kN;
+                        kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
+                        vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
+                        most = fmaxf(most, fabsf(vx[e]));
+                    }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    // the tile kScaleRing before has been attended: its V was consumed for this stage
+                    if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+#pragma unroll
+                    for (int e = 0; e < kTile / kN; ++e) {
+                        sk[me + e * kN] = kx[e];
+                        sk[kTile + me + e * kN] = vx[e];
+                    }
+                    if (lane == 0) vmost[j % G::kScaleRing][warp - 10] = most;
+                } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
+                    break;
+                }
+                if (!wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag)) break;
+                const char *src = smem + G::kRawAt + rs * G::kRawBytes;
+                char *dst = ring + s * G::kTileBytes;
+#pragma unroll 4
+                for (int x = me; x < kTile * kChunks; x += kN) {
+                    const int r = x / kChunks, c = x % kChunks;
+                    const uint4 w = *(const uint4 *)(src + x * 16);
+                    const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u,
+                                           w.w ^ 0x80808080u};
+                    uint4 a, b;
+                    a.x = i8x2_to_f16<0x4140>(u[0]); a.y = i8x2_to_f16<0x4342>(u[0]);
+                    a.z = i8x2_to_f16<0x4140>(u[1]); a.w = i8x2_to_f16<0x4342>(u[1]);
+                    b.x = i8x2_to_f16<0x4140>(u[2]); b.y = i8x2_to_f16<0x4342>(u[2]);
+                    b.z = i8x2_to_f16<0x4140>(u[3]); b.w = i8x2_to_f16<0x4342>(u[3]);
+                    char *o = dst + (c / 4) * (kTile * 128) + r * 128;
+                    *(uint4 *)(o + (((2 * (c % 4)) ^ (r & 7)) << 4)) = a;
+                    *(uint4 *)(o + (((2 * (c % 4) + 1) ^ (r & 7)) << 4)) = b;
+                }
+                fence_proxy_async();
+                mbar_arrive(&raw_empty[rs]);
+                mbar_arrive(&full[s]);
+            }
+        }
+    } else {
+        // ---- softmax: thread = row
+        const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
+        const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // key tiles of this warpgroup
+        const int m = m0 + (alt ? r : w * kTile + r);
+        const bool row_ok = (alt ? r : w * kTile + r) < rows;
+        const int b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
+        int first = 0, last = hi - 1;
+        if (seq >= 0) {
+            last = t < nq ? min(hi - 1, len - nq + t) : -1;
+            if (p.window) first = len - nq + t - p.window + 1;
+        }
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + w * kTile + lanes, to = tmem + 2 * kTile + w * HD + lanes;
+        float zs = p.scale2;
+        if constexpr (I8) zs = qscale[alt ? r : w * kTile + r];
+        float top = kNegInf, sum = 0.f, vnorm = 0.f;
+        bool ok = true;
+        for (int i = 0; i < mine; ++i) {
+            const int j = alt ? 2 * i + w : i, j0 = lo + j * kTile;
+            ok = wait_phase(&s_full[w], (uint32_t)i & 1, abort_flag);
+            if (I8) ok = ok && wait_phase(&full[(2 * j + 1) % kStages], (uint32_t)((2 * j + 1) / kStages) & 1, abort_flag);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t raw[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
+            tc::wait_ld();
+            float z[kTile];
+            const float *sk = scales + (j % G::kScaleRing) * 2 * kTile;
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) z[c] = __uint_as_float(raw[c / 32][c % 32]);
+            if constexpr (I8) {
+#pragma unroll
+                for (int c = 0; c < kTile; c += 4) {
+                    const float4 s4 = *(const float4 *)(sk + c);
+                    z[c] *= s4.x; z[c + 1] *= s4.y; z[c + 2] *= s4.z; z[c + 3] *= s4.w;
+                }
+            }
+            if (j0 < first || j0 + kTile - 1 > last) {
+                const int x0 = first - j0, x1 = last - j0;
+#pragma unroll
+                for (int c = 0; c < kTile; ++c)
+                    if (c < x0 || c > x1) z[c] = kNegInf;
+            }
+            float best[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+            for (int c = 4; c < kTile; c += 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], z[c + e]);
+            const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * zs;
+            float keep = 1.f;
+            if (now > top + kGrow || (top == kNegInf && now > kNegInf)) {
+                keep = ex2(top - now);                // top = -inf: 0
+                top = now;
+            }
+            sum *= keep;
+            float vinv = 1.f;
+            if constexpr (I8) {
+                // V's scales relative to the largest so far (a power of two), times 2^6:
+                // weights up to 2^kGrow then stay within FP16's 2^16, and what its small
+                // numbers lose is below 2^-31 of the largest; the same in all threads
+                const float most = fmaxf(fmaxf(vmost[j % G::kScaleRing][0], vmost[j % G::kScaleRing][1]), 1e-30f);
+                const float norm = __uint_as_float(__float_as_uint(most) & 0x7f800000u);
+                if (norm > vnorm) {
+                    keep *= vnorm / norm;
+                    vnorm = norm;
+                }
+                vinv = 64.f / vnorm;
+            }
+            if (i > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    tc::ld32(to + 32 * c, o);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                    tc::st32(to + 32 * c, o);
+                }
+            }
+            const float base = top == kNegInf ? 0.f : -top;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) {
+                z[c] = ex2(fmaf(z[c], zs, base));
+                part[c & 3] += z[c];
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            if constexpr (I8) {
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) {
+                    uint32_t ph[16], pl[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 s4 = *(const float4 *)(sk + kTile + c + e);
+                        split2(z[c + e] * (s4.x * vinv), z[c + e + 1] * (s4.y * vinv), ph[e / 2], pl[e / 2]);
+                        split2(z[c + e + 2] * (s4.z * vinv), z[c + e + 3] * (s4.w * vinv), ph[e / 2 + 1],
+                               pl[e / 2 + 1]);
+                    }
+                    tc::st16(ts + c / 2, ph);
+                    tc::st16(ts + kTile / 2 + c / 2, pl);
+                }
+            } else {
+                // the softmax weights are rounded to the cache's type for the product;
+                // their sum keeps 32 bits
+#pragma unroll
+                for (int c = 0; c < kTile; c += 64) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) pk[e] = pack2<BF>(z[c + 2 * e], z[c + 2 * e + 1]);
+                    tc::st32(ts + c / 2, pk);
+                }
+            }
+            tc::wait_st();
+            tc::fence_before();
+            mbar_arrive(&p_full[w]);
+        }
+        if (mine > 0 && ok) ok = wait_phase(&o_full[w], 0, abort_flag);
+        tc::fence_after();
+        if (ok && (alt || w < tiles)) {
+            const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
+            const float lse = sum == 0.f ? kNegInf : (top == kNegInf ? 0.f : top) + log2f(sum);
+            const long long nrows = (long long)p.batch * p.tokens * p.heads;
+            const long long row = ((long long)b * p.tokens + t) * p.heads + h;
+            const bool direct = p.prefix_slots + p.own_slots == 1;
+            const long long part = (slot + (alt ? w : 0)) * nrows + row;
+            const bool write = row_ok && (!direct || t < own_tokens(p, b));
+            if (row_ok) {
+                if (!direct) {
+                    p.part_lse[part] = lse;
+                } else {
+                    if (p.row_lse) p.row_lse[row] = lse;
+                    if (p.lse && write) p.lse[row] = lse * kLn2;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                if (mine > 0) {
+                    tc::ld32(to + 32 * c, o);
+                    tc::wait_ld();
+                }
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+                if (!write) continue;
+                if (!direct) {
+                    float4 *dst = (float4 *)(p.part_o + part * HD + 32 * c);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                } else {
+                    char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + 32 * c) * (I8 ? 4 : 2);
+                    if constexpr (I8) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            ((float4 *)dst)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            ((uint4 *)dst)[e] =
+                                make_uint4(pack2<BF>(v[8 * e], v[8 * e + 1]), pack2<BF>(v[8 * e + 2], v[8 * e + 3]),
+                                           pack2<BF>(v[8 * e + 4], v[8 * e + 5]), pack2<BF>(v[8 * e + 6], v[8 * e + 7]));
+                    }
+                }
+            }
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 8) tc::dealloc(tmem, 512);
+}
+
+// ---- host ------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    });
+    return fn;
+}
+
+// Map of a cache [seqs][heads][keys][hd] in tiles of kTile keys: 128-byte
+// swizzled chunks of 64 16-bit values, or whole INT8 rows.  Axes of stride 0
+// (or one element) get extent 1 and their flag 0: the kernel's coordinate stays 0.
+bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long keys, long long heads, long long seqs,
+               long long key_stride, long long head_stride, long long seq_stride, int *head_flag, int *seq_flag) {
+    auto fn = encoder();
+    if (!fn) {
+        set_error("cuTensorMapEncodeTiled is unavailable");
+        return false;
+    }
+    const bool i8 = type == kCacheI8;
+    const long long size = i8 ? 1 : 2, row = hd * size;
+    *head_flag = head_stride != 0 && heads > 1;
+    *seq_flag = seq_stride != 0 && seqs > 1;
+    if (!*head_flag) heads = 1;
+    if (!*seq_flag) seqs = 1;
+    const long long ks = keys > 1 && key_stride ? key_stride * size : row;
+    if (keys > 1 && !key_stride) keys = 1;       // refused by the caller
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)keys, (cuuint64_t)heads, (cuuint64_t)seqs};
+    const cuuint64_t strides[3] = {(cuuint64_t)ks, (cuuint64_t)(*head_flag ? head_stride * size : row),
+                                   (cuuint64_t)(*seq_flag ? seq_stride * size : row)};
+    const cuuint32_t box[4] = {(cuuint32_t)(i8 ? hd : 64), (cuuint32_t)kTile, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r =
+        fn(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims,
+           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("prefix attention: the cache's strides cannot be described to the copy engine");
+        return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
+                         cudaStream_t st) {
+    auto run = [&](auto type, auto hd) -> bool {
+        using G = TileGeom<type(), hd()>;
+        TileGrid grid{};
+        const int rows = p.tokens * p.group;
+        CUtensorMap mk{}, mv{}, mpk{}, mpv{};
+        int unused;
+        if (own.tiles) {
+            grid.own_alt = own.alt;
+            grid.own_rows = own.alt ? kTile : 2 * kTile;
+            grid.own_tiles = ceil_div(rows, grid.own_rows);
+            grid.own_ranges = own.ranges;
+            grid.own_units = p.batch * p.kvheads * grid.own_tiles * own.ranges;
+            if (!cache_map(&mk, p.k, type(), hd(), p.capacity, p.kvheads, cache_rows, p.ks[2], p.ks[1], p.ks[0],
+                           &grid.k_head, &grid.k_seq) ||
+                !cache_map(&mv, p.v, type(), hd(), p.capacity, p.kvheads, cache_rows, p.vs[2], p.vs[1], p.vs[0],
+                           &grid.v_head, &grid.v_seq))
+                return false;
+        }
+        if (prefix.tiles) {
+            grid.prefix_alt = prefix.alt;
+            grid.prefix_rows = prefix.alt ? kTile : 2 * kTile;
+            grid.prefix_tiles = ceil_div(p.batch * rows, grid.prefix_rows);
+            grid.prefix_ranges = prefix.ranges;
+            grid.prefix_units = p.kvheads * grid.prefix_tiles * prefix.ranges;
+            if (!cache_map(&mpk, p.pk, type(), hd(), p.prefix, p.kvheads, 1, p.pks[1], p.pks[0], 0, &grid.pk_head,
+                           &unused) ||
+                !cache_map(&mpv, p.pv, type(), hd(), p.prefix, p.kvheads, 1, p.pvs[1], p.pvs[0], 0, &grid.pv_head,
+                           &unused))
+                return false;
+        }
+        const int blocks = grid.own_units + grid.prefix_units;
+        if (blocks == 0) return true;
+        auto kernel = prefix_tile_kernel<type(), hd()>;
+        static bool configured[64] = {};
+        int dev = 0;
+        NB_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            NB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+        kernel<<<blocks, G::kThreads, G::kSmem, st>>>(p, grid, mk, mv, mpk, mpv);
+        NB_CUDA_TRY(cudaGetLastError());
+        return true;
+    };
+    if (p.hd == 64) {
+        if (p.type == kCacheI8) return run(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 64>());
+        if (p.type == kCacheBF16)
+            return run(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 64>());
+        return run(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 64>());
+    }
+    if (p.type == kCacheI8) return run(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 128>());
+    if (p.type == kCacheBF16) return run(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 128>());
+    return run(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 128>());
+}
+
+}  // namespace nb200

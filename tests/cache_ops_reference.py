@@ -49,6 +49,7 @@ def attention(c, window=0, tokens=None, scale=None):
     mix = torch.zeros_like(out)          # sum of p |v|, what an output's rounding errors are relative to
     dz = torch.zeros(b, t, heads, dtype=torch.float64)   # sum |q k| of the largest
     total_v = torch.zeros_like(out)      # sum of |v| over the visible keys
+    most_v = torch.zeros(b, t, heads, dtype=torch.float64)   # their number times the largest |v| scale times 127
     for i in range(b):
         n = max(0, min(int(c["lengths"][i]), s))
         m = t if tokens is None else max(0, min(int(tokens[i]), t))
@@ -72,10 +73,15 @@ def attention(c, window=0, tokens=None, scale=None):
                     mix[i, x, h] = soft @ v[seen].abs()
                     total_v[i, x, h] = v[seen].abs().sum(0)
                     dz[i, x, h] = scale * (k[seen].abs() @ q[i, x, h].abs()).max()
+                    if c["v_scales"] is not None:
+                        vs = c["v_scales"][i, g, :n]
+                        vs = (torch.cat((c["prefix_v_scales"][g], vs)) if p else vs)[seen].double()
+                        most_v[i, x, h] = len(seen) * 127 * vs.abs().max()
                     own = torch.tensor([j - p for j in seen if j >= p], dtype=torch.long)
                     gained[i, g, own] += soft[len(seen) - len(own):]
     weights += gained
-    return {"out": out, "lse": lse, "weights": weights, "gained": gained, "mix": mix, "dz": dz, "total_v": total_v}
+    return {"out": out, "lse": lse, "weights": weights, "gained": gained, "mix": mix, "dz": dz, "total_v": total_v,
+            "most_v": most_v}
 
 
 def bounds(c, ref):
@@ -87,14 +93,17 @@ def bounds(c, ref):
     e enters a softmax weight as the factor 1 + 2 e.  The exponential and the
     sums add 2^-20.  16-bit caches round each softmax weight (half a step, and
     half of the smallest FP16 number, 2^-25, where they fall below its normal
-    range) and the output (half a step)."""
+    range) and the output (half a step).  INT8 caches multiply the softmax weights
+    by V's scales over the power of two at or below the largest, times at least
+    2^6, and round the product to an FP16 pair: 2^-22 of it, or half of the
+    smallest FP16 number, 2^-25 / 2^6, of the largest scale for each key."""
     d = c["q"].shape[-1]
     e = ref["dz"] * (d / 4 + 12) * 2.0 ** -24 + 2.0 ** -22 * ref["lse"].abs().nan_to_num(posinf=0.0)
     rel = 2 * e + 2.0 ** -20
     out = ref["mix"] * rel.unsqueeze(-1)
     kind = c["k"].dtype
     if kind == torch.int8:
-        out = out + 2.0 ** -24 * ref["out"].abs() + 2.0 ** -30 * ref["total_v"]
+        out = out + 2.0 ** -24 * ref["out"].abs() + 2.0 ** -31 * ref["most_v"].unsqueeze(-1)
     else:
         half = torch.finfo(kind).eps / 2
         out = (out + half * ref["mix"]) * (1 + half) + half * ref["out"].abs()
