@@ -20,6 +20,9 @@ INCLUDE = PKG.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fno-fast-math",
          "--expt-relaxed-constexpr", f"-I{INCLUDE}"]
+# Sources without device symbols of other files, compiled as whole programs: the
+# assembler ignores setmaxnreg in relocatable device code.
+WHOLE_PROGRAM = {"prefix_attention_tc.cu"}
 
 
 def nvcc() -> str:
@@ -54,7 +57,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         objs.append(str(obj))
         # an object is reused only when it is newer than its source and every header
         if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, newest_header):
-            jobs.append([nvcc(), *ARCH, *FLAGS, "-dc", str(src), "-o", str(obj)])
+            jobs.append([nvcc(), *ARCH, *FLAGS, "-c" if src.name in WHOLE_PROGRAM else "-dc", str(src), "-o",
+                         str(obj)])
 
     def run(cmd):
         if verbose:

@@ -13,6 +13,7 @@
 #include "../../include/needle2_b200.h"
 #include "common.cuh"
 #include "cq_gemv.cuh"
+#include "prefix_attention.cuh"
 #include "cq_handle.cuh"
 #include "cq_kernels.cuh"
 
@@ -914,7 +915,10 @@ int needle2_b200_activation_quant(float *x, int rows, int dim, int bits) {
     return ok ? 0 : -1;
 }
 
-int needle2_b200_device_fault() { return nb200::read_and_clear_gemv_fault(); }
+int needle2_b200_device_fault() {
+    const int matmul = nb200::read_and_clear_gemv_fault(), tiles = nb200::read_and_clear_tile_fault();
+    return matmul < 0 || tiles < 0 ? -1 : matmul | tiles;
+}
 
 int needle2_cq_geometry(void *handle, int *g) {
     auto *m = static_cast<Matrix *>(handle);

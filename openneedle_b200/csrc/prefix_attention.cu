@@ -1,28 +1,18 @@
 // Shared-prefix attention for few query rows per KV head (decode), the merge of
 // partial results and the accumulated key weights.  Formulas and the row and
 // partial-result conventions: prefix_attention.cuh.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
 #include "pdl.cuh"
 #include "prefix_attention.cuh"
-#include "sm100_async.cuh"
+#include "tile_math.cuh"
 
 namespace nb200 {
 namespace {
 
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNegInf = -__builtin_huge_valf();
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+using namespace tile;
 
 // ---- matrix fragments ------------------------------------------------------
 
@@ -51,36 +41,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(a)
                  : "memory");
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (BF) {
-        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&v);
-    } else {
-        __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&v);
-    }
-}
-
-// x = hi + lo in FP16, 22 significand bits of each value within range
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// Two FP16 values of two int8 codes, exactly: the code plus 128 put into the
-// low bits of 1024.0 gives 1024 + 128 + code, from which 1152 is taken.  `u`
-// holds four codes with their sign bits flipped; `sel` picks the two bytes.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t i8x2_to_f16(uint32_t u) {
-    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 // 16-byte copy to shared memory, zeros where the source does not exist
@@ -278,11 +238,9 @@ __global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(const Prefix
             }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // a power of two that brings the row's largest value to [2^12, 2^13): the
-        // FP16 pair then keeps 22 bits of every value that matters beside it
-        const int ex = most > 0.f ? min(max((int)((__float_as_uint(most) >> 23) & 255) - 127, -100), 100) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
-        qscale *= __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+        float up, down;
+        row_scale(most, up, down);
+        qscale *= down;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             split2(x[k][0] * up, x[k][1] * up, qa[k][0], qa[k][1]);
@@ -710,9 +668,8 @@ __global__ __launch_bounds__(128) void key_weights_kernel(const PrefixAttn p) {
                     }
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const int ex = most > 0.f ? min(max((int)((__float_as_uint(most) >> 23) & 255) - 127, -100), 100) : 0;
-                const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
-                down = __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+                float up;
+                row_scale(most, up, down);
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     uint32_t h0, l0, h1, l1;

@@ -79,5 +79,8 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream
 // first axis of k and v.
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
                          cudaStream_t st);
+// 1 if a bounded wait of the tile kernels ran out since the last call, -1 if
+// the flag could not be read.
+int read_and_clear_tile_fault();
 
 }  // namespace nb200

@@ -12,10 +12,7 @@
 // O.  While one tile is in its softmax the tensor core works for the other.
 // Up to 128 rows run with both warpgroups on the same rows and alternate key
 // tiles, as two key ranges.
-#include <cuda.h>
 #include <cudaTypedefs.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <mutex>
@@ -24,103 +21,17 @@
 #include "common.cuh"
 #include "pdl.cuh"
 #include "prefix_attention.cuh"
-#include "tcgen05.cuh"
+#include "tile_math.cuh"
 
 namespace nb200 {
-
-extern __device__ int g_gemv_fault;
-
 namespace {
 
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kTile = 128;                       // rows of a tile, keys of a step
+using namespace tile;
+
+__device__ int g_tile_fault = 0;                 // a bounded wait ran out
+
+constexpr int kFmaOf8 = 2;                       // of 8 powers of two, those on the FP32 pipe
 constexpr float kGrow = 8.f;                     // log2 growth of a maximum that is left to the weights
-constexpr uint32_t kWaitLimit = 1u << 22;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Bounded wait; on its end the CTA gives up and raises the device fault flag.
-__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    const uint32_t a = smem_addr(bar);
-    for (uint32_t i = 0; i < kWaitLimit; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 255) == 255 && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    atomicExch(&g_gemv_fault, 1);
-    return false;
-}
-
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5}], [%6];" ::"r"(smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
-        : "memory");
-}
-
-// 128-byte swizzled operands: rows of 128 bytes in atoms of 8 rows.  K-major
-// (Q, K): SBO = 1024 between 8-row groups.  MN-major (V, whose keys are the rows
-// and whose dimensions run along them): SBO = 1024 between groups of 8 keys,
-// LBO between chunks of 64 dimensions.
-__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(kTile * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-// kind::f16, f32 accumulator: types at bits 7 and 10 (0 f16, 1 bf16), B
-// MN-major at bit 16, N / 8 at bit 17, M / 16 at bit 24.
-__host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int n) {
-    return (1u << 4) | ((uint32_t)bf << 7) | ((uint32_t)bf << 10) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(desc), "r"(acc)
-        : "memory");
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (BF) {
-        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&v);
-    } else {
-        __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&v);
-    }
-}
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t i8x2_to_f16(uint32_t u) {
-    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 
 template <int TYPE, int HD>
 struct TileGeom {
@@ -138,8 +49,8 @@ struct TileGeom {
     static constexpr int kScaleAt = kRawAt + kRaw * kRawBytes;
     static constexpr int kSmem = kScaleAt + (I8 ? kScaleRing * 2 * kTile * 4 : 0) + 1024;
     static constexpr int kConverters = I8 ? 2 : 0;                // warps
-    static constexpr int kThreads = 320 + 32 * kConverters;
-    static_assert(kSmem <= 232448 - 2048, "shared memory of a CTA");
+    static constexpr int kThreads = kTileThreads;
+    static_assert(kSmem <= 232448 - 4096, "shared memory of a CTA");
 };
 
 // Units of work: (range, row tiles, KV head[, sequence]).
@@ -166,6 +77,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
     __shared__ float qscale[I8 ? 256 : 1];
     __shared__ float vmost[G::kScaleRing][2];
+    __shared__ const char *qrow[256];
     __shared__ uint32_t tmem_at;
     __shared__ int abort_at;
     volatile int *abort_flag = &abort_at;
@@ -257,48 +169,59 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     if (warp == 8) tc::alloc(&tmem_at, 512);
 
     // the queries, in the products' layout; rows that do not exist are zeros
+    for (int r = threadIdx.x; r < tiles * kTile; r += G::kThreads) {
+        const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
+        qrow[r] = r < rows ? (const char *)p.q + (b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) * (I8 ? 4 : 2) : nullptr;
+    }
+    __syncthreads();
     if constexpr (I8) {
-        for (int r = warp; r < tiles * kTile; r += G::kThreads / 32) {
-            float x[HD / 32], most = 0.f;
+        // HD / 4 lanes a row, four rows of each lane in flight
+        constexpr int kLanes = HD / 4, kPer = G::kThreads / kLanes;
+        const int l = threadIdx.x % kLanes;
+        for (int r0 = threadIdx.x / kLanes; r0 < tiles * kTile; r0 += 4 * kPer) {
+            float4 x[4];
 #pragma unroll
-            for (int e = 0; e < HD / 32; ++e) x[e] = 0.f;
-            if (r < rows) {
-                const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
-                const float *q = (const float *)p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2] + lane * (HD / 32);
-#pragma unroll
-                for (int e = 0; e < HD / 32; ++e) {
-                    x[e] = q[e];
-                    most = fmaxf(most, fabsf(x[e]));
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int r = r0 + e * kPer;
+                const char *q = r < tiles * kTile ? qrow[r] : nullptr;
+                x[e] = q ? *(const float4 *)(q + l * 16) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
-            for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            // a power of two that brings the row's largest value to [2^12, 2^13)
-            const int ex = most > 0.f ? min(max((int)((__float_as_uint(most) >> 23) & 255) - 127, -100), 100) : 0;
-            const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
-            if (lane == 0) qscale[r] = p.scale2 * __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
-            char *q0 = smem + (r / kTile) * 2 * G::kTileBytes;
+            for (int e = 0; e < 4; ++e) {
+                const int r = r0 + e * kPer;
+                float most = fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w)));
 #pragma unroll
-            for (int e = 0; e < HD / 32; e += 2) {
-                uint32_t h, l;
-                split2(x[e] * up, x[e + 1] * up, h, l);
-                const int d = lane * (HD / 32) + e, rr = r % kTile;
-                const int at = (d / 64) * (kTile * 128) + rr * 128 + (((d % 64) / 8) ^ (rr & 7)) * 16 + (d % 8) * 2;
-                *(uint32_t *)(q0 + at) = h;
-                *(uint32_t *)(q0 + G::kTileBytes + at) = l;
+                for (int d = kLanes / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                float up, down;
+                row_scale(most, up, down);
+                uint2 h, lo2;
+                split2(x[e].x * up, x[e].y * up, h.x, lo2.x);
+                split2(x[e].z * up, x[e].w * up, h.y, lo2.y);
+                if (r < tiles * kTile) {
+                    if (l == 0) qscale[r] = p.scale2 * down;
+                    char *q = smem + (r / kTile) * 2 * G::kTileBytes + piece_at(r % kTile, l / 2) + (l & 1) * 8;
+                    *(uint2 *)q = h;
+                    *(uint2 *)(q + G::kTileBytes) = lo2;
+                }
             }
         }
     } else {
-        constexpr int kChunks = HD / 8;
-        for (int i = threadIdx.x; i < tiles * kTile * kChunks; i += G::kThreads) {
-            const int r = i / kChunks, c = i % kChunks, rr = r % kTile;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows) {
-                const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
-                v = *(const uint4 *)((const char *)p.q + (b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) * 2 + c * 16);
+        constexpr int kChunks = HD / 8, kPer = G::kThreads / kChunks;
+        const int c = threadIdx.x % kChunks;
+        for (int r0 = threadIdx.x / kChunks; r0 < tiles * kTile; r0 += 6 * kPer) {
+            uint4 x[6];
+#pragma unroll
+            for (int e = 0; e < 6; ++e) {
+                const int r = r0 + e * kPer;
+                const char *q = r < tiles * kTile ? qrow[r] : nullptr;
+                x[e] = q ? *(const uint4 *)(q + c * 16) : make_uint4(0, 0, 0, 0);
             }
-            *(uint4 *)(smem + (r / kTile) * G::kTileBytes + (c / 8) * (kTile * 128) + rr * 128 +
-                       (((c % 8) ^ (rr & 7)) << 4)) = v;
+#pragma unroll
+            for (int e = 0; e < 6; ++e) {
+                const int r = r0 + e * kPer;
+                if (r < tiles * kTile)
+                    *(uint4 *)(smem + (r / kTile) * G::kTileBytes + piece_at(r % kTile, c)) = x[e];
+            }
         }
     }
     fence_proxy_async();
@@ -307,189 +230,186 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     tc::fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp == 9) {
-        // ---- copies: tile j's K, then its V
-        if (lane == 0) {
-            int issued = 0;
-            for (int i = 0; i < 2 * n; ++i) {
-                const CUtensorMap *map = i & 1 ? vm : km;
-                const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kTile;
-                if constexpr (I8) {
-                    const int s = i % G::kRaw;
-                    if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
-                    mbar_arrive_expect_tx(&raw_full[s], G::kRawBytes);
-                    tma_load_4d(smem + G::kRawAt + s * G::kRawBytes, map, 0, key, z, w, &raw_full[s]);
-                } else {
-                    const int s = i % kStages;
-                    if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
-                    mbar_arrive_expect_tx(&full[s], G::kTileBytes);
-#pragma unroll
-                    for (int c = 0; c < HD / 64; ++c)
-                        tma_load_4d(ring + s * G::kTileBytes + c * (kTile * 128), map, 64 * c, key, z, w, &full[s]);
+    if (warp >= 8) {
+        fewer_registers();
+        if (warp == 9) {
+            // ---- copies: tile j's K, then its V
+            if (lane == 0) {
+                int issued = 0;
+                for (int i = 0; i < 2 * n; ++i) {
+                    const CUtensorMap *map = i & 1 ? vm : km;
+                    const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kTile;
+                    if constexpr (I8) {
+                        const int s = i % G::kRaw;
+                        if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
+                        mbar_arrive_expect_tx(&raw_full[s], G::kRawBytes);
+                        tma_load_4d(smem + G::kRawAt + s * G::kRawBytes, map, 0, key, z, w, &raw_full[s]);
+                    } else {
+                        const int s = i % kStages;
+                        if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+                        mbar_arrive_expect_tx(&full[s], G::kTileBytes);
+    #pragma unroll
+                        for (int c = 0; c < HD / 64; ++c)
+                            tma_load_4d(ring + s * G::kTileBytes + c * (kTile * 128), map, 64 * c, key, z, w, &full[s]);
+                    }
+                    ++issued;
                 }
-                ++issued;
+                // no copy is in flight when the CTA ends, whatever became of its consumers
+                constexpr int kDepth = I8 ? G::kRaw : kStages;
+                for (int i = max(0, issued - kDepth); i < issued; ++i)
+                    mbar_wait(I8 ? &raw_full[i % kDepth] : &full[i % kDepth], (uint32_t)(i / kDepth) & 1);
             }
-            // no copy is in flight when the CTA ends, whatever became of its consumers
-            constexpr int kDepth = I8 ? G::kRaw : kStages;
-            for (int i = max(0, issued - kDepth); i < issued; ++i)
-                mbar_wait(I8 ? &raw_full[i % kDepth] : &full[i % kDepth], (uint32_t)(i / kDepth) & 1);
-        }
-        __syncwarp();
-    } else if (warp == 8) {
-        // ---- products
-        const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring);
-        constexpr uint32_t ids = idesc(BF, false, kTile), ido = idesc(BF, true, HD);
-        auto logits = [&](int w, int j) {             // S_w = Q_w K_j^T
-            const uint32_t k = r0 + ((2 * j) % kStages) * G::kTileBytes;
-            const uint32_t q = q0 + (alt ? 0 : w) * (G::kPieces * G::kTileBytes);
-#pragma unroll
-            for (int x = 0; x < G::kPieces; ++x)
-#pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
-                    tc::mma_bf16_ss(tmem + w * kTile, desc_k(q + x * G::kTileBytes + at), desc_k(k + at), ids,
-                                    x + c > 0);
+            __syncwarp();
+        } else if (warp == 8) {
+            // ---- products
+            const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring);
+            constexpr uint32_t ids = idesc(BF, false, kTile), ido = idesc(BF, true, HD);
+            auto logits = [&](int w, int j) {             // S_w = Q_w K_j^T
+                const uint32_t k = r0 + ((2 * j) % kStages) * G::kTileBytes;
+                const uint32_t q = q0 + (alt ? 0 : w) * (G::kPieces * G::kTileBytes);
+    #pragma unroll
+                for (int x = 0; x < G::kPieces; ++x)
+    #pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {
+                        const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
+                        tc::mma_bf16_ss(tmem + w * kTile, desc_k(q + x * G::kTileBytes + at), desc_k(k + at), ids,
+                                        x + c > 0);
+                    }
+                tc::commit(&s_full[w]);
+            };
+            auto values = [&](int w, int j, bool first) {  // O_w += P_w V_j
+                const uint32_t v = r0 + ((2 * j + 1) % kStages) * G::kTileBytes;
+    #pragma unroll
+                for (int x = 0; x < G::kPieces; ++x)
+    #pragma unroll
+                    for (int c = 0; c < kTile / 16; ++c)
+                        mma_ts(tmem + 2 * kTile + w * HD, tmem + w * kTile + x * (kTile / 2) + c * 8, desc_mn(v + c * 2048),
+                               ido, !first || x + c > 0);
+            };
+            auto have = [&](int i) { return wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
+            auto have_v = [&](int j) {
+                if (!have(2 * j + 1)) return false;
+                const int valid = hi - lo - j * kTile;
+                if (!I8 && valid < kTile) {               // rows behind the range: whatever they hold, zeros
+                    char *v = ring + ((2 * j + 1) % kStages) * G::kTileBytes;
+                    for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
+    #pragma unroll
+                        for (int c = 0; c < HD / 64; ++c)
+                            *(uint4 *)(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
                 }
-            tc::commit(&s_full[w]);
-        };
-        auto values = [&](int w, int j, bool first) {  // O_w += P_w V_j
-            const uint32_t v = r0 + ((2 * j + 1) % kStages) * G::kTileBytes;
-#pragma unroll
-            for (int x = 0; x < G::kPieces; ++x)
-#pragma unroll
-                for (int c = 0; c < kTile / 16; ++c)
-                    mma_ts(tmem + 2 * kTile + w * HD, tmem + w * kTile + x * (kTile / 2) + c * 8, desc_mn(v + c * 2048),
-                           ido, !first || x + c > 0);
-        };
-        auto have = [&](int i) { return wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
-        auto have_v = [&](int j) {
-            if (!have(2 * j + 1)) return false;
-            const int valid = hi - lo - j * kTile;
-            if (!I8 && valid < kTile) {               // rows behind the range: whatever they hold, zeros
-                char *v = ring + ((2 * j + 1) % kStages) * G::kTileBytes;
-                for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
-#pragma unroll
-                    for (int c = 0; c < HD / 64; ++c)
-                        *(uint4 *)(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
-                __syncwarp();
-            }
-            return true;
-        };
-        bool ok = n > 0;
-        if (alt) {
-            for (int j = 0; ok && j < min(n, 2); ++j) {
-                ok = have(2 * j);
-                if (ok && lane == 0) {
-                    tc::fence_after();
-                    logits(j, j);
-                    tc::commit(&empty[(2 * j) % kStages]);
-                }
-            }
-            for (int j = 0; ok && j < n; ++j) {
-                const int w = j & 1;
-                ok = have_v(j) && wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
-                if (!ok) break;
-                if (lane == 0) {
-                    tc::fence_after();
-                    values(w, j, j < 2);
-                    tc::commit(&empty[(2 * j + 1) % kStages]);
-                    if (j + 2 >= n) tc::commit(&o_full[w]);
-                }
-                if (j + 2 < n) {
-                    ok = have(2 * j + 4);
+                return true;
+            };
+            bool ok = n > 0;
+            if (alt) {
+                for (int j = 0; ok && j < min(n, 2); ++j) {
+                    ok = have(2 * j);
                     if (ok && lane == 0) {
                         tc::fence_after();
-                        logits(w, j + 2);
-                        tc::commit(&empty[(2 * j + 4) % kStages]);
+                        logits(j, j);
+                        tc::commit(&empty[(2 * j) % kStages]);
                     }
                 }
-            }
-        } else {
-            ok = ok && have(0);
-            if (ok && lane == 0) {
-                tc::fence_after();
-                for (int w = 0; w < tiles; ++w) logits(w, 0);
-                tc::commit(&empty[0]);
-            }
-            for (int j = 0; ok && j < n; ++j) {
-                ok = have_v(j);
-                for (int w = 0; ok && w < tiles; ++w) {
-                    ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
+                for (int j = 0; ok && j < n; ++j) {
+                    const int w = j & 1;
+                    ok = have_v(j) && wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
                     if (!ok) break;
                     if (lane == 0) {
                         tc::fence_after();
-                        values(w, j, j == 0);
-                        if (w == tiles - 1) tc::commit(&empty[(2 * j + 1) % kStages]);
-                        if (j == n - 1) tc::commit(&o_full[w]);
+                        values(w, j, j < 2);
+                        tc::commit(&empty[(2 * j + 1) % kStages]);
+                        if (j + 2 >= n) tc::commit(&o_full[w]);
                     }
-                    if (j + 1 < n) {
-                        ok = w > 0 || have(2 * j + 2);
+                    if (j + 2 < n) {
+                        ok = have(2 * j + 4);
                         if (ok && lane == 0) {
                             tc::fence_after();
-                            logits(w, j + 1);
-                            if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
+                            logits(w, j + 2);
+                            tc::commit(&empty[(2 * j + 4) % kStages]);
+                        }
+                    }
+                }
+            } else {
+                ok = ok && have(0);
+                if (ok && lane == 0) {
+                    tc::fence_after();
+                    for (int w = 0; w < tiles; ++w) logits(w, 0);
+                    tc::commit(&empty[0]);
+                }
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = have_v(j);
+                    for (int w = 0; ok && w < tiles; ++w) {
+                        ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            tc::fence_after();
+                            values(w, j, j == 0);
+                            if (w == tiles - 1) tc::commit(&empty[(2 * j + 1) % kStages]);
+                            if (j == n - 1) tc::commit(&o_full[w]);
+                        }
+                        if (j + 1 < n) {
+                            ok = w > 0 || have(2 * j + 2);
+                            if (ok && lane == 0) {
+                                tc::fence_after();
+                                logits(w, j + 1);
+                                if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
+                            }
                         }
                     }
                 }
             }
-        }
-        __syncwarp();
-    } else if (warp >= 10) {
-        // ---- INT8 tiles to FP16, exactly
-        if constexpr (I8) {
-            const int me = threadIdx.x - 320;
-            constexpr int kN = 32 * G::kConverters, kChunks = HD / 16;
-            for (int i = 0; i < 2 * n; ++i) {
-                const int s = i % kStages, rs = i % G::kRaw, j = i >> 1;
-                if (!(i & 1)) {
-                    // both scales of the tile's keys (V's zero behind the range), and V's largest
-                    float *sk = scales + (j % G::kScaleRing) * 2 * kTile, most = 0.f;
-                    float kx[kTile / kN], vx[kTile / kN];
-#pragma unroll
-                    for (int e = 0; e < kTile / kN; ++e) {
-                        const int key = lo + j * kTile + me + e * kN;
-                        kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
-                        vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
-                        most = fmaxf(most, fabsf(vx[e]));
+            __syncwarp();
+        } else if (warp >= 10) {
+            // ---- INT8 tiles to FP16, exactly
+            if constexpr (I8) {
+                const int me = threadIdx.x - 320;
+                constexpr int kN = 32 * G::kConverters, kChunks = HD / 16;
+                for (int i = 0; i < 2 * n; ++i) {
+                    const int s = i % kStages, rs = i % G::kRaw, j = i >> 1;
+                    if (!(i & 1)) {
+                        // both scales of the tile's keys (V's zero behind the range), and V's largest
+                        float *sk = scales + (j % G::kScaleRing) * 2 * kTile, most = 0.f;
+                        float kx[kTile / kN], vx[kTile / kN];
+    #pragma unroll
+                        for (int e = 0; e < kTile / kN; ++e) {
+                            const int key = lo + j * kTile + me + e * kN;
+                            kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
+                            vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
+                            most = fmaxf(most, fabsf(vx[e]));
+                        }
+    #pragma unroll
+                        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                        // the tile kScaleRing before has been attended: its V was consumed for this stage
+                        if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+    #pragma unroll
+                        for (int e = 0; e < kTile / kN; ++e) {
+                            sk[me + e * kN] = kx[e];
+                            sk[kTile + me + e * kN] = vx[e];
+                        }
+                        if (lane == 0) vmost[j % G::kScaleRing][warp - 10] = most;
+                    } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
+                        break;
                     }
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                    // the tile kScaleRing before has been attended: its V was consumed for this stage
-                    if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
-#pragma unroll
-                    for (int e = 0; e < kTile / kN; ++e) {
-                        sk[me + e * kN] = kx[e];
-                        sk[kTile + me + e * kN] = vx[e];
+                    if (!wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag)) break;
+                    const char *src = smem + G::kRawAt + rs * G::kRawBytes;
+                    char *dst = ring + s * G::kTileBytes;
+    #pragma unroll 4
+                    for (int x = me; x < kTile * kChunks; x += kN) {
+                        const int r = x / kChunks, c = x % kChunks;
+                        uint4 a, b;
+                        i8x16_to_f16(*(const uint4 *)(src + x * 16), a, b);
+                        *(uint4 *)(dst + piece_at(r, 2 * c)) = a;
+                        *(uint4 *)(dst + piece_at(r, 2 * c + 1)) = b;
                     }
-                    if (lane == 0) vmost[j % G::kScaleRing][warp - 10] = most;
-                } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
-                    break;
+                    fence_proxy_async();
+                    mbar_arrive(&raw_empty[rs]);
+                    mbar_arrive(&full[s]);
                 }
-                if (!wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag)) break;
-                const char *src = smem + G::kRawAt + rs * G::kRawBytes;
-                char *dst = ring + s * G::kTileBytes;
-#pragma unroll 4
-                for (int x = me; x < kTile * kChunks; x += kN) {
-                    const int r = x / kChunks, c = x % kChunks;
-                    const uint4 w = *(const uint4 *)(src + x * 16);
-                    const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u,
-                                           w.w ^ 0x80808080u};
-                    uint4 a, b;
-                    a.x = i8x2_to_f16<0x4140>(u[0]); a.y = i8x2_to_f16<0x4342>(u[0]);
-                    a.z = i8x2_to_f16<0x4140>(u[1]); a.w = i8x2_to_f16<0x4342>(u[1]);
-                    b.x = i8x2_to_f16<0x4140>(u[2]); b.y = i8x2_to_f16<0x4342>(u[2]);
-                    b.z = i8x2_to_f16<0x4140>(u[3]); b.w = i8x2_to_f16<0x4342>(u[3]);
-                    char *o = dst + (c / 4) * (kTile * 128) + r * 128;
-                    *(uint4 *)(o + (((2 * (c % 4)) ^ (r & 7)) << 4)) = a;
-                    *(uint4 *)(o + (((2 * (c % 4) + 1) ^ (r & 7)) << 4)) = b;
-                }
-                fence_proxy_async();
-                mbar_arrive(&raw_empty[rs]);
-                mbar_arrive(&full[s]);
             }
         }
     } else {
+        more_registers();
         // ---- softmax: thread = row
         const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
         const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // key tiles of this warpgroup
@@ -517,28 +437,38 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
 #pragma unroll
             for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
             tc::wait_ld();
-            float z[kTile];
+            float2 z[kTile / 2];
             const float *sk = scales + (j % G::kScaleRing) * 2 * kTile;
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) z[c] = __uint_as_float(raw[c / 32][c % 32]);
+            for (int c = 0; c < kTile / 2; ++c)
+                z[c] = make_float2(__uint_as_float(raw[c / 16][2 * (c % 16)]),
+                                   __uint_as_float(raw[c / 16][2 * (c % 16) + 1]));
             if constexpr (I8) {
 #pragma unroll
-                for (int c = 0; c < kTile; c += 4) {
-                    const float4 s4 = *(const float4 *)(sk + c);
-                    z[c] *= s4.x; z[c + 1] *= s4.y; z[c + 2] *= s4.z; z[c + 3] *= s4.w;
+                for (int c = 0; c < kTile / 2; c += 2) {
+                    const float4 s4 = *(const float4 *)(sk + 2 * c);
+                    z[c] = mul2(z[c], make_float2(s4.x, s4.y));
+                    z[c + 1] = mul2(z[c + 1], make_float2(s4.z, s4.w));
                 }
             }
             if (j0 < first || j0 + kTile - 1 > last) {
                 const int x0 = first - j0, x1 = last - j0;
 #pragma unroll
-                for (int c = 0; c < kTile; ++c)
-                    if (c < x0 || c > x1) z[c] = kNegInf;
+                for (int c = 0; c < kTile / 2; ++c) {
+                    if (2 * c < x0 || 2 * c > x1) z[c].x = kNegInf;
+                    if (2 * c + 1 < x0 || 2 * c + 1 > x1) z[c].y = kNegInf;
+                }
             }
-            float best[4] = {z[0], z[1], z[2], z[3]};
+            float best[4] = {z[0].x, z[0].y, z[1].x, z[1].y};
 #pragma unroll
-            for (int c = 4; c < kTile; c += 4)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], z[c + e]);
+            for (int c = 2; c < kTile / 2 - 2; c += 4) {
+                best[0] = max3(best[0], z[c].x, z[c].y);
+                best[1] = max3(best[1], z[c + 1].x, z[c + 1].y);
+                best[2] = max3(best[2], z[c + 2].x, z[c + 2].y);
+                best[3] = max3(best[3], z[c + 3].x, z[c + 3].y);
+            }
+            best[0] = max3(best[0], z[kTile / 2 - 2].x, z[kTile / 2 - 2].y);
+            best[1] = max3(best[1], z[kTile / 2 - 1].x, z[kTile / 2 - 1].y);
             const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * zs;
             float keep = 1.f;
             if (now > top + kGrow || (top == kNegInf && now > kNegInf)) {
@@ -571,44 +501,48 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
             }
             const float base = top == kNegInf ? 0.f : -top;
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 zs2 = make_float2(zs, zs), base2 = make_float2(base, base);
+            float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            constexpr int kStep = I8 ? 16 : 32;       // 32-bit columns of TMEM a store takes
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) {
-                z[c] = ex2(fmaf(z[c], zs, base));
-                part[c & 3] += z[c];
-            }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            if constexpr (I8) {
+            for (int c = 0; c < kTile / 2; c += kStep) {
+                uint32_t hi16[kStep], lo16[I8 ? kStep : 1];
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    uint32_t ph[16], pl[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 s4 = *(const float4 *)(sk + kTile + c + e);
-                        split2(z[c + e] * (s4.x * vinv), z[c + e + 1] * (s4.y * vinv), ph[e / 2], pl[e / 2]);
-                        split2(z[c + e + 2] * (s4.z * vinv), z[c + e + 3] * (s4.w * vinv), ph[e / 2 + 1],
-                               pl[e / 2 + 1]);
+                for (int e = 0; e < kStep; ++e) {
+                    float2 x = fma2(z[c + e], zs2, base2);
+                    if ((e & 7) < kFmaOf8) {
+                        x = ex2_fma2(x);
+                    } else {
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
                     }
-                    tc::st16(ts + c / 2, ph);
-                    tc::st16(ts + kTile / 2 + c / 2, pl);
+                    part[e & 1] = add2(part[e & 1], x);
+                    if constexpr (I8) {
+                        const float2 v2 = *(const float2 *)(sk + kTile + 2 * (c + e));
+                        x = mul2(x, mul2(v2, make_float2(vinv, vinv)));
+                        split2(x.x, x.y, hi16[e], lo16[e]);
+                    } else {
+                        // the softmax weights are rounded to the cache's type for the
+                        // product; their sum keeps 32 bits
+                        hi16[e] = pack2<BF>(x.x, x.y);
+                    }
                 }
-            } else {
-                // the softmax weights are rounded to the cache's type for the product;
-                // their sum keeps 32 bits
-#pragma unroll
-                for (int c = 0; c < kTile; c += 64) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) pk[e] = pack2<BF>(z[c + 2 * e], z[c + 2 * e + 1]);
-                    tc::st32(ts + c / 2, pk);
+                if constexpr (I8) {
+                    tc::st16(ts + c, hi16);
+                    tc::st16(ts + kTile / 2 + c, lo16);
+                } else {
+                    tc::st32(ts + c, hi16);
                 }
             }
+            part[0] = add2(part[0], part[1]);
+            sum += part[0].x + part[0].y;
             tc::wait_st();
             tc::fence_before();
             mbar_arrive(&p_full[w]);
         }
         if (mine > 0 && ok) ok = wait_phase(&o_full[w], 0, abort_flag);
         tc::fence_after();
+        if (top == kNegInf && sum == sum) sum = 0.f;  // no visible key (its weights counted as 2^-126 each)
         if (ok && (alt || w < tiles)) {
             const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
             const float lse = sum == 0.f ? kNegInf : (top == kNegInf ? 0.f : top) + log2f(sum);
@@ -661,6 +595,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     __syncthreads();
     tc::fence_after();
     if (warp == 8) tc::dealloc(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
 }
 
 // ---- host ------------------------------------------------------------------
@@ -713,6 +648,13 @@ bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long k
 }
 
 }  // namespace
+
+int read_and_clear_tile_fault() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tile_fault, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_tile_fault, &zero, sizeof(int));
+    return v ? 1 : 0;
+}
 
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
                          cudaStream_t st) {

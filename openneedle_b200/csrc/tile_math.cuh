@@ -1,0 +1,196 @@
+// Arithmetic and tensor-core helpers of the attention tiles: paired FP32
+// instructions, powers of two, FP16 splits, swizzled operand descriptors,
+// bounded waits.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "tcgen05.cuh"
+
+namespace nb200 {
+namespace tile {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// Two FP32 operations an instruction, each rounded to nearest.
+__device__ __forceinline__ unsigned long long bits2(float2 a) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair2(unsigned long long a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return pair2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return pair2(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return pair2(r);
+}
+
+// 2^x of two values on the FP32 pipe, which relieves the special-function unit:
+// x = n + f with n the nearest integer (the sum with 1.5 * 2^23 leaves it in the
+// low bits), 2^f by a polynomial of degree 5 whose relative error on
+// [-1/2, 1/2] is least (Remez exchange: 7.5e-8, 2.1e-7 with FP32 roundings), n
+// added to the exponent.  x below -126 counts as -126.
+__device__ __forceinline__ float2 ex2_fma2(float2 x) {
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 big = make_float2(12582912.f, 12582912.f);
+    const float2 r = add2(x, big);
+    const float2 f = add2(x, mul2(add2(r, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f)));
+    float2 y = make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
+    y = fma2(y, f, make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
+    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
+    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
+    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
+    return y;
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    } else {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+}
+
+// x = hi + lo in FP16: 22 significand bits of each value within range
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// The powers of two that bring a row's largest absolute value to [2^12, 2^13)
+// (an FP16 pair then keeps 22 bits of every value that matters beside it), and back.
+__device__ __forceinline__ void row_scale(float most, float &up, float &down) {
+    const int ex = most > 0.f ? min(max((int)((__float_as_uint(most) >> 23) & 255) - 127, -100), 100) : 0;
+    up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
+    down = __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+}
+
+// Two FP16 values of two int8 codes, exactly: the code plus 128 put into the
+// low bits of 1024.0 gives 1024 + 128 + code, from which 1152 is taken.  `u`
+// holds four codes with their sign bits flipped; SEL picks the two bytes.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t i8x2_to_f16(uint32_t u) {
+    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// Sixteen codes to FP16, in order.
+__device__ __forceinline__ void i8x16_to_f16(uint4 w, uint4 &a, uint4 &b) {
+    const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+    a = make_uint4(i8x2_to_f16<0x4140>(u[0]), i8x2_to_f16<0x4342>(u[0]), i8x2_to_f16<0x4140>(u[1]),
+                   i8x2_to_f16<0x4342>(u[1]));
+    b = make_uint4(i8x2_to_f16<0x4140>(u[2]), i8x2_to_f16<0x4342>(u[2]), i8x2_to_f16<0x4140>(u[3]),
+                   i8x2_to_f16<0x4342>(u[3]));
+}
+
+constexpr int kTile = 128;   // rows of a tile, keys of a step
+
+// 128-byte swizzled operands: rows of 128 bytes in atoms of 8 rows, a 16-byte
+// piece c of row r at piece c ^ (r % 8).  K-major (Q, K): SBO = 1024 between
+// 8-row groups.  MN-major (V, whose keys are the rows and whose dimensions run
+// along them): SBO = 1024 between groups of 8 keys, LBO between chunks of 64
+// dimensions.
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(kTile * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// Byte of 16-byte piece c of row r in a tile of kTile rows of HD 16-bit values.
+__device__ __forceinline__ int piece_at(int r, int c) {
+    return (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+// kind::f16, M = 128, f32 accumulator: types at bits 7 and 10 (0 f16, 1 bf16), B
+// MN-major at bit 16, N / 8 at bit 17, M / 16 at bit 24.
+__host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int n) {
+    return (1u << 4) | ((uint32_t)bf << 7) | ((uint32_t)bf << 10) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] x B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(desc), "r"(acc)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// Bounded wait; on its end the CTA's warps give up (and the kernel raises its
+// fault flag).
+constexpr uint32_t kWaitLimit = 1u << 22;
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    const uint32_t a = smem_addr(bar);
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 255) == 255 && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+
+// Registers move between the warpgroups of a CTA of 384 threads of 168: two
+// softmax warpgroups of 208 and one of 88, 64512 in all as at the launch.
+constexpr int kTileThreads = 384;
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+
+}  // namespace tile
+}  // namespace nb200
