@@ -50,8 +50,8 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
 
 struct Plan {
     PrefixSplit prefix, own;
-    bool logits, row_lse;
-    long long part_o, part_lse, row_lse_at, logits_at, bytes;
+    bool logits, row_lse, weight_tiles;
+    long long part_o, part_lse, row_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
 
 int sm_count() {
@@ -94,6 +94,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     }
     p.logits = a.weights && a.tokens > 0 && !p.own.tiles;     // (the tile kernel's rows are too many to keep)
     p.row_lse = a.weights != nullptr;
+    p.weight_tiles = a.weights && p.own.tiles && R <= 128;
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long r = at;
@@ -107,6 +108,10 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     }
     if (p.row_lse) p.row_lse_at = take(rows * 4);
     if (p.logits) p.logits_at = take((long long)a.batch * a.kvheads * a.tokens * R * a.capacity * 4);
+    if (p.weight_tiles && a.cache_type == kCacheI8) {
+        p.q16_at = take(rows * a.head_dim * 4);
+        p.q16_scale_at = take(rows * 4);
+    }
     p.bytes = at;
     return p;
 }
@@ -182,7 +187,13 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
             return false;
     }
     if (!launch_prefix_finish(p, st)) return false;
-    return !a.weights || plan.logits || launch_key_weights(p, st);
+    if (!a.weights || plan.logits) return true;
+    if (!plan.weight_tiles) return launch_key_weights(p, st);
+    if (a.cache_type == kCacheI8) {
+        p.q16 = base + plan.q16_at;
+        p.q16_scale = reinterpret_cast<float *>(base + plan.q16_scale_at);
+    }
+    return launch_weight_tiles(p, st);
 }
 
 bool evict(const needle2_evict_args &a, cudaStream_t st) {

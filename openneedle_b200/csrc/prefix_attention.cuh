@@ -50,6 +50,8 @@ struct PrefixAttn {
     float *part_o;                                   // [slots][rows][hd], rows = B * tokens * heads as out's
     float *part_lse;                                 // [slots][rows]
     float *row_lse;                                  // [rows], log2 (null: not needed)
+    void *q16;                                       // weights of an INT8 cache's many rows: split queries
+    float *q16_scale;                                // and their factors
     float *logits;                                   // [B * kvheads][tokens * R][capacity], log2 (null: not kept)
 };
 
@@ -79,6 +81,8 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream
 // first axis of k and v.
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
                          cudaStream_t st);
+// Weights of many rows from row_lse (and, INT8, q16): group up to 128.
+bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st);
 // 1 if a bounded wait of the tile kernels ran out since the last call, -1 if
 // the flag could not be read.
 int read_and_clear_tile_fault();

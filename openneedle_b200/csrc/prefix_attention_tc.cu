@@ -31,6 +31,7 @@ using namespace tile;
 __device__ int g_tile_fault = 0;                 // a bounded wait ran out
 
 constexpr int kFmaOf8 = 2;                       // of 8 powers of two, those on the FP32 pipe
+constexpr int kWeightFmaOf8 = 3;                 // the same of the key weights
 constexpr float kGrow = 8.f;                     // log2 growth of a maximum that is left to the weights
 
 template <int TYPE, int HD>
@@ -598,6 +599,297 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
 }
 
+// ---- accumulated key weights ------------------------------------------------
+//
+// The logits once more, keys as the rows: S^T = K Q^T for two tiles of 128 keys
+// against 128 query rows at a time, and sum over the rows of 2^(z - lse_row).
+// Thread = key: the sum runs along the thread's TMEM lane, so no value crosses
+// threads and the order of the additions is fixed.  K stays in shared memory
+// for the whole CTA; the rows come by TMA, their lse beside them; two TMEM
+// buffers a tile let the next product run during the exponentials, which bound
+// the kernel (one a logit, on the special-function unit or the FP32 pipe).
+
+template <int TYPE, int HD>
+struct WeightGeom {
+    static constexpr bool I8 = TYPE == kCacheI8;
+    static constexpr int kPieces = I8 ? 2 : 1;
+    static constexpr int kTileBytes = kTile * HD * 2;
+    static constexpr int kStageBytes = kPieces * kTileBytes;      // 128 query rows
+    static constexpr int kStages = HD == 64 ? 4 : (I8 ? 2 : 4);
+    static constexpr int kRing = 2 * kTileBytes;                  // behind the two key tiles
+    static constexpr int kSmem = kRing + kStages * kStageBytes + 1024;
+    static_assert(kSmem <= 232448 - 6144, "shared memory of a CTA");
+};
+
+// FP32 queries as FP16 pairs: hi and lo rows [B][kvheads][tokens * R][hd] each
+// and the factor of every row, for the weights kernel's loads.
+template <int HD>
+__global__ __launch_bounds__(256) void split_queries_kernel(const PrefixAttn p) {
+    constexpr int kLanes = HD / 4, kPer = 256 / kLanes;
+    const long long rows = (long long)p.batch * p.tokens * p.heads;
+    const long long row = (long long)blockIdx.x * kPer + threadIdx.x / kLanes;
+    const int l = threadIdx.x % kLanes, TR = p.tokens * p.group;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) {
+        const long long bg = row / TR;
+        const int m = (int)(row % TR), b = (int)(bg / p.kvheads), g = (int)(bg % p.kvheads);
+        x = *(const float4 *)((const float *)p.q + b * p.qs[0] + m / p.group * p.qs[1] +
+                              (g * p.group + m % p.group) * p.qs[2] + 4 * l);
+    }
+    float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int d = kLanes / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    float up, down;
+    row_scale(most, up, down);
+    pdl_enter();      // the next kernel waits for this one only: so this one ends after its predecessor
+    if (row >= rows) return;
+    uint2 h, lo;
+    split2(x.x * up, x.y * up, h.x, lo.x);
+    split2(x.z * up, x.w * up, h.y, lo.y);
+    *(uint2 *)((char *)p.q16 + (row * HD + 4 * l) * 2) = h;
+    *(uint2 *)((char *)p.q16 + ((rows + row) * HD + 4 * l) * 2) = lo;
+    if (l == 0) p.q16_scale[row] = p.scale2 * down;
+}
+
+template <int TYPE, int HD>
+__global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const PrefixAttn p, int tile_rows,
+                                                                      const __grid_constant__ CUtensorMap mq) {
+    using G = WeightGeom<TYPE, HD>;
+    constexpr bool I8 = G::I8, BF = TYPE == kCacheBF16;
+    constexpr int kStages = G::kStages;
+    extern __shared__ __align__(16) char smem_raw[];
+    char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2][2], s_free[2][2];
+    __shared__ __align__(16) float lse[kStages][I8 ? 2 : 1][kTile];   // -lse of the rows, INT8: their factors
+    __shared__ uint32_t tmem_at;
+    __shared__ int abort_at;
+    volatile int *abort_flag = &abort_at;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int R = p.group, TR = p.tokens * R;
+    const int pairs = p.batch * p.kvheads, unit = blockIdx.x % pairs;
+    const int g = unit % p.kvheads, b = unit / p.kvheads, key0 = blockIdx.x / pairs * 2 * kTile;
+    const int len = own_length(p, b), nq = own_tokens(p, b), past = len - nq;   // own index of query 0
+    // the rows that see a key of this CTA: queries [t0, t1)
+    const int t0 = max(0, key0 - past);
+    const long long behind = p.window ? (long long)min(key0 + 2 * kTile, len) - 1 + p.window - past : nq;
+    const int t1 = (int)min((long long)nq, behind);
+    const int m0 = t0 * R, rows = key0 < len ? max(0, (t1 - t0) * R) : 0;
+    const int n = ceil_div(rows, tile_rows);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1 + 32);
+            mbar_init(&empty[i], 1 + 2 * kTile);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i >> 1][i & 1], 1);
+            mbar_init(&s_free[i >> 1][i & 1], kTile);
+        }
+        abort_at = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8) tc::alloc(&tmem_at, 512);
+    pdl_enter();
+    if (n > 0) {
+        // two tiles of keys (zeros where there are none)
+        constexpr int kChunks = HD * (I8 ? 1 : 2) / 16, kPer = kTileThreads / kChunks;
+        const long long crow = p.cache_row ? p.cache_row[b] : b;
+        const char *k = (const char *)p.k + (crow * p.ks[0] + g * p.ks[1]) * (I8 ? 1 : 2);
+        const long long step = p.ks[2] * (I8 ? 1 : 2);
+        const int c = threadIdx.x % kChunks;
+        for (int r0 = threadIdx.x / kChunks; r0 < 2 * kTile; r0 += 4 * kPer) {
+            uint4 x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = r0 + e * kPer;
+                x[e] = r < 2 * kTile && key0 + r < len ? *(const uint4 *)(k + (key0 + r) * step + c * 16)
+                                                       : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = r0 + e * kPer;
+                if (r >= 2 * kTile) continue;
+                char *t = smem + (r / kTile) * G::kTileBytes;
+                if constexpr (I8) {
+                    uint4 a, d;
+                    i8x16_to_f16(x[e], a, d);
+                    *(uint4 *)(t + piece_at(r % kTile, 2 * c)) = a;
+                    *(uint4 *)(t + piece_at(r % kTile, 2 * c + 1)) = d;
+                } else {
+                    *(uint4 *)(t + piece_at(r % kTile, c)) = x[e];
+                }
+            }
+        }
+        // rows behind a short tile stay what they are here: zeros
+        if (tile_rows < kTile) {
+            char *q = smem + G::kRing;
+            for (int i = threadIdx.x; i < kStages * G::kStageBytes / 16; i += kTileThreads)
+                *(uint4 *)(q + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    fence_proxy_async();
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp >= 8) {
+        if (warp == 9) {
+            // ---- query rows and their lse
+            int issued = 0;
+            const long long lrow = (long long)b * p.tokens;
+            for (int i = 0; i < n; ++i) {
+                const int s = i % kStages, mi = m0 + i * tile_rows, left = rows - i * tile_rows;
+                // (the loads ahead of the wait for the stage)
+                float l[kTile / 32], f[kTile / 32];
+#pragma unroll
+                for (int e = 0; e < kTile / 32; ++e) {
+                    const int x = lane + 32 * e, m = mi + x;
+                    l[e] = kNegInf;
+                    f[e] = 0.f;
+                    if (x < tile_rows && x < left) {
+                        l[e] = -p.row_lse[(lrow + m / R) * p.heads + g * R + m % R];
+                        if constexpr (I8) f[e] = p.q16_scale[(long long)unit * TR + m];
+                    }
+                }
+                if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+#pragma unroll
+                for (int e = 0; e < kTile / 32; ++e) {
+                    lse[s][0][lane + 32 * e] = l[e];
+                    if constexpr (I8) lse[s][1][lane + 32 * e] = f[e];
+                }
+                mbar_arrive(&full[s]);
+                if (lane == 0) {
+                    char *dst = smem + G::kRing + s * G::kStageBytes;
+                    mbar_arrive_expect_tx(&full[s], G::kPieces * HD * 2 * tile_rows);
+                    for (int x = 0; x < G::kPieces; ++x)
+                        for (int c = 0; c < HD / 64; ++c) {
+                            char *d = dst + x * G::kTileBytes + c * (kTile * 128);
+                            // rows (t, r): INT8 from the split copy [pieces][B * kvheads][tokens * R][hd]
+                            if constexpr (I8)
+                                tma_load_4d(d, &mq, 64 * c, mi, unit, x, &full[s]);
+                            else
+                                tma_load_4d(d, &mq, 64 * c, g * R, mi / R, b, &full[s]);
+                        }
+                }
+                ++issued;
+            }
+            if (lane == 0)
+                for (int i = max(0, issued - kStages); i < issued; ++i)
+                    mbar_wait(&full[i % kStages], (uint32_t)(i / kStages) & 1);
+            __syncwarp();
+        } else if (warp == 8 && lane == 0) {
+            // ---- products
+            constexpr uint32_t ids = idesc(BF, false, kTile);
+            const uint32_t k0 = smem_addr(smem), q0 = smem_addr(smem) + G::kRing;
+            for (int i = 0; i < n; ++i) {
+                const int s = i % kStages;
+                if (!wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag)) break;
+                bool ok = true;
+                for (int w = 0; w < 2; ++w) {
+                    if (i >= 2) ok = ok && wait_phase(&s_free[w][i & 1], (uint32_t)(i / 2 - 1) & 1, abort_flag);
+                    if (!ok) break;
+                    tc::fence_after();
+#pragma unroll
+                    for (int x = 0; x < G::kPieces; ++x)
+#pragma unroll
+                        for (int c = 0; c < HD / 16; ++c) {
+                            const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
+                            tc::mma_bf16_ss(tmem + (2 * w + (i & 1)) * kTile, desc_k(k0 + w * G::kTileBytes + at),
+                                            desc_k(q0 + s * G::kStageBytes + x * G::kTileBytes + at), ids, x + c > 0);
+                        }
+                    tc::commit(&s_full[w][i & 1]);
+                }
+                if (!ok) break;
+                tc::commit(&empty[s]);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- thread = key
+        const int w = warp >> 2, j = key0 + w * kTile + (threadIdx.x & (kTile - 1));
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        float ks = p.scale2;
+        if constexpr (I8) {
+            const long long crow = p.cache_row ? p.cache_row[b] : b;
+            ks = j < len ? p.kscale[crow * p.kss[0] + g * p.kss[1] + j * p.kss[2]] : 0.f;
+        }
+        // the rows that see the key: [from, to) of the CTA's
+        long long from = max(0LL, ((long long)j - past - t0) * R), to = rows;
+        if (p.window) to = min(to, ((long long)j + p.window - past - t0) * R);
+        if (j >= len) to = 0;
+        float total = 0.f;
+        const float2 k2 = make_float2(ks, ks);
+        for (int i = 0; i < n; ++i) {
+            const int s = i % kStages;
+            if (!wait_phase(&s_full[w][i & 1], (uint32_t)(i / 2) & 1, abort_flag)) break;
+            // (the rows' lse: written before the products' wait for the same phase)
+            if (!wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag)) break;
+            tc::fence_after();
+            const uint32_t ts = tmem + (2 * w + (i & 1)) * kTile + lanes;
+            uint32_t raw[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
+            tc::wait_ld();
+            tc::fence_before();
+            mbar_arrive(&s_free[w][i & 1]);
+            const int x0 = (int)max(0LL, min((long long)kTile, from - (long long)i * tile_rows));
+            const int x1 = (int)max(0LL, min((long long)kTile, to - (long long)i * tile_rows));
+            float2 part[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) part[c] = make_float2(0.f, 0.f);
+            const bool whole = x0 == 0 && x1 == kTile;
+            if (__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+                for (int c = 0; c < kTile; c += 4) {
+                    const float4 l4 = *(const float4 *)&lse[s][0][c];
+                    float2 a = make_float2(__uint_as_float(raw[c / 32][c % 32]),
+                                           __uint_as_float(raw[c / 32][c % 32 + 1]));
+                    float2 d = make_float2(__uint_as_float(raw[c / 32][c % 32 + 2]),
+                                           __uint_as_float(raw[c / 32][c % 32 + 3]));
+                    if constexpr (I8) {
+                        const float4 f4 = *(const float4 *)&lse[s][1][c];
+                        a = fma2(a, mul2(k2, make_float2(f4.x, f4.y)), make_float2(l4.x, l4.y));
+                        d = fma2(d, mul2(k2, make_float2(f4.z, f4.w)), make_float2(l4.z, l4.w));
+                    } else {
+                        a = fma2(a, k2, make_float2(l4.x, l4.y));
+                        d = fma2(d, k2, make_float2(l4.z, l4.w));
+                    }
+                    if ((c / 4) % 8 < kWeightFmaOf8)
+                        a = ex2_fma2(a);
+                    else
+                        a = make_float2(ex2(a.x), ex2(a.y));
+                    if ((c / 4) % 8 < kWeightFmaOf8)
+                        d = ex2_fma2(d);
+                    else
+                        d = make_float2(ex2(d.x), ex2(d.y));
+                    part[(c / 4) & 1] = add2(part[(c / 4) & 1], a);
+                    part[2 + ((c / 4) & 1)] = add2(part[2 + ((c / 4) & 1)], d);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kTile; ++c) {
+                    float f = ks;
+                    if constexpr (I8) f *= lse[s][1][c];
+                    const float y = ex2(fmaf(__uint_as_float(raw[c / 32][c % 32]), f, lse[s][0][c]));
+                    if (c >= x0 && c < x1) part[c & 3].x += y;
+                }
+            }
+            mbar_arrive(&empty[s]);
+            part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+            total += part[0].x + part[0].y;
+        }
+        if (j < p.capacity)
+            p.weights_out[b * p.wos[0] + g * p.wos[1] + j * p.wos[2]] =
+                p.weights[b * p.ws[0] + g * p.ws[1] + j * p.ws[2]] + total;
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 8) tc::dealloc(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
+}
+
 // ---- host ------------------------------------------------------------------
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -645,6 +937,21 @@ bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long k
         return false;
     }
     return true;
+}
+
+}  // namespace
+
+namespace {
+
+template <typename F>
+bool by_geometry(const PrefixAttn &p, F f) {
+    using I8 = std::integral_constant<int, kCacheI8>;
+    using BF = std::integral_constant<int, kCacheBF16>;
+    using F16 = std::integral_constant<int, kCacheF16>;
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (p.hd == 64) return p.type == kCacheI8 ? f(I8(), D64()) : p.type == kCacheBF16 ? f(BF(), D64()) : f(F16(), D64());
+    return p.type == kCacheI8 ? f(I8(), D128()) : p.type == kCacheBF16 ? f(BF(), D128()) : f(F16(), D128());
 }
 
 }  // namespace
@@ -702,15 +1009,67 @@ bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const P
         NB_CUDA_TRY(cudaGetLastError());
         return true;
     };
-    if (p.hd == 64) {
-        if (p.type == kCacheI8) return run(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 64>());
-        if (p.type == kCacheBF16)
-            return run(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 64>());
-        return run(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 64>());
-    }
-    if (p.type == kCacheI8) return run(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 128>());
-    if (p.type == kCacheBF16) return run(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 128>());
-    return run(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 128>());
+    return by_geometry(p, run);
+}
+
+bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st) {
+    auto run = [&](auto type, auto hd) -> bool {
+        using G = WeightGeom<type(), hd()>;
+        auto fn = encoder();
+        if (!fn) {
+            set_error("cuTensorMapEncodeTiled is unavailable");
+            return false;
+        }
+        const int R = p.group, tile_rows = kTile / R * R;
+        const long long rows = (long long)p.batch * p.tokens * p.heads;
+        CUtensorMap mq{};
+        CUresult r;
+        const cuuint32_t estr[4] = {1, 1, 1, 1};
+        if constexpr (G::I8) {
+            // [2][B * kvheads][tokens * R][hd], the split copy
+            const long long TR = (long long)p.tokens * R, units = (long long)p.batch * p.kvheads;
+            const cuuint64_t dims[4] = {(cuuint64_t)hd(), (cuuint64_t)TR, (cuuint64_t)units, 2};
+            const cuuint64_t strides[3] = {(cuuint64_t)hd() * 2, (cuuint64_t)(TR * hd() * 2),
+                                           (cuuint64_t)(rows * hd() * 2)};
+            const cuuint32_t box[4] = {64, (cuuint32_t)tile_rows, 1, 1};
+            r = fn(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, p.q16, dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        } else {
+            // [B][tokens][heads][hd]: R heads of tile_rows / R tokens a box
+            auto stride = [&](long long s, int n) { return (cuuint64_t)(n > 1 ? s * 2 : hd() * 2); };
+            const cuuint64_t dims[4] = {(cuuint64_t)hd(), (cuuint64_t)p.heads, (cuuint64_t)p.tokens,
+                                        (cuuint64_t)p.batch};
+            const cuuint64_t strides[3] = {stride(p.qs[2], p.heads), stride(p.qs[1], p.tokens),
+                                           stride(p.qs[0], p.batch)};
+            const cuuint32_t box[4] = {64, (cuuint32_t)R, (cuuint32_t)(tile_rows / R), 1};
+            r = fn(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(p.q), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        }
+        if (r != CUDA_SUCCESS) {
+            set_error("prefix attention: the queries' strides cannot be described to the copy engine");
+            return false;
+        }
+        if constexpr (G::I8) {
+            const int per = 256 / (hd() / 4);
+            NB_CUDA_TRY(launch_pdl(split_queries_kernel<hd()>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0,
+                                   st, p));
+        }
+        auto kernel = weight_tile_kernel<type(), hd()>;
+        static bool configured[64] = {};
+        int dev = 0;
+        NB_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            NB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+        const int blocks = p.batch * p.kvheads * ceil_div(p.capacity, 2 * kTile);
+        if (blocks == 0) return true;
+        NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kTileThreads), (size_t)G::kSmem, st, p, tile_rows, mq));
+        return true;
+    };
+    return by_geometry(p, run);
 }
 
 }  // namespace nb200
