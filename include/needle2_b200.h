@@ -258,26 +258,24 @@ typedef struct {
     int window;                                    /* 0: every own key up to the query */
     int cache_type;                                /* 0 INT8 with scales, 1 bf16, 2 f16 */
     float scale;                                   /* softmax scale, positive */
-    const void *q;                                 /* [batch][tokens][heads][head_dim] */
-    long long q_stride[3];                         /* batch, token, head */
-    void *out;                                     /* like q; not overlapping the inputs */
-    long long out_stride[3];
-    const void *k, *v;                             /* [batch][kvheads][capacity][head_dim] */
+    long long q_stride[3], out_stride[3];          /* batch, token, head */
     long long k_stride[3], v_stride[3];            /* batch, KV head, key */
-    const float *k_scales, *v_scales;              /* [batch][kvheads][capacity], INT8 only */
     long long k_scale_stride[3], v_scale_stride[3];
-    const void *prefix_k, *prefix_v;               /* [kvheads][prefix][head_dim] */
-    long long prefix_k_stride[2], prefix_v_stride[2];
-    const float *prefix_k_scales, *prefix_v_scales; /* [kvheads][prefix], INT8 only */
+    long long prefix_k_stride[2], prefix_v_stride[2];             /* KV head, key */
     long long prefix_k_scale_stride[2], prefix_v_scale_stride[2];
+    long long weights_stride[3], weights_out_stride[3];
+    const void *q;                                 /* [batch][tokens][heads][head_dim] */
+    void *out;                                     /* like q; not overlapping the inputs */
+    const void *k, *v;                             /* [batch][kvheads][capacity][head_dim] */
+    const float *k_scales, *v_scales;              /* [batch][kvheads][capacity], INT8 only */
+    const void *prefix_k, *prefix_v;               /* [kvheads][prefix][head_dim] */
+    const float *prefix_k_scales, *prefix_v_scales; /* [kvheads][prefix], INT8 only */
     const int *lengths;                            /* [batch] own keys */
     const int *token_counts;                       /* [batch] queries, or NULL: `tokens` each */
     const int *cache_rows;                         /* [batch] row of k, v and scales, or NULL: the sequence's index */
     float *lse;                                    /* [batch][tokens][heads], or NULL */
     const float *weights;                          /* [batch][kvheads][capacity], or NULL: no weights */
-    long long weights_stride[3];
     float *weights_out;                            /* may be `weights` itself, with the same strides */
-    long long weights_out_stride[3];
 } needle2_prefix_attention_args;
 
 /* Bytes of device workspace of a call with these sizes (pointers are not read;
@@ -303,19 +301,13 @@ int needle2_prefix_attention_device(const needle2_prefix_attention_args *args, v
 typedef struct {
     int batch, kvheads, head_dim, capacity, out_capacity, keep, first, recent;
     int cache_type;
+    long long k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3], weights_stride[3];
+    long long k_out_stride[3], v_out_stride[3], k_scale_out_stride[3], v_scale_out_stride[3], weights_out_stride[3];
     const void *k, *v;
-    long long k_stride[3], v_stride[3];
-    const float *k_scales, *v_scales;
-    long long k_scale_stride[3], v_scale_stride[3];
-    const float *weights;
-    long long weights_stride[3];
+    const float *k_scales, *v_scales, *weights;
     const int *lengths;
     void *k_out, *v_out;
-    long long k_out_stride[3], v_out_stride[3];
-    float *k_scales_out, *v_scales_out;
-    long long k_scale_out_stride[3], v_scale_out_stride[3];
-    float *weights_out;
-    long long weights_out_stride[3];
+    float *k_scales_out, *v_scales_out, *weights_out;
     int *indices, *lengths_out;
 } needle2_evict_args;
 int needle2_evict_device(const needle2_evict_args *args, void *stream);

@@ -9,6 +9,7 @@ CUDA tensors and do not synchronise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as ct
 import functools
 import struct
@@ -187,10 +188,11 @@ class KVCache:
 # without synchronising, allocate through torch (results and workspace belong to
 # that stream, so captured graphs each keep their own) and have no gradients.
 
-# needle2_prefix_attention_args and needle2_evict_args, field by field
-_ATTENTION_ARGS = struct.Struct("@9i f P 3q P 3q 2P 6q 2P 6q 2P 4q 2P 4q 3P P P 3q P 3q")
-_EVICT_ARGS = struct.Struct("@9i 0q 2P 6q 2P 6q P 3q P 2P 6q 2P 6q P 3q 2P")
-_NO_STRIDES2, _NO_STRIDES3 = (0, 0), (0, 0, 0)
+# needle2_prefix_attention_args and needle2_evict_args: sizes and strides, then the pointers
+_ATTENTION_SIZES = struct.Struct("@9if32q")
+_ATTENTION_POINTERS = struct.Struct("@16P")
+_EVICT_SIZES = struct.Struct("@9i0q30q")
+_EVICT_POINTERS = struct.Struct("@13P")
 
 
 class Evicted(NamedTuple):
@@ -215,7 +217,14 @@ def _bind_operators():
     lib.needle2_evict_device.restype = _i
     import torch
     types = {torch.int8: (0, torch.float32), torch.bfloat16: (1, torch.bfloat16), torch.float16: (2, torch.float16)}
-    return lib, torch, types
+
+    def current_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+    return lib, torch, types, getattr(torch._C, "_cuda_getCurrentRawStream", current_stream)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on_stream(torch, device, stream):
@@ -223,7 +232,7 @@ def _on_stream(torch, device, stream):
     if device.type != "cuda":
         raise ValueError("the operators run on CUDA tensors")
     if stream is None:
-        return torch.cuda.device(device)
+        return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
         handle = _stream_ptr(stream)
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
@@ -233,7 +242,7 @@ def _on_stream(torch, device, stream):
 
 
 def _want(x, name, shape, dtype, device, last=True):
-    if x.dtype != dtype or x.device != device or x.shape != shape:
+    if x.dtype != dtype or x.shape != shape or x.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}, got {x.dtype} "
                          f"{tuple(x.shape)} on {x.device}")
     if last and x.stride(-1) != 1 and x.shape[-1] > 1:
@@ -242,22 +251,26 @@ def _want(x, name, shape, dtype, device, last=True):
 
 def _span(x):
     """First and past-the-last byte that a tensor's elements take."""
-    if not x.numel():
+    size = x.nbytes
+    if not size:
         return 0, 0
     a = x.data_ptr()
-    return a, a + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+    if not x.is_contiguous():
+        size = (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+    return a, a + size
 
 
-def _apart(out, inputs, name):
-    """Refuse an output that shares memory with an input, or with itself."""
-    if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
-        raise ValueError(f"{name} must not be expanded")
-    a0, a1 = _span(out)
-    for x in inputs:
-        if x is not None:
-            b0, b1 = _span(x)
-            if a0 < b1 and b0 < a1:
-                raise ValueError(f"{name} overlaps an input")
+def _apart(outs, inputs):
+    """Refuse outputs [(tensor, name)] that share memory with an input, with one another, or with themselves."""
+    taken = [_span(x) for x in inputs if x is not None]
+    for x, name in outs:
+        if not x.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride())):
+            raise ValueError(f"{name} must not be expanded")
+        a, b = _span(x)
+        for c, d in taken:
+            if a < d and c < b:
+                raise ValueError(f"{name} overlaps an input or another output")
+        taken.append((a, b))
 
 
 def _no_gradients(torch, *tensors):
@@ -265,54 +278,77 @@ def _no_gradients(torch, *tensors):
         raise ValueError("these operators have no gradients: detach the inputs or call them under torch.no_grad()")
 
 
-def _cache_operands(torch, types, k, v, k_scales, v_scales, lead, keys, head_dim, name):
-    """Check K, V and their scales of a cache [*lead, keys, head_dim]; their pointers and strides."""
-    dtype, device, shape = k.dtype, k.device, (*lead, keys, head_dim)
-    _want(k, name + "k", shape, dtype, device)
-    _want(v, name + "v", shape, dtype, device)
-    if dtype == torch.int8:
+def _want_cache(torch, k, v, k_scales, v_scales, shape, name):
+    """Check K, V and their scales of a cache of the given shape."""
+    _want(k, name + "k", shape, k.dtype, k.device)
+    _want(v, name + "v", shape, k.dtype, k.device)
+    if k.dtype == torch.int8:
         if k_scales is None or v_scales is None:
             raise ValueError(f"an INT8 cache needs {name}k_scales and {name}v_scales")
-        _want(k_scales, name + "k_scales", shape[:-1], torch.float32, device, last=False)
-        _want(v_scales, name + "v_scales", shape[:-1], torch.float32, device, last=False)
-        return (k.data_ptr(), v.data_ptr(), *k.stride()[:-1], *v.stride()[:-1],
-                k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride(), *v_scales.stride())
-    if k_scales is not None or v_scales is not None:
+        _want(k_scales, name + "k_scales", shape[:-1], torch.float32, k.device, last=False)
+        _want(v_scales, name + "v_scales", shape[:-1], torch.float32, k.device, last=False)
+    elif k_scales is not None or v_scales is not None:
         raise ValueError(f"{name}k_scales and {name}v_scales belong to INT8 caches only")
-    return (k.data_ptr(), v.data_ptr(), *k.stride()[:-1], *v.stride()[:-1], 0, 0, *([0] * (2 * len(lead) + 2)))
 
 
-def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
-            prefix_v_scales, tokens, window, scale, out, return_lse, stream):
-    lib, torch, types = _bind_operators()
+def _strides(axes, *tensors):
+    """The first `axes` strides of each tensor, zeros for None."""
+    return [n for x in tensors for n in ((0,) * axes if x is None else x.stride()[:axes])]
+
+
+def _layout(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.device)
+
+
+def _pointer(x):
+    return 0 if x is None else x.data_ptr()
+
+
+# What the checks of a call's shapes, strides, types and options came to: its
+# packed sizes and workspace, by those alone.
+_plans = {}
+_MOST_PLANS = 512
+
+
+def _remember(key, plan):
+    if len(_plans) >= _MOST_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales,
+                    prefix_k_scales, prefix_v_scales, tokens, window, scale, out):
+    """Check a call; its packed sizes, its workspace's bytes, its result's type."""
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
     device = k.device
     cache_type, qtype = types[k.dtype]
-    single = q.dim() == 3                              # one token per sequence
     if q.dim() not in (3, 4):
         raise ValueError("q must be [batch, tokens, heads, head_dim], or [batch, heads, head_dim] for one token")
-    q4 = q.unsqueeze(1) if single else q
-    count, heads = q4.shape[1], q4.shape[2]
-    _want(q4, "q", (batch, count, heads, head_dim), qtype, device)
-    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights)
-    own = _cache_operands(torch, types, k, v, k_scales, v_scales, (batch, kvheads), capacity, head_dim, "")
+    single = q.dim() == 3
+    count, heads = (1, q.shape[1]) if single else q.shape[1:3]
+    _want(q, "q", (batch, heads, head_dim) if single else (batch, count, heads, head_dim), qtype, device)
+    _want_cache(torch, k, v, k_scales, v_scales, (batch, kvheads, capacity, head_dim), "")
     prefix = 0
-    shared = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     if (prefix_k is None) != (prefix_v is None):
         raise ValueError("prefix_k and prefix_v go together")
     if prefix_k is not None:
-        prefix = prefix_k.shape[1] if prefix_k.dim() == 3 else -1
-        if prefix_k.dtype != k.dtype or prefix_k.device != device or prefix < 0:
+        if prefix_k.dim() != 3 or prefix_k.dtype != k.dtype or prefix_k.device != device:
             raise ValueError("prefix_k and prefix_v must be [kvheads, prefix, head_dim] of the cache's type and device")
-        shared = _cache_operands(torch, types, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales, (kvheads,),
-                                 prefix, head_dim, "prefix_")
+        prefix = prefix_k.shape[1]
+        _want_cache(torch, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales, (kvheads, prefix, head_dim),
+                    "prefix_")
     elif prefix_k_scales is not None or prefix_v_scales is not None:
         raise ValueError("prefix scales without a prefix")
     _want(lengths, "lengths", (batch,), torch.int32, device)
     if tokens is not None:
         _want(tokens, "tokens", (batch,), torch.int32, device)
+        if not tokens.is_contiguous():
+            raise ValueError("tokens must be contiguous")
+    if not lengths.is_contiguous():
+        raise ValueError("lengths must be contiguous")
     window = int(window)
     if window < 0:
         raise ValueError("window must not be negative")
@@ -322,36 +358,64 @@ def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales
         _want(weights, "weights", (batch, kvheads, capacity), torch.float32, device, last=False)
     if out is not None:
         _want(out, "out", q.shape, qtype, device)
-        _apart(out, (q, k, v, prefix_k, prefix_v, lengths, tokens, weights, k_scales, v_scales, prefix_k_scales,
-                     prefix_v_scales, weights_out), "out")
     if weights_out is not None:
         _want(weights_out, "weights_out", (batch, kvheads, capacity), torch.float32, device, last=False)
-        same = weights_out.data_ptr() == weights.data_ptr() and weights_out.stride() == weights.stride()
-        _apart(weights_out, (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales,
-                             prefix_v_scales, None if same else weights), "weights_out")
+    weigh = weights is not None and capacity > 0
+
+    def rows(x):                                           # batch, token, head
+        if x is None:                                      # a new tensor
+            return [count * heads * head_dim, heads * head_dim, head_dim]
+        return [x.stride(0), 0, x.stride(1)] if single else list(x.stride()[:3])
+
+    wide = [kvheads * capacity, capacity, 1] if weights_out is None else list(weights_out.stride())
+    sizes = _ATTENTION_SIZES.pack(
+        batch, count, heads, kvheads, head_dim, prefix, capacity, window, cache_type, scale, *rows(q), *rows(out),
+        *_strides(3, k, v, k_scales, v_scales), *_strides(2, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales),
+        *_strides(3, weights), *wide)
+    one = 4096 if weigh else 0                             # (given or not: the pointers are not read)
+    size = lib.needle2_prefix_attention_workspace(sizes + _ATTENTION_POINTERS.pack(*[4096] * 14, one, one))
+    if size < 0:
+        raise ValueError(last_error())
+    return sizes, size, (batch, count, heads), weigh
+
+
+def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
+            prefix_v_scales, tokens, window, scale, out, return_lse, stream):
+    lib, torch, types, raw_stream = _bind_operators()
+    key = (_layout(q), _layout(k), _layout(v), _layout(lengths), _layout(weights), _layout(weights_out),
+           _layout(prefix_k), _layout(prefix_v), _layout(k_scales), _layout(v_scales), _layout(prefix_k_scales),
+           _layout(prefix_v_scales), _layout(tokens), window, scale, _layout(out))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, prefix_k,
+                                              prefix_v, k_scales, v_scales, prefix_k_scales, prefix_v_scales, tokens,
+                                              window, scale, out))
+    sizes, size, rows, weigh = plan
+    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights)
+    device = k.device
+    if out is not None or weights_out is not None:
+        same = weights_out is not None and weights_out.data_ptr() == weights.data_ptr() and \
+            weights_out.stride() == weights.stride()
+        outs = [] if out is None else [(out, "out")]
+        if weights_out is not None:
+            outs.append((weights_out, "weights_out"))
+        _apart(outs, (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales,
+                      prefix_v_scales, None if same else weights))
     with _on_stream(torch, device, stream):
         if out is None:
-            out = torch.empty(q.shape, dtype=qtype, device=device)
-        lse = torch.empty((batch, count, heads), dtype=torch.float32, device=device) if return_lse else None
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lse = torch.empty(rows, dtype=torch.float32, device=device) if return_lse else None
         if weights is not None and weights_out is None:
-            weights_out = torch.empty((batch, kvheads, capacity), dtype=torch.float32, device=device)
-        weigh = weights is not None and capacity > 0
-        o = out.stride()
-        o3 = (o[0], 0, o[1]) if single else o[:3]
-        args = _ATTENTION_ARGS.pack(
-            batch, count, heads, kvheads, head_dim, prefix, capacity, window, cache_type, scale,
-            q4.data_ptr(), *q4.stride()[:3], out.data_ptr(), *o3, *own, *shared, lengths.data_ptr(),
-            0 if tokens is None else tokens.data_ptr(), 0, 0 if lse is None else lse.data_ptr(),
-            weights.data_ptr() if weigh else 0, *(weights.stride() if weigh else _NO_STRIDES3),
-            weights_out.data_ptr() if weigh else 0, *(weights_out.stride() if weigh else _NO_STRIDES3))
-        size = lib.needle2_prefix_attention_workspace(args)
-        if size < 0:
-            raise ValueError(last_error())
+            weights_out = torch.empty(weights.shape, dtype=torch.float32, device=device)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _check(lib.needle2_prefix_attention_device(args, workspace.data_ptr() if size else None, size,
-                                                   torch.cuda.current_stream(device).cuda_stream),
-               "prefix_attention")
-    if return_lse and single:
+        args = sizes + _ATTENTION_POINTERS.pack(
+            q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales),
+            _pointer(prefix_k), _pointer(prefix_v), _pointer(prefix_k_scales), _pointer(prefix_v_scales),
+            lengths.data_ptr(), _pointer(tokens), 0, _pointer(lse), weights.data_ptr() if weigh else 0,
+            weights_out.data_ptr() if weigh else 0)
+        if lib.needle2_prefix_attention_device(args, _pointer(workspace), size, raw_stream(device.index)):
+            _check(-1, "prefix_attention")
+    if return_lse and q.dim() == 3:
         lse = lse.squeeze(1)
     return out, lse, weights_out
 
@@ -411,55 +475,74 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     The result goes to ``out`` (an ``Evicted`` of tensors with n >= keep slots),
     to the inputs themselves (``in_place``; lengths and indices are new), or to
     new tensors of ``keep`` slots, zero behind the kept keys."""
-    lib, torch, types = _bind_operators()
+    lib, torch, types, raw_stream = _bind_operators()
+    key = (_layout(k), _layout(v), _layout(weights), _layout(lengths), _layout(k_scales), _layout(v_scales), keep, first,
+           recent, in_place, None if out is None else tuple(map(_layout, out)))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales,
+                                          out, in_place))
+    sizes, shape = plan
+    _no_gradients(torch, k, v, weights)
+    device = k.device
+    with _on_stream(torch, device, stream):
+        if in_place:
+            _apart([(x, "the cache") for x in (k, v, weights, k_scales, v_scales) if x is not None], (lengths,))
+            out = Evicted(k, v, weights, torch.empty(shape[:1], dtype=torch.int32, device=device),
+                          torch.empty(shape, dtype=torch.int32, device=device), k_scales, v_scales)
+        elif out is None:
+            f32 = {"dtype": torch.float32, "device": device}
+            out = Evicted(torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device),
+                          torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device), torch.empty(shape, **f32),
+                          torch.empty(shape[:1], dtype=torch.int32, device=device),
+                          torch.empty(shape, dtype=torch.int32, device=device),
+                          None if k_scales is None else torch.zeros(shape, **f32),
+                          None if v_scales is None else torch.zeros(shape, **f32))
+        else:
+            out = Evicted(*out)
+            _apart([(x, "out") for x in out if x is not None], (k, v, weights, lengths, k_scales, v_scales))
+        args = sizes + _EVICT_POINTERS.pack(
+            k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales), weights.data_ptr(), lengths.data_ptr(),
+            out.k.data_ptr(), out.v.data_ptr(), _pointer(out.k_scales), _pointer(out.v_scales), out.weights.data_ptr(),
+            out.indices.data_ptr(), out.lengths.data_ptr())
+        if lib.needle2_evict_device(args, raw_stream(device.index)):
+            _check(-1, "evict")
+    return out
+
+
+def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales, out, in_place):
+    """Check an eviction; its packed sizes and [batch, kvheads, keep]."""
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
     device, keep, first, recent = k.device, int(keep), int(first), int(recent)
     if keep < 0 or first < 0 or recent < 0 or first + recent > keep:
         raise ValueError("first and recent must not be negative, nor exceed keep together")
-    _no_gradients(torch, k, v, weights)
-    cache = _cache_operands(torch, types, k, v, k_scales, v_scales, (batch, kvheads), capacity, head_dim, "")
+    _want_cache(torch, k, v, k_scales, v_scales, (batch, kvheads, capacity, head_dim), "")
     _want(weights, "weights", (batch, kvheads, capacity), torch.float32, device, last=False)
     _want(lengths, "lengths", (batch,), torch.int32, device)
-    int8 = k.dtype == torch.int8
-    with _on_stream(torch, device, stream):
-        if in_place:
-            if out is not None:
-                raise ValueError("evict: out and in_place exclude each other")
-            if keep > capacity:
-                raise ValueError("evict: in place, keep must not exceed the capacity")
-            for x in (k, v, weights, k_scales, v_scales):
-                if x is not None:
-                    _apart(x, [y for y in (k, v, weights, lengths, k_scales, v_scales) if y is not x], "the cache")
-            out = Evicted(k, v, weights, torch.empty(batch, dtype=torch.int32, device=device),
-                          torch.empty((batch, kvheads, keep), dtype=torch.int32, device=device), k_scales, v_scales)
-        elif out is None:
-            shape = (batch, kvheads, keep)
-            f32 = {"dtype": torch.float32, "device": device}
-            out = Evicted(torch.zeros((*shape, head_dim), dtype=k.dtype, device=device),
-                          torch.zeros((*shape, head_dim), dtype=k.dtype, device=device), torch.empty(shape, **f32),
-                          torch.empty(batch, dtype=torch.int32, device=device),
-                          torch.empty(shape, dtype=torch.int32, device=device),
-                          torch.zeros(shape, **f32) if int8 else None, torch.zeros(shape, **f32) if int8 else None)
-        else:
-            out = Evicted(*out)
-            if out.k.dim() != 4 or out.k.shape[2] < keep or out.k.dtype != k.dtype or out.k.device != device:
-                raise ValueError("evict: out.k must be a cache of the input's type with at least keep slots")
-            _want(out.weights, "out.weights", (batch, kvheads, out.k.shape[2]), torch.float32, device, last=False)
-            _want(out.lengths, "out.lengths", (batch,), torch.int32, device)
-            _want(out.indices, "out.indices", (batch, kvheads, keep), torch.int32, device)
-            if not out.indices.is_contiguous():
-                raise ValueError("out.indices must be contiguous")
-            outs = [x for x in out if x is not None]
-            for i, x in enumerate(outs):
-                _apart(x, [k, v, weights, lengths, k_scales, v_scales, *outs[:i]], "out")
+    if not lengths.is_contiguous():
+        raise ValueError("lengths must be contiguous")
+    slots = keep
+    new = [kvheads * keep, keep, 1]
+    to = [keep * kvheads * head_dim, keep * head_dim, head_dim] * 2 + new * 2 + new
+    if in_place:
+        if out is not None:
+            raise ValueError("evict: out and in_place exclude each other")
+        if keep > capacity:
+            raise ValueError("evict: in place, keep must not exceed the capacity")
+        slots, to = capacity, _strides(3, k, v, k_scales, v_scales, weights)
+    elif out is not None:
+        out = Evicted(*out)
+        if out.k.dim() != 4 or out.k.shape[2] < keep or out.k.dtype != k.dtype or out.k.device != device:
+            raise ValueError("evict: out.k must be a cache of the input's type with at least keep slots")
         slots = out.k.shape[2]
-        packed = _cache_operands(torch, types, out.k, out.v, out.k_scales, out.v_scales, (batch, kvheads), slots,
-                                 head_dim, "out.")
-        args = _EVICT_ARGS.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
-                                *cache, weights.data_ptr(), *weights.stride(), lengths.data_ptr(), *packed,
-                                out.weights.data_ptr(), *out.weights.stride(), out.indices.data_ptr(),
-                                out.lengths.data_ptr())
-        _check(lib.needle2_evict_device(args, torch.cuda.current_stream(device).cuda_stream), "evict")
-    return out
+        _want_cache(torch, out.k, out.v, out.k_scales, out.v_scales, (batch, kvheads, slots, head_dim), "out.")
+        _want(out.weights, "out.weights", (batch, kvheads, slots), torch.float32, device, last=False)
+        _want(out.lengths, "out.lengths", (batch,), torch.int32, device)
+        _want(out.indices, "out.indices", (batch, kvheads, keep), torch.int32, device)
+        if not out.indices.is_contiguous() or not out.lengths.is_contiguous():
+            raise ValueError("out.indices and out.lengths must be contiguous")
+        to = _strides(3, out.k, out.v, out.k_scales, out.v_scales, out.weights)
+    return _EVICT_SIZES.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
+                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep)

@@ -180,11 +180,12 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
     if (a.tokens > 0) {
         const bool stream_prefix = plan.prefix.ranges && !plan.prefix.tiles;
         const bool stream_own = plan.own.ranges && !plan.own.tiles;
-        if ((stream_prefix || stream_own) && !launch_prefix_stream(p, stream_prefix, stream_own, st)) return false;
+        const bool tiles = plan.prefix.tiles || plan.own.tiles, stream = stream_prefix || stream_own;
         // the first axis of a cache addressed by cache_rows has an extent that only the caller knows
-        if ((plan.prefix.tiles || plan.own.tiles) &&
-            !launch_prefix_tiles(p, plan.prefix, plan.own, a.cache_rows ? 1LL << 30 : a.batch, st))
+        if (tiles &&
+            !launch_prefix_tiles(p, plan.prefix, plan.own, a.cache_rows ? 1LL << 30 : a.batch, stream, st))
             return false;
+        if (stream && !launch_prefix_stream(p, stream_prefix, stream_own, tiles, st)) return false;
     }
     if (!launch_prefix_finish(p, st)) return false;
     if (!a.weights || plan.logits) return true;

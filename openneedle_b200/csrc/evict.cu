@@ -9,6 +9,7 @@
 #include "common.cuh"
 #include "evict.cuh"
 #include "pdl.cuh"
+#include "sm100_async.cuh"
 
 namespace nb200 {
 namespace {
@@ -22,8 +23,172 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per (sequence, KV head): the key of the last weight that stays by
-// four passes over its bytes, then the positions in order.
+// Selection with a row's weights in registers: a cluster of C CTAs per
+// (sequence, KV head), each thread up to kMine weights of its CTA's contiguous
+// segment.  The key of the last weight that stays is found four bits at a time
+// from the top: every thread counts its keys by digit, the counts meet in shared
+// memory and, across the cluster, by distributed shared memory.  Then ties and
+// kept positions are ranked in index order, and everything is written.  The
+// weights are read once; bound by the latency of the eight rounds.
+constexpr int kMine = 16;
+
+template <int C, int T>
+__global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
+    constexpr int kWarpsIn = T / 32;
+    const int row = blockIdx.x / C, rank = blockIdx.x % C;
+    const int g = row % e.kvheads, b = row / e.kvheads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = max(0, min(e.lengths[b], e.capacity)), kept = min(n, e.keep);
+    const float *w = e.weights + b * e.ws[0] + g * e.ws[1];
+    float *wo = e.weights_o + b * e.wos[0] + g * e.wos[1];
+    int *idx = e.indices + (long long)row * e.keep;
+    __shared__ int counts[8][16];
+    __shared__ int ranks[2][kMine * kWarpsIn + 1];   // ties, kept: of (i, warp), then exclusive sums; last: their total
+    for (int i = tid; i < 128; i += T) (&counts[0][0])[i] = 0;
+
+    const int lo = e.first, hi = n - e.recent, seg = ceil_div(ceil_div(e.capacity, C), T) * T, j0 = rank * seg;
+    const int mine = min(kMine, ceil_div(max(0, min(seg, n - j0)), T));
+    float x[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int j = j0 + i * T + tid;
+        x[i] = i < mine && j < n ? w[j * e.ws[2]] : 0.f;
+    }
+    auto all_sync = [&] {
+        if constexpr (C > 1) {
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        } else {
+            __syncthreads();
+        }
+    };
+    // the value of another CTA's copy of a shared variable
+    auto of_cta = [&](const int *v, int cta) -> int {
+        if constexpr (C == 1) return *v;
+        uint32_t a = smem_addr(v), r;
+        int y;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(cta));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(y) : "r"(r) : "memory");
+        return y;
+    };
+    all_sync();                                      // counts are zero; no weight is read after this
+
+    const bool choose = n > e.keep;
+    int need = e.keep - e.first - e.recent;          // of the keys equal to `prefix` so far
+    const bool none = need == 0;
+    uint32_t prefix = 0;
+    if (choose && !none) {                           // the same in every CTA of the row
+        for (int it = 0; it < 8; ++it) {
+            const int shift = 28 - 4 * it;
+            const uint32_t mask = it == 0 ? 0u : ~0u << (shift + 4);
+            // sixteen counts of up to kMine: a byte each
+            uint32_t c[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                if (i >= mine) break;
+                const int j = j0 + i * T + tid;
+                const uint32_t u = weight_key(x[i]);
+                if (j >= lo && j < hi && (u & mask) == prefix) {
+                    const uint32_t d = (u >> shift) & 15, one = 1u << (8 * (d & 3));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) c[q] += q == (int)(d >> 2) ? one : 0u;
+                }
+            }
+            // of the warp: 16 bits each
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t even = __reduce_add_sync(0xffffffffu, c[q] & 0x00ff00ffu);
+                const uint32_t odd = __reduce_add_sync(0xffffffffu, (c[q] >> 8) & 0x00ff00ffu);
+                const uint32_t v = lane & 1 ? odd : even;
+                if (lane < 4 && v) atomicAdd(&counts[it][4 * q + lane], (int)(lane & 2 ? v >> 16 : v & 0xffff));
+            }
+            all_sync();
+            // every warp: lane d has digit d's total, then the digit in which the need-th largest lies
+            int mineof = 0;
+            if (lane < 16)
+                for (int r = 0; r < C; ++r) mineof += of_cta(&counts[it][15 - lane], r);   // from above
+            int above = mineof;
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, above, d);
+                if (lane >= d) above += y;
+            }
+            const unsigned at = __ballot_sync(0xffffffffu, lane < 16 && above >= need);
+            const int l = __ffs(at) - 1;
+            need -= __shfl_sync(0xffffffffu, above - mineof, l);
+            prefix |= (uint32_t)(15 - l) << shift;
+        }
+    }
+
+    // ranks of the ties: exclusive sums over (i, warp), then over the CTAs
+    auto exclusive = [&](int which) -> int {         // the CTA's own offset
+        int *v = ranks[which];
+        __syncthreads();
+        if (warp == 0) {
+            int carry = 0;
+            for (int k = 0; k < mine * kWarpsIn; k += 32) {
+                const int y = k + lane < mine * kWarpsIn ? v[k + lane] : 0;
+                int s = y;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int z = __shfl_up_sync(0xffffffffu, s, d);
+                    if (lane >= d) s += z;
+                }
+                if (k + lane < mine * kWarpsIn) v[k + lane] = carry + s - y;
+                carry += __shfl_sync(0xffffffffu, s, 31);
+            }
+            if (lane == 0) v[kMine * kWarpsIn] = carry;
+        }
+        all_sync();
+        int before = 0;
+        for (int r = 0; r < rank; ++r) before += of_cta(&v[kMine * kWarpsIn], r);
+        return before;
+    };
+    int tie_base = 0;
+    if (choose && !none) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (i >= mine) break;
+            const int j = j0 + i * T + tid;
+            const unsigned m = __ballot_sync(0xffffffffu, j >= lo && j < hi && weight_key(x[i]) == prefix);
+            if (lane == 0) ranks[0][i * kWarpsIn + warp] = __popc(m);
+        }
+        tie_base = exclusive(0);
+    }
+    uint32_t stays = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        if (i >= mine) break;
+        const int j = j0 + i * T + tid;
+        const uint32_t u = weight_key(x[i]);
+        const bool middle = choose && j >= lo && j < hi;
+        const bool tie = middle && !none && u == prefix;
+        const unsigned m = __ballot_sync(0xffffffffu, tie);
+        bool s = j < n && (!middle || (!none && u > prefix));
+        if (tie) s = tie_base + ranks[0][i * kWarpsIn + warp] + __popc(m & ((1u << lane) - 1)) < need;
+        const unsigned k = __ballot_sync(0xffffffffu, s);
+        if (lane == 0) ranks[1][i * kWarpsIn + warp] = __popc(k);
+        stays |= (uint32_t)s << i;
+    }
+    const int base = exclusive(1);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        if (i >= mine) break;
+        const bool s = stays >> i & 1;
+        const unsigned k = __ballot_sync(0xffffffffu, s);
+        if (s) {
+            const int at = base + ranks[1][i * kWarpsIn + warp] + __popc(k & ((1u << lane) - 1));
+            idx[at] = j0 + i * T + tid;
+            wo[at * e.wos[2]] = x[i];
+        }
+    }
+    for (int i = kept + rank * T + tid; i < e.keep; i += C * T) idx[i] = -1;
+    for (int i = kept + rank * T + tid; i < e.out_capacity; i += C * T) wo[i * e.wos[2]] = 0.f;
+    if (g == 0 && rank == 0 && tid == 0) e.lengths_o[b] = kept;
+    if constexpr (C > 1) all_sync();                 // no CTA ends while another reads its counts
+}
+
+// Selection of rows too long for that: one CTA per (sequence, KV head) reads the
+// weights in four passes over the keys' bytes, then ranks them in chunks.
 __global__ __launch_bounds__(kThreads) void evict_select_kernel(const Evict e) {
     const int g = blockIdx.x % e.kvheads, b = blockIdx.x / e.kvheads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -116,24 +281,51 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const Evict e) {
     if (g == 0 && tid == 0) e.lengths_o[b] = kept;
 }
 
-// Kept rows to other memory: a 16-byte piece of K and of V a thread.
-__global__ __launch_bounds__(256) void evict_gather_kernel(const Evict e, int chunks) {
-    pdl_enter();
+// Kept rows to other memory: 16-byte pieces of K and of V, kRowsOf rows of a
+// thread in flight at once.
+constexpr int kRowsOf = 4;
+
+__global__ __launch_bounds__(256) void evict_gather_kernel(const Evict e, int chunks, int pieces, int shift) {
     const int unit = blockIdx.x / chunks, g = unit % e.kvheads, b = unit / e.kvheads;
-    const int pieces = e.row_bytes / 16, rows = 256 / pieces;
-    const int piece = threadIdx.x % pieces;
+    const int rows = 256 >> shift, piece = threadIdx.x & (pieces - 1);
+    const int i0 = blockIdx.x % chunks * (kRowsOf * rows) + (threadIdx.x >> shift);
+    pdl_enter();
     const int kept = min(max(0, min(e.lengths[b], e.capacity)), e.keep);
-    const int i = blockIdx.x % chunks * rows + threadIdx.x / pieces;
-    if (i >= kept) return;
-    const long long j = e.indices[(long long)unit * e.keep + i];
-    const uint4 k = *(const uint4 *)(e.k + b * e.ks[0] + g * e.ks[1] + j * e.ks[2] + piece * 16);
-    const uint4 v = *(const uint4 *)(e.v + b * e.vs[0] + g * e.vs[1] + j * e.vs[2] + piece * 16);
-    *(uint4 *)(e.ko + b * e.kos[0] + g * e.kos[1] + i * e.kos[2] + piece * 16) = k;
-    *(uint4 *)(e.vo + b * e.vos[0] + g * e.vos[1] + i * e.vos[2] + piece * 16) = v;
-    if (piece == 0 && e.kscale) {
-        e.kscale_o[b * e.ksos[0] + g * e.ksos[1] + i * e.ksos[2]] = e.kscale[b * e.kss[0] + g * e.kss[1] + j * e.kss[2]];
-        e.vscale_o[b * e.vsos[0] + g * e.vsos[1] + i * e.vsos[2]] = e.vscale[b * e.vss[0] + g * e.vss[1] + j * e.vss[2]];
+    const int *idx = e.indices + (long long)unit * e.keep;
+    long long j[kRowsOf];
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r) j[r] = i0 + r * rows < kept ? idx[i0 + r * rows] : -1;
+    const char *k = e.k + b * e.ks[0] + g * e.ks[1] + piece * 16, *v = e.v + b * e.vs[0] + g * e.vs[1] + piece * 16;
+    uint4 x[kRowsOf], y[kRowsOf];
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r)
+        if (j[r] >= 0) {
+            x[r] = __ldcs((const uint4 *)(k + j[r] * e.ks[2]));
+            y[r] = __ldcs((const uint4 *)(v + j[r] * e.vs[2]));
+        }
+    float s[kRowsOf];
+    const bool scales = e.kscale && piece < 2;       // piece 0 moves K's, piece 1 V's
+    if (scales) {
+        const float *sc = piece == 0 ? e.kscale + b * e.kss[0] + g * e.kss[1] : e.vscale + b * e.vss[0] + g * e.vss[1];
+        const long long step = piece == 0 ? e.kss[2] : e.vss[2];
+#pragma unroll
+        for (int r = 0; r < kRowsOf; ++r)
+            if (j[r] >= 0) s[r] = sc[j[r] * step];
     }
+    char *ko = e.ko + b * e.kos[0] + g * e.kos[1] + piece * 16, *vo = e.vo + b * e.vos[0] + g * e.vos[1] + piece * 16;
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r)
+        if (j[r] >= 0) {
+            const long long i = i0 + r * rows;
+            *(uint4 *)(ko + i * e.kos[2]) = x[r];
+            *(uint4 *)(vo + i * e.vos[2]) = y[r];
+            if (scales) {
+                if (piece == 0)
+                    e.kscale_o[b * e.ksos[0] + g * e.ksos[1] + i * e.ksos[2]] = s[r];
+                else
+                    e.vscale_o[b * e.vsos[0] + g * e.vsos[1] + i * e.vsos[2]] = s[r];
+            }
+        }
 }
 
 // The same in place: one CTA moves a (sequence, KV head) front to back, a
@@ -176,18 +368,54 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const Evict e) {
 
 }  // namespace
 
+namespace {
+
+template <int C, int T>
+bool launch_rank(const Evict &e, int rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(rows * C);
+    cfg.blockDim = dim3(T);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NB_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_rank_kernel<C, T>, e));
+    return true;
+}
+
+}  // namespace
+
 bool launch_evict(const Evict &e, cudaStream_t st) {
     const int units = e.batch * e.kvheads;
     if (units == 0) return true;
-    evict_select_kernel<<<units, kThreads, 0, st>>>(e);
-    NB_CUDA_TRY(cudaGetLastError());
+    // a row's weights in registers: as few CTAs as hold them
+    const int n = e.capacity;
+    bool ok;
+    if (n <= 256 * kMine)
+        ok = launch_rank<1, 256>(e, units, st);
+    else if (n <= 1024 * kMine)
+        ok = launch_rank<1, 1024>(e, units, st);
+    else if (n <= 4 * 1024 * kMine)
+        ok = launch_rank<4, 1024>(e, units, st);
+    else if (n <= 8 * 1024 * kMine)
+        ok = launch_rank<8, 1024>(e, units, st);
+    else {
+        evict_select_kernel<<<units, kThreads, 0, st>>>(e);
+        NB_CUDA_TRY(cudaGetLastError());
+        ok = true;
+    }
+    if (!ok) return false;
     if (e.in_place) {
         NB_CUDA_TRY(launch_pdl(evict_move_kernel, dim3(units), dim3(kThreads), 0, st, e));
         return true;
     }
-    const int chunks = ceil_div(e.keep, 256 / (e.row_bytes / 16));
+    const int pieces = e.row_bytes / 16, shift = pieces == 4 ? 2 : pieces == 8 ? 3 : 4;
+    const int chunks = ceil_div(e.keep, kRowsOf * (256 >> shift));
     if (chunks == 0) return true;
-    NB_CUDA_TRY(launch_pdl(evict_gather_kernel, dim3(units * chunks), dim3(256), 0, st, e, chunks));
+    NB_CUDA_TRY(launch_pdl(evict_gather_kernel, dim3(units * chunks), dim3(256), 0, st, e, chunks, pieces, shift));
     return true;
 }
 

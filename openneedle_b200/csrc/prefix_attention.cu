@@ -128,7 +128,7 @@ __device__ __forceinline__ void copy_block(const KeySet &s, int j0, int j1, char
 }
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(const PrefixAttn p, const StreamGrid grid) {
+__device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGrid &grid) {
     using G = StreamGeom<TYPE, HD>;
     constexpr bool I8 = G::I8, BF = TYPE == kCacheBF16;
     constexpr int NT = G::kKeys / 8;                 // 8-key columns of a block
@@ -512,6 +512,13 @@ __global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(const Prefix
     }
 }
 
+template <int TYPE, int HD>
+__global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(const __grid_constant__ PrefixAttn p,
+                                                                    const __grid_constant__ StreamGrid grid) {
+    stream_unit<TYPE, HD>(p, grid);
+    pdl_enter();   // (at the end: what follows this kernel follows the tile kernel beside it too)
+}
+
 // ---- merge -----------------------------------------------------------------
 
 // HD / 4 threads a row: L over the row's partial results, then their weighted sum.
@@ -727,7 +734,7 @@ bool by_geometry(const PrefixAttn &p, F f) {
 
 }  // namespace
 
-bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream_t st) {
+bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after_tiles, cudaStream_t st) {
     return by_geometry(p, [&](auto type, auto hd) -> bool {
         using G = StreamGeom<type(), hd()>;
         StreamGrid grid{};
@@ -748,8 +755,12 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream
         }
         const int blocks = grid.own_units + grid.prefix_units;
         if (blocks == 0) return true;
-        kernel<<<blocks, kWarps * 32, G::kSmem, st>>>(p, grid);
-        NB_CUDA_TRY(cudaGetLastError());
+        if (after_tiles) {
+            NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kWarps * 32), (size_t)G::kSmem, st, p, grid));
+        } else {
+            kernel<<<blocks, kWarps * 32, G::kSmem, st>>>(p, grid);
+            NB_CUDA_TRY(cudaGetLastError());
+        }
         return true;
     });
 }

@@ -75,12 +75,14 @@ struct PrefixSplit {
 // weights of any number of rows from row_lse.
 bool launch_prefix_finish(const PrefixAttn &p, cudaStream_t st);
 bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
-// Streaming kernel: `prefix` / `own` say which key sets it takes.
-bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, cudaStream_t st);
+// Streaming kernel: `prefix` / `own` say which key sets it takes; after_tiles:
+// the tile kernel of the same call was launched before it with stream_next, runs
+// beside it, and has ended when it ends.
+bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after_tiles, cudaStream_t st);
 // Tile kernel for the sets whose split says `tiles`; cache_rows: extent of the
 // first axis of k and v.
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
-                         cudaStream_t st);
+                         bool stream_next, cudaStream_t st);
 // Weights of many rows from row_lse (and, INT8, q16): group up to 128.
 bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st);
 // 1 if a bounded wait of the tile kernels ran out since the last call, -1 if

@@ -58,6 +58,7 @@ struct TileGeom {
 struct TileGrid {
     int own_units, own_tiles, own_ranges, own_alt, own_rows;          // rows of a unit
     int prefix_units, prefix_tiles, prefix_ranges, prefix_alt, prefix_rows;
+    int stream_next;
     // whether the cache's head and sequence axes advance in the tensor maps
     int k_head, k_seq, v_head, v_seq, pk_head, pv_head;
 };
@@ -146,6 +147,8 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             vsc_step = p.pvss[1];
         }
     }
+    // the streaming kernel of the same call works on other keys: it may start beside this one
+    if (grid.stream_next) pdl_launch_dependents();
     if (rows <= 0) return;                        // the whole CTA
     const int n = ceil_div(max(0, hi - lo), kTile);              // key tiles
     const int tiles = alt ? 1 : (rows > kTile ? 2 : 1);          // row tiles
@@ -964,10 +967,11 @@ int read_and_clear_tile_fault() {
 }
 
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
-                         cudaStream_t st) {
+                         bool stream_next, cudaStream_t st) {
     auto run = [&](auto type, auto hd) -> bool {
         using G = TileGeom<type(), hd()>;
         TileGrid grid{};
+        grid.stream_next = stream_next;
         const int rows = p.tokens * p.group;
         CUtensorMap mk{}, mv{}, mpk{}, mpv{};
         int unused;

@@ -92,9 +92,6 @@ def test_outputs_must_not_overlap_inputs():
     ({"in_place": True, "out": ()}, "exclude"), ({"in_place": True, "keep": 31}, "capacity"),
     ({"k_scales": None}, "needs k_scales"), ({}, "CUDA tensors")])
 def test_evict_refuses(more, message):
-    if message in ("exclude", "capacity"):
-        if not torch.cuda.is_available():
-            message = "CUDA tensors"                        # (the stream's device is looked at first)
     with pytest.raises(ValueError, match=message):
         evict(inputs(), **{"keep": 8, **more})
 
@@ -107,12 +104,13 @@ def pack(**change):
              scale=0.125, q=4096, out=8192, k=4096, v=4096, ks=4096, vs=4096, pk=4096, pv=4096, pks=4096, pvs=4096,
              lengths=4096, counts=0, rows=0, lse=0, weights=0, weights_out=0, kstride=64)
     a.update(change)
-    return attention._ATTENTION_ARGS.pack(
+    three, flat, flat2 = (8192, 2048, a["kstride"]), (128, 32, 1), (16, 1)
+    return attention._ATTENTION_SIZES.pack(
         a["batch"], a["tokens"], a["heads"], a["kvheads"], a["head_dim"], a["prefix"], a["capacity"], a["window"],
-        a["cache_type"], a["scale"], a["q"], 512, 512, 64, a["out"], 512, 512, 64,
-        a["k"], a["v"], 8192, 2048, a["kstride"], 8192, 2048, 64, a["ks"], a["vs"], 128, 32, 1, 128, 32, 1,
-        a["pk"], a["pv"], 1024, 64, 1024, 64, a["pks"], a["pvs"], 16, 1, 16, 1,
-        a["lengths"], a["counts"], a["rows"], a["lse"], a["weights"], 128, 32, 1, a["weights_out"], 128, 32, 1)
+        a["cache_type"], a["scale"], 512, 512, 64, 512, 512, 64, *three, 8192, 2048, 64, *flat, *flat, 1024, 64, 1024,
+        64, *flat2, *flat2, *flat, *flat) + attention._ATTENTION_POINTERS.pack(
+        a["q"], a["out"], a["k"], a["v"], a["ks"], a["vs"], a["pk"], a["pv"], a["pks"], a["pvs"], a["lengths"],
+        a["counts"], a["rows"], a["lse"], a["weights"], a["weights_out"])
 
 
 def test_workspace_grows_with_what_is_asked():
@@ -139,20 +137,23 @@ def test_c_abi_refuses(change, message):
     assert message in attention.last_error()
 
 
-@pytest.mark.parametrize("index,value,message", [
-    (0, -1, "negative size"), (2, 80, "head_dim"), (8, 7, "cache type"), (5, 3, "exceed keep"), (4, 7, "fewer than keep"),
-    (9, 0, "k is null"), (9, 4100, "multiples of 16"), (13, 72, "multiples of 16"), (17, 0, "needs its scales"),
-    (25, 0, "weights is null"), (29, 0, "null pointer"), (29, 65536, "must not be lengths"), (30, 4096, "in place")])
-def test_c_abi_refuses_evictions(index, value, message):
+@pytest.mark.parametrize("change,message", [
+    ({"batch": -1}, "negative size"), ({"head_dim": 80}, "head_dim"), ({"cache_type": 7}, "cache type"),
+    ({"keep": 3}, "exceed keep"), ({"out_capacity": 7}, "fewer than keep"), ({"batch": 1 << 29}, "too large"),
+    ({"k": 0}, "k is null"), ({"k": 4100}, "multiples of 16"), ({"kstride": 72}, "multiples of 16"),
+    ({"v_out": 4104}, "v_out"), ({"k_scales": 0}, "needs its scales"), ({"weights": 0}, "weights is null"),
+    ({"weights_out": 0}, "weights_out is null"), ({"lengths": 0}, "null pointer"),
+    ({"lengths": 65536}, "must not be lengths"), ({"k_out": 4096}, "in place")])
+def test_c_abi_refuses_evictions(change, message):
     lib = attention._bind_operators()[0]
-    three = (8192, 2048, 64)
-    flat = (128, 32, 1)
-    a = [2, 4, 64, 32, 32, 8, 2, 2, 0, 4096, 4096, *three, *three, 4096, 4096, *flat, *flat, 4096, *flat, 4096,
-         16384, 16384, *three, *three, 16384, 16384, *flat, *flat, 16384, *flat, 16384, 65536]
-    if message == "must not be lengths":
-        a[29] = a[-1]
-    else:
-        a[index] = value
-    assert lib.needle2_evict_device(attention._EVICT_ARGS.pack(*a), None) == -1
+    a = dict(batch=2, kvheads=4, head_dim=64, capacity=32, out_capacity=32, keep=8, first=2, recent=2, cache_type=0)
+    p = dict(k=4096, v=4096, k_scales=4096, v_scales=4096, weights=4096, lengths=4096, k_out=16384, v_out=16384,
+             k_scales_out=16384, v_scales_out=16384, weights_out=16384, indices=16384, lengths_out=65536)
+    three, flat = (8192, 2048, change.pop("kstride", 64)), (128, 32, 1)
+    for n, x in change.items():
+        (a if n in a else p)[n] = x
+    sizes = attention._EVICT_SIZES.pack(*a.values(), *three, *three, *flat, *flat, *flat, *three, *three, *flat, *flat,
+                                        *flat)
+    assert lib.needle2_evict_device(sizes + attention._EVICT_POINTERS.pack(*p.values()), None) == -1
     assert message in attention.last_error()
     assert lib.needle2_evict_device(None, None) == -1
