@@ -25,11 +25,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 // Selection with a row's weights in registers: a cluster of C CTAs per
 // (sequence, KV head), each thread up to kMine weights of its CTA's contiguous
-// segment.  The key of the last weight that stays is found four bits at a time
-// from the top: every thread counts its keys by digit, the counts meet in shared
-// memory and, across the cluster, by distributed shared memory.  Then ties and
-// kept positions are ranked in index order, and everything is written.  The
-// weights are read once; bound by the latency of the eight rounds.
+// segment.  The key of the last weight that stays is found eight bits at a time
+// from the top: the keys that still match are counted by digit in shared memory
+// (few of them after the first round, so that counting costs little), the counts
+// of a cluster's CTAs meet by distributed shared memory.  Then ties and kept
+// positions are ranked in index order, and everything is written.  The weights
+// are read once; bound by the latency of the rounds.
 constexpr int kMine = 16;
 
 template <int C, int T>
@@ -42,9 +43,10 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
     const float *w = e.weights + b * e.ws[0] + g * e.ws[1];
     float *wo = e.weights_o + b * e.wos[0] + g * e.wos[1];
     int *idx = e.indices + (long long)row * e.keep;
-    __shared__ int counts[8][16];
+    __shared__ int counts[4][256];
+    __shared__ int sums[8], found[2];
     __shared__ int ranks[2][kMine * kWarpsIn + 1];   // ties, kept: of (i, warp), then exclusive sums; last: their total
-    for (int i = tid; i < 128; i += T) (&counts[0][0])[i] = 0;
+    for (int i = tid; i < 1024; i += T) (&counts[0][0])[i] = 0;
 
     const int lo = e.first, hi = n - e.recent, seg = ceil_div(ceil_div(e.capacity, C), T) * T, j0 = rank * seg;
     const int mine = min(kMine, ceil_div(max(0, min(seg, n - j0)), T));
@@ -77,45 +79,40 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
     const bool none = need == 0;
     uint32_t prefix = 0;
     if (choose && !none) {                           // the same in every CTA of the row
-        for (int it = 0; it < 8; ++it) {
-            const int shift = 28 - 4 * it;
-            const uint32_t mask = it == 0 ? 0u : ~0u << (shift + 4);
-            // sixteen counts of up to kMine: a byte each
-            uint32_t c[4] = {0, 0, 0, 0};
+        for (int it = 0; it < 4; ++it) {
+            const int shift = 24 - 8 * it;
+            const uint32_t mask = it == 0 ? 0u : ~0u << (shift + 8);
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
                 if (i >= mine) break;
                 const int j = j0 + i * T + tid;
                 const uint32_t u = weight_key(x[i]);
-                if (j >= lo && j < hi && (u & mask) == prefix) {
-                    const uint32_t d = (u >> shift) & 15, one = 1u << (8 * (d & 3));
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) c[q] += q == (int)(d >> 2) ? one : 0u;
-                }
-            }
-            // of the warp: 16 bits each
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t even = __reduce_add_sync(0xffffffffu, c[q] & 0x00ff00ffu);
-                const uint32_t odd = __reduce_add_sync(0xffffffffu, (c[q] >> 8) & 0x00ff00ffu);
-                const uint32_t v = lane & 1 ? odd : even;
-                if (lane < 4 && v) atomicAdd(&counts[it][4 * q + lane], (int)(lane & 2 ? v >> 16 : v & 0xffff));
+                if (j >= lo && j < hi && (u & mask) == prefix) atomicAdd(&counts[it][(u >> shift) & 255], 1);
             }
             all_sync();
-            // every warp: lane d has digit d's total, then the digit in which the need-th largest lies
-            int mineof = 0;
-            if (lane < 16)
-                for (int r = 0; r < C; ++r) mineof += of_cta(&counts[it][15 - lane], r);   // from above
-            int above = mineof;
+            // thread d has the digit 255 - d: the one in which the need-th largest key lies
+            int total = 0, above = 0;
+            if (tid < 256) {
+                for (int r = 0; r < C; ++r) total += of_cta(&counts[it][255 - tid], r);
+                above = total;
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, above, d);
-                if (lane >= d) above += y;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, above, d);
+                    if (lane >= d) above += y;
+                }
+                if (lane == 31) sums[warp] = above;
             }
-            const unsigned at = __ballot_sync(0xffffffffu, lane < 16 && above >= need);
-            const int l = __ffs(at) - 1;
-            need -= __shfl_sync(0xffffffffu, above - mineof, l);
-            prefix |= (uint32_t)(15 - l) << shift;
+            __syncthreads();
+            if (tid < 256) {
+                for (int k = 0; k < warp; ++k) above += sums[k];
+                if (above >= need && above - total < need) {
+                    found[0] = 255 - tid;
+                    found[1] = need - (above - total);
+                }
+            }
+            __syncthreads();
+            prefix |= (uint32_t)found[0] << shift;
+            need = found[1];
         }
     }
 

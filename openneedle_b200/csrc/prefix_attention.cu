@@ -63,6 +63,7 @@ __device__ __forceinline__ void cp4z(uint32_t dst, const void *src, bool valid) 
 // copies; the four states meet in shared memory at the end.
 
 constexpr int kWarps = 4;
+constexpr int kShortRange = 64;   // keys of a range that one warp takes by itself
 
 template <int TYPE, int HD>
 struct StreamGeom {
@@ -70,7 +71,7 @@ struct StreamGeom {
     static constexpr int kSize = I8 ? 1 : 2;
     static constexpr int kRows = I8 ? 8 : 16;                             // query rows of a tile
     static constexpr int kKeys = I8 ? 32 : (HD == 64 ? 32 : 16);          // keys of a block
-    static constexpr int kStages = 3;
+    static constexpr int kStages = 2;
     static constexpr int kKRow = HD * kSize;                              // bytes of a K row in shared memory
     // INT8 V rows are read a word per (key, four dimensions), keys of one
     // access two rows apart: 16 bytes of padding spread them over the banks
@@ -96,38 +97,69 @@ struct StreamGrid {
     int own_slots, prefix_slots;
 };
 
+// One lane's part of the copies of a warp's blocks: 16-byte pieces of K and V
+// rows, a scale of each; advances by a fixed number of keys.
 template <int TYPE, int HD>
-__device__ __forceinline__ void copy_block(const KeySet &s, int j0, int j1, char *stage, int lane) {
+struct BlockCopy {
     using G = StreamGeom<TYPE, HD>;
-    const uint32_t base = smem_addr(stage);
-    constexpr int kChunks = HD * G::kSize / 16;      // 16-byte pieces of a row
-    constexpr int kPer = 32 / kChunks;               // rows of one warp-wide copy
-    const int c = lane % kChunks, r0 = lane / kChunks;
-#pragma unroll
-    for (int i = 0; i < G::kKeys / kPer; ++i) {
-        const int r = r0 + i * kPer, j = j0 + r;
-        const bool valid = j < j1;
-        const long long jj = valid ? j : j0;
-        int kc = c, vc = c;
-        if constexpr (TYPE != kCacheI8) {
-            kc = vc = c ^ (r & 7);                   // rows of an 8x8 matrix on different banks
-        } else if constexpr (HD == 128) {
-            kc = c ^ ((r & 1) << 2);
-        }
-        cp16z(base + r * G::kKRow + kc * 16, s.k + jj * s.k_step + c * 16, valid);
-        cp16z(base + G::kVOff + r * G::kVRow + vc * 16, s.v + jj * s.v_step + c * 16, valid);
-    }
-    if constexpr (TYPE == kCacheI8) {
-        static_assert(G::kKeys == 32, "one scale a lane");
-        const int j = j0 + lane;
-        const bool valid = j < j1;
-        const long long jj = valid ? j : j0;
-        cp4z(base + G::kSOff + lane * 4, s.ks + jj * s.ks_step, valid);
-        cp4z(base + G::kSOff + 128 + lane * 4, s.vs + jj * s.vs_step, valid);
-    }
-}
+    static constexpr int kChunks = HD * G::kSize / 16;      // 16-byte pieces of a row
+    static constexpr int kPer = 32 / kChunks;               // rows of one warp-wide copy
+    const char *k, *v;
+    const float *ks, *vs;
+    long long k_per, v_per, k_next, v_next, ks_next, vs_next;
 
-template <int TYPE, int HD>
+    __device__ __forceinline__ BlockCopy(const KeySet &s, int j0, int keys, int lane) {
+        const long long r = j0 + lane / kChunks, piece = lane % kChunks * 16;
+        k = s.k + r * s.k_step + piece;
+        v = s.v + r * s.v_step + piece;
+        k_per = kPer * s.k_step;
+        v_per = kPer * s.v_step;
+        k_next = keys * s.k_step;
+        v_next = keys * s.v_step;
+        if constexpr (G::I8) {
+            static_assert(G::kKeys == 32, "one scale a lane");
+            ks = s.ks + (long long)(j0 + lane) * s.ks_step;
+            vs = s.vs + (long long)(j0 + lane) * s.vs_step;
+            ks_next = keys * s.ks_step;
+            vs_next = keys * s.vs_step;
+        }
+    }
+
+    // `left` keys exist; rows behind them become zeros
+    __device__ __forceinline__ void block(char *stage, int left, int lane) {
+        const uint32_t base = smem_addr(stage);
+        const int c = lane % kChunks, r0 = lane / kChunks;
+        const char *kp = k, *vp = v;
+#pragma unroll
+        for (int i = 0; i < G::kKeys / kPer; ++i) {
+            const int r = r0 + i * kPer;
+            int kc = c, vc = c;
+            if constexpr (TYPE != kCacheI8) {
+                kc = vc = c ^ (r & 7);                       // rows of an 8x8 matrix on different banks
+            } else if constexpr (HD == 128) {
+                kc = c ^ ((r & 1) << 2);
+            }
+            const bool valid = r < left;
+            cp16z(base + r * G::kKRow + kc * 16, valid ? kp : k, valid);
+            cp16z(base + G::kVOff + r * G::kVRow + vc * 16, valid ? vp : v, valid);
+            kp += k_per;
+            vp += v_per;
+        }
+        k += k_next;
+        v += v_next;
+        if constexpr (G::I8) {
+            const bool valid = lane < left;
+            cp4z(base + G::kSOff + lane * 4, ks, valid);
+            cp4z(base + G::kSOff + 128 + lane * 4, vs, valid);
+            ks += ks_next;
+            vs += vs_next;
+        }
+    }
+};
+
+// W warps share a unit's keys: four where the ranges are long, one (and four
+// units a CTA, no merge between warps) where they are short.
+template <int TYPE, int HD, int W>
 __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGrid &grid) {
     using G = StreamGeom<TYPE, HD>;
     constexpr bool I8 = G::I8, BF = TYPE == kCacheBF16;
@@ -137,10 +169,12 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g8 = lane >> 2, c = lane & 3;
     char *ring = smem + warp * G::kWarpBytes;
+    const int part = warp % W;                       // of the unit's warps
 
     // the unit: rows [m0, m0 + rows) of KV head g, keys [lo, hi)
     const int R = p.group, TR = p.tokens * R;
-    int unit = blockIdx.x, g, m0, rows, lo, hi, slot, seq = -1, len = 0, nq = 0;
+    int unit = blockIdx.x * (kWarps / W) + warp / W, g, m0, rows, lo, hi, slot, seq = -1, len = 0, nq = 0;
+    if (unit >= grid.own_units + grid.prefix_units) return;
     KeySet s;
     if (unit < grid.own_units) {
         slot = unit % grid.own_slots;
@@ -199,10 +233,13 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
 
     // first copies, then the queries
     const int blocks = ceil_div(max(0, hi - lo), G::kKeys);
-    const int mine = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
+    const int mine = blocks > part ? (blocks - part + W - 1) / W : 0;
+    BlockCopy<TYPE, HD> copy(s, lo + part * G::kKeys, W * G::kKeys, lane);
+    int left = hi - lo - part * G::kKeys;            // keys from the next block to be copied on
 #pragma unroll
     for (int i = 0; i < G::kStages - 1; ++i) {
-        if (i < mine) copy_block<TYPE, HD>(s, lo + (warp + i * kWarps) * G::kKeys, hi, ring + i * G::kStage, lane);
+        if (i < mine) copy.block(ring + i * G::kStage, left, lane);
+        left -= W * G::kKeys;
         cp_async_commit();
     }
 
@@ -221,7 +258,9 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
             last[e] = t < nq ? len - nq + t : -1;
             first[e] = p.window ? len - nq + t - p.window + 1 : 0;
         }
+        last[e] = min(last[e], hi - 1);
     }
+    const int all_from = max(first[0], first[kMine - 1]), all_to = min(last[0], last[kMine - 1]);
     uint32_t qa[KS][4];
     float qscale = p.scale2;
     if constexpr (I8) {
@@ -271,14 +310,13 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         __syncwarp();
         {   // the stage that was read last takes the copy two blocks ahead
             const int n = i + G::kStages - 1;
-            if (n < mine)
-                copy_block<TYPE, HD>(s, lo + (warp + n * kWarps) * G::kKeys, hi, ring + (n % G::kStages) * G::kStage,
-                                     lane);
+            if (n < mine) copy.block(ring + (n % G::kStages) * G::kStage, left, lane);
+            left -= W * G::kKeys;
             cp_async_commit();
         }
         const char *stage = ring + (i % G::kStages) * G::kStage;
         const uint32_t base = smem_addr(stage);
-        const int j0 = lo + (warp + i * kWarps) * G::kKeys;
+        const int j0 = lo + (part + i * W) * G::kKeys;
 
         // z = Q K^T
         float z[NT][4];
@@ -320,7 +358,6 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         float vs[NT][2], vmax = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int j = j0 + 8 * n + 2 * c;
             if constexpr (I8) {
                 const float2 ks = *(const float2 *)(stage + G::kSOff + (8 * n + 2 * c) * 4);
                 const float2 v2 = *(const float2 *)(stage + G::kSOff + 128 + (8 * n + 2 * c) * 4);
@@ -333,20 +370,29 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[n][e] *= qscale;
             }
+        }
+        if (j0 < all_from || j0 + G::kKeys - 1 > all_to) {
 #pragma unroll
-            for (int e = 0; e < 2 * kMine; ++e) {
-                const int key = j + (e & 1);
-                if (key >= hi || key > last[e >> 1] || key < first[e >> 1]) z[n][e] = kNegInf;
-                best[e >> 1] = fmaxf(best[e >> 1], z[n][e]);
-            }
-            if (logits) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2 * kMine; ++e) {
-                    const int row = g8 + 8 * (e >> 1), key = j + (e & 1);
+                    const int key = j0 + 8 * n + 2 * c + (e & 1);
+                    if (key > last[e >> 1] || key < first[e >> 1]) z[n][e] = kNegInf;
+                }
+        }
+        if (logits) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2 * kMine; ++e) {
+                    const int row = g8 + 8 * (e >> 1), key = j0 + 8 * n + 2 * c + (e & 1);
                     if (row < rows && key < hi) logits[(long long)row * p.capacity + key] = z[n][e];
                 }
-            }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2 * kMine; ++e) best[e >> 1] = fmaxf(best[e >> 1], z[n][e]);
         float keep[kMine];
         bool moved = false;
 #pragma unroll
@@ -468,23 +514,27 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
             *(float2 *)(mo + (g8 + 8) * HD + 8 * d + 2 * c) = make_float2(o[d][2], o[d][3]);
         }
     }
-    __syncthreads();
+    if constexpr (W == 1)
+        __syncwarp();
+    else
+        __syncthreads();
 
     const long long nrows = (long long)p.batch * p.tokens * p.heads;
     const bool direct = p.prefix_slots + p.own_slots == 1;
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) {
+    const char *states = ring - part * G::kWarpBytes;
+    for (int i = threadIdx.x % (32 * W); i < rows * (HD / 4); i += 32 * W) {
         const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float tops[kWarps], t = kNegInf, total = 0.f;
+        float tops[W], t = kNegInf, total = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            tops[w] = ((const float *)(smem + w * G::kWarpBytes) + 16 * HD)[2 * r];
+        for (int w = 0; w < W; ++w) {
+            tops[w] = ((const float *)(states + w * G::kWarpBytes) + 16 * HD)[2 * r];
             t = fmaxf(t, tops[w]);
         }
         const float t0 = t == kNegInf ? 0.f : t;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float *q = (const float *)(smem + w * G::kWarpBytes);
+        for (int w = 0; w < W; ++w) {
+            const float *q = (const float *)(states + w * G::kWarpBytes);
             const float f = ex2(tops[w] - t0);
             total += f * q[16 * HD + 2 * r + 1];
             const float4 v = *(const float4 *)(q + r * HD + d);
@@ -512,10 +562,10 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
     }
 }
 
-template <int TYPE, int HD>
-__global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(const __grid_constant__ PrefixAttn p,
-                                                                    const __grid_constant__ StreamGrid grid) {
-    stream_unit<TYPE, HD>(p, grid);
+template <int TYPE, int HD, int W>
+__global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(
+    const __grid_constant__ PrefixAttn p, const __grid_constant__ StreamGrid grid) {
+    stream_unit<TYPE, HD, W>(p, grid);
     pdl_enter();   // (at the end: what follows this kernel follows the tile kernel beside it too)
 }
 
@@ -602,15 +652,33 @@ __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, 
     const float *z = p.logits + (long long)(b * p.kvheads + g) * TR * p.capacity;
     const float *win = p.weights + b * p.ws[0] + g * p.ws[1];
     float *wout = p.weights_out + b * p.wos[0] + g * p.wos[1];
-    const int end = min(p.capacity, (chunk + 1) * kWeightKeys);
-    for (int j = chunk * kWeightKeys + threadIdx.x; j < end; j += 128) {
-        float w = 0.f;
-        for (int r = 0; r < nq * p.group; ++r) {
-            const int i = len - nq + r / p.group;     // own index of the row's query
-            if (j <= i && (!p.window || j > i - p.window))
-                w += ex2(z[(long long)r * p.capacity + j] - lse[r]);
+    // kWeightKeys / 128 keys of a thread, their loads in flight together
+    constexpr int kMine = kWeightKeys / 128;
+    const int j0 = chunk * kWeightKeys + threadIdx.x, past = len - nq;
+    float w[kMine], old[kMine];
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        const int j = j0 + e * 128;
+        old[e] = j < p.capacity ? win[j * p.ws[2]] : 0.f;
+        w[e] = 0.f;
+    }
+#pragma unroll 2
+    for (int r = 0; r < nq * p.group; ++r) {
+        const int i = past + r / p.group;             // own index of the row's query
+        const int from = p.window ? i - p.window + 1 : 0;
+        float x[kMine];
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) {
+            const int j = j0 + e * 128;
+            x[e] = j <= i && j >= from ? z[(long long)r * p.capacity + j] : kNegInf;
         }
-        wout[j * p.wos[2]] = win[j * p.ws[2]] + w;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) w[e] += ex2(x[e] - lse[r]);
+    }
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        const int j = j0 + e * 128;
+        if (j < p.capacity) wout[j * p.wos[2]] = old[e] + w[e];
     }
 }
 
@@ -745,23 +813,31 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after
         grid.prefix_tiles = ceil_div(p.batch * rows, G::kRows);
         grid.own_units = own ? p.batch * p.kvheads * grid.own_tiles * grid.own_slots : 0;
         grid.prefix_units = prefix ? p.kvheads * grid.prefix_tiles * grid.prefix_slots : 0;
-        auto kernel = prefix_stream_kernel<type(), hd()>;
-        static bool configured[64] = {};
-        int dev = 0;
-        NB_CUDA_TRY(cudaGetDevice(&dev));
-        if (dev < 0 || dev >= 64 || !configured[dev]) {
-            NB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
-            if (dev >= 0 && dev < 64) configured[dev] = true;
-        }
-        const int blocks = grid.own_units + grid.prefix_units;
-        if (blocks == 0) return true;
-        if (after_tiles) {
-            NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kWarps * 32), (size_t)G::kSmem, st, p, grid));
-        } else {
-            kernel<<<blocks, kWarps * 32, G::kSmem, st>>>(p, grid);
-            NB_CUDA_TRY(cudaGetLastError());
-        }
-        return true;
+        const int units = grid.own_units + grid.prefix_units;
+        if (units == 0) return true;
+        auto launch = [&](auto warps) -> bool {
+            auto kernel = prefix_stream_kernel<type(), hd(), warps()>;
+            static bool configured[64] = {};
+            int dev = 0;
+            NB_CUDA_TRY(cudaGetDevice(&dev));
+            if (dev < 0 || dev >= 64 || !configured[dev]) {
+                NB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
+                if (dev >= 0 && dev < 64) configured[dev] = true;
+            }
+            const int blocks = ceil_div(units, kWarps / warps());
+            if (after_tiles) {
+                NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kWarps * 32), (size_t)G::kSmem, st, p, grid));
+            } else {
+                kernel<<<blocks, kWarps * 32, G::kSmem, st>>>(p, grid);
+                NB_CUDA_TRY(cudaGetLastError());
+            }
+            return true;
+        };
+        const int span = p.window ? std::min<long long>(p.capacity, (long long)p.window + p.tokens) : p.capacity;
+        const int longest = std::max(own ? ceil_div(span, grid.own_slots) : 0,
+                                     prefix ? ceil_div(p.prefix, grid.prefix_slots) : 0);
+        return longest <= kShortRange ? launch(std::integral_constant<int, 1>())
+                                      : launch(std::integral_constant<int, kWarps>());
     });
 }
 

@@ -309,56 +309,68 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             if (alt) {
                 for (int j = 0; ok && j < min(n, 2); ++j) {
                     ok = have(2 * j);
-                    if (ok && lane == 0) {
+                    __syncwarp();
+                    if (ok && elect_one()) {
                         tc::fence_after();
                         logits(j, j);
                         tc::commit(&empty[(2 * j) % kStages]);
                     }
+                    __syncwarp();
                 }
                 for (int j = 0; ok && j < n; ++j) {
                     const int w = j & 1;
                     ok = have_v(j) && wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
                     if (!ok) break;
-                    if (lane == 0) {
+                    __syncwarp();
+                    if (elect_one()) {
                         tc::fence_after();
                         values(w, j, j < 2);
                         tc::commit(&empty[(2 * j + 1) % kStages]);
                         if (j + 2 >= n) tc::commit(&o_full[w]);
                     }
+                    __syncwarp();
                     if (j + 2 < n) {
                         ok = have(2 * j + 4);
-                        if (ok && lane == 0) {
+                        __syncwarp();
+                        if (ok && elect_one()) {
                             tc::fence_after();
                             logits(w, j + 2);
                             tc::commit(&empty[(2 * j + 4) % kStages]);
                         }
+                        __syncwarp();
                     }
                 }
             } else {
                 ok = ok && have(0);
-                if (ok && lane == 0) {
+                __syncwarp();
+                if (ok && elect_one()) {
                     tc::fence_after();
                     for (int w = 0; w < tiles; ++w) logits(w, 0);
                     tc::commit(&empty[0]);
                 }
+                __syncwarp();
                 for (int j = 0; ok && j < n; ++j) {
                     ok = have_v(j);
                     for (int w = 0; ok && w < tiles; ++w) {
                         ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
                         if (!ok) break;
-                        if (lane == 0) {
+                        __syncwarp();
+                        if (elect_one()) {
                             tc::fence_after();
                             values(w, j, j == 0);
                             if (w == tiles - 1) tc::commit(&empty[(2 * j + 1) % kStages]);
                             if (j == n - 1) tc::commit(&o_full[w]);
                         }
+                        __syncwarp();
                         if (j + 1 < n) {
                             ok = w > 0 || have(2 * j + 2);
-                            if (ok && lane == 0) {
+                            __syncwarp();
+                            if (ok && elect_one()) {
                                 tc::fence_after();
                                 logits(w, j + 1);
                                 if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
                             }
+                            __syncwarp();
                         }
                     }
                 }
@@ -781,30 +793,34 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
                 for (int i = max(0, issued - kStages); i < issued; ++i)
                     mbar_wait(&full[i % kStages], (uint32_t)(i / kStages) & 1);
             __syncwarp();
-        } else if (warp == 8 && lane == 0) {
+        } else if (warp == 8) {
             // ---- products
             constexpr uint32_t ids = idesc(BF, false, kTile);
             const uint32_t k0 = smem_addr(smem), q0 = smem_addr(smem) + G::kRing;
-            for (int i = 0; i < n; ++i) {
+            bool ok = true;
+            for (int i = 0; ok && i < n; ++i) {
                 const int s = i % kStages;
-                if (!wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag)) break;
-                bool ok = true;
-                for (int w = 0; w < 2; ++w) {
-                    if (i >= 2) ok = ok && wait_phase(&s_free[w][i & 1], (uint32_t)(i / 2 - 1) & 1, abort_flag);
+                ok = wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag);
+                for (int w = 0; ok && w < 2; ++w) {
+                    if (i >= 2) ok = wait_phase(&s_free[w][i & 1], (uint32_t)(i / 2 - 1) & 1, abort_flag);
                     if (!ok) break;
-                    tc::fence_after();
+                    __syncwarp();
+                    if (elect_one()) {
+                        tc::fence_after();
 #pragma unroll
-                    for (int x = 0; x < G::kPieces; ++x)
+                        for (int x = 0; x < G::kPieces; ++x)
 #pragma unroll
-                        for (int c = 0; c < HD / 16; ++c) {
-                            const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
-                            tc::mma_bf16_ss(tmem + (2 * w + (i & 1)) * kTile, desc_k(k0 + w * G::kTileBytes + at),
-                                            desc_k(q0 + s * G::kStageBytes + x * G::kTileBytes + at), ids, x + c > 0);
-                        }
-                    tc::commit(&s_full[w][i & 1]);
+                            for (int c = 0; c < HD / 16; ++c) {
+                                const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
+                                tc::mma_bf16_ss(tmem + (2 * w + (i & 1)) * kTile, desc_k(k0 + w * G::kTileBytes + at),
+                                                desc_k(q0 + s * G::kStageBytes + x * G::kTileBytes + at), ids,
+                                                x + c > 0);
+                            }
+                        tc::commit(&s_full[w][i & 1]);
+                        if (w == 1) tc::commit(&empty[s]);
+                    }
+                    __syncwarp();
                 }
-                if (!ok) break;
-                tc::commit(&empty[s]);
             }
         }
         __syncwarp();

@@ -147,6 +147,17 @@ __host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int n) {
     return (1u << 4) | ((uint32_t)bf << 7) | ((uint32_t)bf << 10) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
+// One lane of a converged warp, the same each time.  The products are issued
+// under it: the compiler then knows that one thread runs and keeps their
+// descriptors in uniform registers (under `lane == 0` an issue took about 100
+// cycles, and the issues bounded the kernels).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // D[tmem] (+)= A[tmem] x B[smem]
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t acc) {
     asm volatile(
