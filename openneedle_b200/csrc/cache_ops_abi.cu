@@ -50,8 +50,8 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
 
 struct Plan {
     PrefixSplit prefix, own;
-    bool logits, row_lse, weight_tiles;
-    long long part_o, part_lse, row_lse_at, logits_at, q16_at, q16_scale_at, bytes;
+    bool logits, neg_lse, weight_tiles;
+    long long part_o, part_lse, neg_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
 
 int sm_count() {
@@ -93,7 +93,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.own.ranges = 1;
     }
     p.logits = a.weights && a.tokens > 0 && !p.own.tiles;     // (the tile kernel's rows are too many to keep)
-    p.row_lse = a.weights != nullptr;
+    p.neg_lse = a.weights != nullptr;
     p.weight_tiles = a.weights && p.own.tiles && R <= 128;
     long long at = 0;
     auto take = [&](long long bytes) {
@@ -106,7 +106,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.part_o = take(rows * n * a.head_dim * 4);
         p.part_lse = take(rows * n * 4);
     }
-    if (p.row_lse) p.row_lse_at = take(rows * 4);
+    if (p.neg_lse) p.neg_lse_at = take(rows * 4);
     if (p.logits) p.logits_at = take((long long)a.batch * a.kvheads * a.tokens * R * a.capacity * 4);
     if (p.weight_tiles && a.cache_type == kCacheI8) {
         p.q16_at = take(rows * a.head_dim * 4);
@@ -175,7 +175,7 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
         p.part_o = reinterpret_cast<float *>(base + plan.part_o);
         p.part_lse = reinterpret_cast<float *>(base + plan.part_lse);
     }
-    if (plan.row_lse) p.row_lse = reinterpret_cast<float *>(base + plan.row_lse_at);
+    if (plan.neg_lse) p.neg_lse = reinterpret_cast<float *>(base + plan.neg_lse_at);
     if (plan.logits) p.logits = reinterpret_cast<float *>(base + plan.logits_at);
     if (a.tokens > 0) {
         const bool stream_prefix = plan.prefix.ranges && !plan.prefix.tiles;

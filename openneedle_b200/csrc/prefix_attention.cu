@@ -554,7 +554,7 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
                     *(uint2 *)dst = make_uint2(pack2<BF>(acc.x, acc.y), pack2<BF>(acc.z, acc.w));
                 if (d == 0 && p.lse) p.lse[row] = lse * kLn2;
             }
-            if (d == 0 && p.row_lse) p.row_lse[row] = lse;
+            if (d == 0 && p.neg_lse) p.neg_lse[neg_lse_at(p, b, tt, h)] = -lse;
         } else {
             *(float4 *)(p.part_o + (slot * nrows + row) * HD + d) = acc;
             if (d == 0) p.part_lse[slot * nrows + row] = lse;
@@ -604,7 +604,7 @@ __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, in
     if (part == 0) {
         const float lse = total == 0.f ? kNegInf : t0 + log2f(total);
         if (p.lse) p.lse[row] = lse * kLn2;
-        if (p.row_lse) p.row_lse[row] = lse;
+        if (p.neg_lse) p.neg_lse[neg_lse_at(p, b, t, h)] = -lse;
     }
 }
 
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, 
         float l = 0.f;
         if (t < nq) {
             if (slots == 1) {
-                l = p.row_lse[row];
+                l = -p.neg_lse[neg_lse_at(p, b, t, h)];
             } else {
                 float top = kNegInf, total = 0.f;
                 for (int i = 0; i < slots; ++i) top = fmaxf(top, p.part_lse[i * nrows + row]);
@@ -765,13 +765,13 @@ __global__ __launch_bounds__(128) void key_weights_kernel(const PrefixAttn p) {
                 const float dn = __shfl_sync(0xffffffffu, down, 4 * (2 * c + x));
                 const int r2 = m + 2 * c + x, t2 = r2 / p.group;
                 if (r2 < nq * p.group) {
-                    const float l = p.row_lse[((long long)b * p.tokens + t2) * p.heads + g * p.group + r2 % p.group];
+                    const float l = p.neg_lse[((long long)b * p.kvheads + g) * TR + r2];
                     const int i = len - nq + t2;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int j = key0 + g8 + 8 * e;
                         if (j <= i && (!p.window || j > i - p.window))
-                            sum[e] += ex2(z[2 * e + x] * (ks[e] * dn) - l);
+                            sum[e] += ex2(z[2 * e + x] * (ks[e] * dn) + l);
                     }
                 }
             }

@@ -49,7 +49,7 @@ struct PrefixAttn {
     int prefix_slots, own_slots;                     // key ranges of the prefix and of the own keys
     float *part_o;                                   // [slots][rows][hd], rows = B * tokens * heads as out's
     float *part_lse;                                 // [slots][rows]
-    float *row_lse;                                  // [rows], log2 (null: not needed)
+    float *neg_lse;                                  // [B][kvheads][tokens * R], minus log2's lse (null: not needed)
     void *q16;                                       // weights of an INT8 cache's many rows: split queries
     float *q16_scale;                                // and their factors
     float *logits;                                   // [B * kvheads][tokens * R][capacity], log2 (null: not kept)
@@ -57,6 +57,10 @@ struct PrefixAttn {
 
 __device__ __forceinline__ int own_length(const PrefixAttn &p, int b) {
     return max(0, min(p.lengths[b], p.capacity));
+}
+// The place of token t, head h of sequence b in neg_lse.
+__device__ __forceinline__ long long neg_lse_at(const PrefixAttn &p, int b, int t, int h) {
+    return (((long long)b * p.kvheads + h / p.group) * p.tokens + t) * p.group + h % p.group;
 }
 __device__ __forceinline__ int own_tokens(const PrefixAttn &p, int b) {
     return p.ntokens ? max(0, min(p.ntokens[b], p.tokens)) : p.tokens;
@@ -72,7 +76,7 @@ struct PrefixSplit {
 };
 
 // The merge of the partial results, weights of few rows from kept logits, and
-// weights of any number of rows from row_lse.
+// weights of any number of rows from neg_lse.
 bool launch_prefix_finish(const PrefixAttn &p, cudaStream_t st);
 bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
 // Streaming kernel: `prefix` / `own` say which key sets it takes; after_tiles:
@@ -83,7 +87,7 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after
 // first axis of k and v.
 bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
                          bool stream_next, cudaStream_t st);
-// Weights of many rows from row_lse (and, INT8, q16): group up to 128.
+// Weights of many rows from neg_lse (and, INT8, q16): group up to 128.
 bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st);
 // 1 if a bounded wait of the tile kernels ran out since the last call, -1 if
 // the flag could not be read.

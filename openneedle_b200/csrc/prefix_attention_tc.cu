@@ -6,12 +6,12 @@
 // One CTA attends up to 256 rows (two tiles of 128) to one key range, 128 keys
 // at a time.  A warp feeds K and V by TMA, one thread issues the products
 // S = Q K^T (into TMEM) and O += P V (P from TMEM, V from shared memory), and
-// each tile has a warpgroup whose thread i owns row i: it reads its 128 logits
-// back, keeps the row's maximum and sum in registers, writes the weights over
-// the logits and, where the maximum grew by more than 2^8, rescales its row of
-// O.  While one tile is in its softmax the tensor core works for the other.
-// Up to 128 rows run with both warpgroups on the same rows and alternate key
-// tiles, as two key ranges.
+// each tile has two warpgroups, whose threads own a row and half of its columns:
+// they read their 64 logits back, settle the row's maximum through shared memory,
+// keep maximum and sum in registers, write the weights over the logits and, where
+// the maximum grew by more than 2^8, rescale their half of the row of O.  While
+// one tile is in its softmax the tensor core works for the other.  Up to 128 rows
+// run with both tiles on the same rows and alternate key tiles, as two key ranges.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -76,9 +76,10 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     char *ring = smem + G::kRing;
     float *scales = (float *)(smem + G::kScaleAt);               // [kScaleRing][K, V][kTile]
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], raw_full[4], raw_empty[4];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], q_full;
     __shared__ float qscale[I8 ? 256 : 1];
     __shared__ float vmost[G::kScaleRing][2];
+    __shared__ float half_max[2][2][2][kTile];                   // [turn][tile][half][row]
     __shared__ const char *qrow[256];
     __shared__ uint32_t tmem_at;
     __shared__ int abort_at;
@@ -164,79 +165,27 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], kTile);
+            mbar_init(&p_full[i], 2 * kTile);
             mbar_init(&o_full[i], 1);
         }
+        mbar_init(&q_full, 32 * kMathWarps);
         abort_at = 0;
         fence_barrier_init();
     }
-    if (warp == 8) tc::alloc(&tmem_at, 512);
+    if (warp == kProductWarp) tc::alloc(&tmem_at, 512);
 
-    // the queries, in the products' layout; rows that do not exist are zeros
     for (int r = threadIdx.x; r < tiles * kTile; r += G::kThreads) {
         const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
         qrow[r] = r < rows ? (const char *)p.q + (b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) * (I8 ? 4 : 2) : nullptr;
     }
-    __syncthreads();
-    if constexpr (I8) {
-        // HD / 4 lanes a row, four rows of each lane in flight
-        constexpr int kLanes = HD / 4, kPer = G::kThreads / kLanes;
-        const int l = threadIdx.x % kLanes;
-        for (int r0 = threadIdx.x / kLanes; r0 < tiles * kTile; r0 += 4 * kPer) {
-            float4 x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r0 + e * kPer;
-                const char *q = r < tiles * kTile ? qrow[r] : nullptr;
-                x[e] = q ? *(const float4 *)(q + l * 16) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r0 + e * kPer;
-                float most = fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w)));
-#pragma unroll
-                for (int d = kLanes / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                float up, down;
-                row_scale(most, up, down);
-                uint2 h, lo2;
-                split2(x[e].x * up, x[e].y * up, h.x, lo2.x);
-                split2(x[e].z * up, x[e].w * up, h.y, lo2.y);
-                if (r < tiles * kTile) {
-                    if (l == 0) qscale[r] = p.scale2 * down;
-                    char *q = smem + (r / kTile) * 2 * G::kTileBytes + piece_at(r % kTile, l / 2) + (l & 1) * 8;
-                    *(uint2 *)q = h;
-                    *(uint2 *)(q + G::kTileBytes) = lo2;
-                }
-            }
-        }
-    } else {
-        constexpr int kChunks = HD / 8, kPer = G::kThreads / kChunks;
-        const int c = threadIdx.x % kChunks;
-        for (int r0 = threadIdx.x / kChunks; r0 < tiles * kTile; r0 += 6 * kPer) {
-            uint4 x[6];
-#pragma unroll
-            for (int e = 0; e < 6; ++e) {
-                const int r = r0 + e * kPer;
-                const char *q = r < tiles * kTile ? qrow[r] : nullptr;
-                x[e] = q ? *(const uint4 *)(q + c * 16) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < 6; ++e) {
-                const int r = r0 + e * kPer;
-                if (r < tiles * kTile)
-                    *(uint4 *)(smem + (r / kTile) * G::kTileBytes + piece_at(r % kTile, c)) = x[e];
-            }
-        }
-    }
-    fence_proxy_async();
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp >= 8) {
+    if (warp >= kMathWarps) {
         fewer_registers();
-        if (warp == 9) {
+        if (warp == kCopyWarp) {
             // ---- copies: tile j's K, then its V
             if (lane == 0) {
                 int issued = 0;
@@ -264,7 +213,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     mbar_wait(I8 ? &raw_full[i % kDepth] : &full[i % kDepth], (uint32_t)(i / kDepth) & 1);
             }
             __syncwarp();
-        } else if (warp == 8) {
+        } else if (warp == kProductWarp) {
             // ---- products
             const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring);
             constexpr uint32_t ids = idesc(BF, false, kTile), ido = idesc(BF, true, HD);
@@ -305,7 +254,9 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
                 return true;
             };
-            bool ok = n > 0;
+            // (K is waited for ahead of the weights where the ring allows it)
+            bool ok = n > 0 && wait_phase(&q_full, 0, abort_flag);
+            constexpr bool kAhead = kStages >= 4;
             if (alt) {
                 for (int j = 0; ok && j < min(n, 2); ++j) {
                     ok = have(2 * j);
@@ -319,7 +270,8 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
                 for (int j = 0; ok && j < n; ++j) {
                     const int w = j & 1;
-                    ok = have_v(j) && wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
+                    ok = have_v(j) && (!kAhead || j + 2 >= n || have(2 * j + 4)) &&
+                         wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
                     if (!ok) break;
                     __syncwarp();
                     if (elect_one()) {
@@ -330,7 +282,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     }
                     __syncwarp();
                     if (j + 2 < n) {
-                        ok = have(2 * j + 4);
+                        ok = kAhead || have(2 * j + 4);
                         __syncwarp();
                         if (ok && elect_one()) {
                             tc::fence_after();
@@ -350,7 +302,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
                 __syncwarp();
                 for (int j = 0; ok && j < n; ++j) {
-                    ok = have_v(j);
+                    ok = have_v(j) && (j + 1 >= n || have(2 * j + 2));
                     for (int w = 0; ok && w < tiles; ++w) {
                         ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
                         if (!ok) break;
@@ -363,9 +315,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                         }
                         __syncwarp();
                         if (j + 1 < n) {
-                            ok = w > 0 || have(2 * j + 2);
-                            __syncwarp();
-                            if (ok && elect_one()) {
+                            if (elect_one()) {
                                 tc::fence_after();
                                 logits(w, j + 1);
                                 if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
@@ -376,10 +326,10 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
             }
             __syncwarp();
-        } else if (warp >= 10) {
+        } else if (warp >= kConvertWarp) {
             // ---- INT8 tiles to FP16, exactly
             if constexpr (I8) {
-                const int me = threadIdx.x - 320;
+                const int me = threadIdx.x - 32 * kConvertWarp;
                 constexpr int kN = 32 * G::kConverters, kChunks = HD / 16;
                 for (int i = 0; i < 2 * n; ++i) {
                     const int s = i % kStages, rs = i % G::kRaw, j = i >> 1;
@@ -403,7 +353,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                             sk[me + e * kN] = kx[e];
                             sk[kTile + me + e * kN] = vx[e];
                         }
-                        if (lane == 0) vmost[j % G::kScaleRing][warp - 10] = most;
+                        if (lane == 0) vmost[j % G::kScaleRing][warp - kConvertWarp] = most;
                     } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
                         break;
                     }
@@ -426,9 +376,65 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
         }
     } else {
         more_registers();
-        // ---- softmax: thread = row
-        const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
-        const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // key tiles of this warpgroup
+        // the queries, in the products' layout; rows that do not exist are zeros
+        constexpr int kN = 32 * kMathWarps;
+        if constexpr (I8) {
+            // HD / 4 lanes a row, four rows of each lane in flight
+            constexpr int kLanes = HD / 4, kPer = kN / kLanes;
+            const int l = threadIdx.x % kLanes;
+            for (int r0 = threadIdx.x / kLanes; r0 < tiles * kTile; r0 += 4 * kPer) {
+                float4 x[4];
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r0 + e * kPer;
+                    const char *q = r < tiles * kTile ? qrow[r] : nullptr;
+                    x[e] = q ? *(const float4 *)(q + l * 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = r0 + e * kPer;
+                    float most = fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w)));
+    #pragma unroll
+                    for (int d = kLanes / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    float up, down;
+                    row_scale(most, up, down);
+                    uint2 h, lo2;
+                    split2(x[e].x * up, x[e].y * up, h.x, lo2.x);
+                    split2(x[e].z * up, x[e].w * up, h.y, lo2.y);
+                    if (r < tiles * kTile) {
+                        if (l == 0) qscale[r] = p.scale2 * down;
+                        char *q = smem + (r / kTile) * 2 * G::kTileBytes + piece_at(r % kTile, l / 2) + (l & 1) * 8;
+                        *(uint2 *)q = h;
+                        *(uint2 *)(q + G::kTileBytes) = lo2;
+                    }
+                }
+            }
+        } else {
+            constexpr int kChunks = HD / 8, kPer = kN / kChunks;
+            const int c = threadIdx.x % kChunks;
+            for (int r0 = threadIdx.x / kChunks; r0 < tiles * kTile; r0 += 6 * kPer) {
+                uint4 x[6];
+    #pragma unroll
+                for (int e = 0; e < 6; ++e) {
+                    const int r = r0 + e * kPer;
+                    const char *q = r < tiles * kTile ? qrow[r] : nullptr;
+                    x[e] = q ? *(const uint4 *)(q + c * 16) : make_uint4(0, 0, 0, 0);
+                }
+    #pragma unroll
+                for (int e = 0; e < 6; ++e) {
+                    const int r = r0 + e * kPer;
+                    if (r < tiles * kTile)
+                        *(uint4 *)(smem + (r / kTile) * G::kTileBytes + piece_at(r % kTile, c)) = x[e];
+                }
+            }
+        }
+        fence_proxy_async();
+        mbar_arrive(&q_full);
+
+        // ---- softmax: thread = row and half of the columns
+        constexpr int kCols = kTile / 2;
+        const int w = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & (kTile - 1);
+        const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // key tiles of this row tile
         const int m = m0 + (alt ? r : w * kTile + r);
         const bool row_ok = (alt ? r : w * kTile + r) < rows;
         const int b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
@@ -438,54 +444,58 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             if (p.window) first = len - nq + t - p.window + 1;
         }
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + w * kTile + lanes, to = tmem + 2 * kTile + w * HD + lanes;
+        const uint32_t ts = tmem + w * kTile + lanes, to = tmem + 2 * kTile + w * HD + lanes + half * (HD / 2);
         float zs = p.scale2;
-        if constexpr (I8) zs = qscale[alt ? r : w * kTile + r];
+        if constexpr (I8) {
+            wait_phase(&q_full, 0, abort_flag);
+            zs = qscale[alt ? r : w * kTile + r];
+        }
         float top = kNegInf, sum = 0.f, vnorm = 0.f;
         bool ok = true;
         for (int i = 0; i < mine; ++i) {
-            const int j = alt ? 2 * i + w : i, j0 = lo + j * kTile;
+            const int j = alt ? 2 * i + w : i, j0 = lo + j * kTile + half * kCols;
             ok = wait_phase(&s_full[w], (uint32_t)i & 1, abort_flag);
-            if (I8) ok = ok && wait_phase(&full[(2 * j + 1) % kStages], (uint32_t)((2 * j + 1) / kStages) & 1, abort_flag);
-            if (!ok) break;
+            if (I8) {
+                const int v = 2 * j + 1;                  // (and the tile's scales)
+                ok = wait_phase(&full[v % kStages], (uint32_t)(v / kStages) & 1, abort_flag) && ok;
+            }
             tc::fence_after();
-            uint32_t raw[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
+            uint32_t raw[2][32];
+            tc::ld32(ts + half * kCols, raw[0]);
+            tc::ld32(ts + half * kCols + 32, raw[1]);
             tc::wait_ld();
-            float2 z[kTile / 2];
-            const float *sk = scales + (j % G::kScaleRing) * 2 * kTile;
+            float2 z[kCols / 2];
+            const float *sk = scales + (j % G::kScaleRing) * 2 * kTile + half * kCols;
 #pragma unroll
-            for (int c = 0; c < kTile / 2; ++c)
+            for (int c = 0; c < kCols / 2; ++c)
                 z[c] = make_float2(__uint_as_float(raw[c / 16][2 * (c % 16)]),
                                    __uint_as_float(raw[c / 16][2 * (c % 16) + 1]));
             if constexpr (I8) {
 #pragma unroll
-                for (int c = 0; c < kTile / 2; c += 2) {
+                for (int c = 0; c < kCols / 2; c += 2) {
                     const float4 s4 = *(const float4 *)(sk + 2 * c);
                     z[c] = mul2(z[c], make_float2(s4.x, s4.y));
                     z[c + 1] = mul2(z[c + 1], make_float2(s4.z, s4.w));
                 }
             }
-            if (j0 < first || j0 + kTile - 1 > last) {
+            if (j0 < first || j0 + kCols - 1 > last) {
                 const int x0 = first - j0, x1 = last - j0;
 #pragma unroll
-                for (int c = 0; c < kTile / 2; ++c) {
+                for (int c = 0; c < kCols / 2; ++c) {
                     if (2 * c < x0 || 2 * c > x1) z[c].x = kNegInf;
                     if (2 * c + 1 < x0 || 2 * c + 1 > x1) z[c].y = kNegInf;
                 }
             }
-            float best[4] = {z[0].x, z[0].y, z[1].x, z[1].y};
+            float best[4] = {fmaxf(z[0].x, z[0].y), fmaxf(z[1].x, z[1].y), fmaxf(z[2].x, z[2].y),
+                             fmaxf(z[3].x, z[3].y)};
 #pragma unroll
-            for (int c = 2; c < kTile / 2 - 2; c += 4) {
-                best[0] = max3(best[0], z[c].x, z[c].y);
-                best[1] = max3(best[1], z[c + 1].x, z[c + 1].y);
-                best[2] = max3(best[2], z[c + 2].x, z[c + 2].y);
-                best[3] = max3(best[3], z[c + 3].x, z[c + 3].y);
-            }
-            best[0] = max3(best[0], z[kTile / 2 - 2].x, z[kTile / 2 - 2].y);
-            best[1] = max3(best[1], z[kTile / 2 - 1].x, z[kTile / 2 - 1].y);
-            const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * zs;
+            for (int c = 4; c < kCols / 2; c += 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = max3(best[e], z[c + e].x, z[c + e].y);
+            const float part_max = max3(fmaxf(best[0], best[1]), best[2], best[3]);
+            half_max[i & 1][w][half][r] = part_max;
+            tile_sync(w);
+            const float now = fmaxf(part_max, half_max[i & 1][w][half ^ 1][r]) * zs;
             float keep = 1.f;
             if (now > top + kGrow || (top == kNegInf && now > kNegInf)) {
                 keep = ex2(top - now);                // top = -inf: 0
@@ -507,24 +517,23 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             }
             if (i > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t o[32];
-                    tc::ld32(to + 32 * c, o);
+                for (int c = 0; c < HD / 2; c += 16) {
+                    uint32_t o[16];
+                    tc::ld16(to + c, o);
                     tc::wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                    tc::st32(to + 32 * c, o);
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                    tc::st16(to + c, o);
                 }
             }
             const float base = top == kNegInf ? 0.f : -top;
             const float2 zs2 = make_float2(zs, zs), base2 = make_float2(base, base);
             float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            constexpr int kStep = I8 ? 16 : 32;       // 32-bit columns of TMEM a store takes
 #pragma unroll
-            for (int c = 0; c < kTile / 2; c += kStep) {
-                uint32_t hi16[kStep], lo16[I8 ? kStep : 1];
+            for (int c = 0; c < kCols / 2; c += 16) {      // 16 columns of TMEM a store takes
+                uint32_t hi16[16], lo16[I8 ? 16 : 1];
 #pragma unroll
-                for (int e = 0; e < kStep; ++e) {
+                for (int e = 0; e < 16; ++e) {
                     float2 x = fma2(z[c + e], zs2, base2);
                     if ((e & 7) < kFmaOf8) {
                         x = ex2_fma2(x);
@@ -543,21 +552,21 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                         hi16[e] = pack2<BF>(x.x, x.y);
                     }
                 }
-                if constexpr (I8) {
-                    tc::st16(ts + c, hi16);
-                    tc::st16(ts + kTile / 2 + c, lo16);
-                } else {
-                    tc::st32(ts + c, hi16);
-                }
+                // (over the logits: every thread of the tile has read its own, tile_sync above)
+                tc::st16(ts + half * (kCols / 2) + c, hi16);
+                if constexpr (I8) tc::st16(ts + kTile / 2 + half * (kCols / 2) + c, lo16);
             }
             part[0] = add2(part[0], part[1]);
             sum += part[0].x + part[0].y;
             tc::wait_st();
             tc::fence_before();
-            mbar_arrive(&p_full[w]);
+            if (ok) mbar_arrive(&p_full[w]);
         }
-        if (mine > 0 && ok) ok = wait_phase(&o_full[w], 0, abort_flag);
+        if (mine > 0) ok = wait_phase(&o_full[w], 0, abort_flag) && ok;
         tc::fence_after();
+        half_max[mine & 1][w][half][r] = sum;
+        tile_sync(w);
+        sum += half_max[mine & 1][w][half ^ 1][r];
         if (top == kNegInf && sum == sum) sum = 0.f;  // no visible key (its weights counted as 2^-126 each)
         if (ok && (alt || w < tiles)) {
             const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
@@ -567,41 +576,42 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             const bool direct = p.prefix_slots + p.own_slots == 1;
             const long long part = (slot + (alt ? w : 0)) * nrows + row;
             const bool write = row_ok && (!direct || t < own_tokens(p, b));
-            if (row_ok) {
+            if (row_ok && half == 0) {
                 if (!direct) {
                     p.part_lse[part] = lse;
                 } else {
-                    if (p.row_lse) p.row_lse[row] = lse;
+                    if (p.neg_lse) p.neg_lse[neg_lse_at(p, b, t, h)] = -lse;
                     if (p.lse && write) p.lse[row] = lse * kLn2;
                 }
             }
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
+            for (int c = 0; c < HD / 2; c += 16) {
+                uint32_t o[16];
                 if (mine > 0) {
-                    tc::ld32(to + 32 * c, o);
+                    tc::ld16(to + c, o);
                     tc::wait_ld();
                 }
-                float v[32];
+                float v[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+                for (int e = 0; e < 16; ++e) v[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
                 if (!write) continue;
+                const int d = half * (HD / 2) + c;
                 if (!direct) {
-                    float4 *dst = (float4 *)(p.part_o + part * HD + 32 * c);
+                    float4 *dst = (float4 *)(p.part_o + part * HD + d);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    for (int e = 0; e < 4; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                 } else {
-                    char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + 32 * c) * (I8 ? 4 : 2);
+                    char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + d) * (I8 ? 4 : 2);
                     if constexpr (I8) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
+                        for (int e = 0; e < 4; ++e)
                             ((float4 *)dst)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            ((uint4 *)dst)[e] =
-                                make_uint4(pack2<BF>(v[8 * e], v[8 * e + 1]), pack2<BF>(v[8 * e + 2], v[8 * e + 3]),
-                                           pack2<BF>(v[8 * e + 4], v[8 * e + 5]), pack2<BF>(v[8 * e + 6], v[8 * e + 7]));
+                        for (int e = 0; e < 2; ++e)
+                            ((uint4 *)dst)[e] = make_uint4(
+                                pack2<BF>(v[8 * e], v[8 * e + 1]), pack2<BF>(v[8 * e + 2], v[8 * e + 3]),
+                                pack2<BF>(v[8 * e + 4], v[8 * e + 5]), pack2<BF>(v[8 * e + 6], v[8 * e + 7]));
                     }
                 }
             }
@@ -610,7 +620,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 8) tc::dealloc(tmem, 512);
+    if (warp == kProductWarp) tc::dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
 }
 
@@ -618,8 +628,8 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
 //
 // The logits once more, keys as the rows: S^T = K Q^T for two tiles of 128 keys
 // against 128 query rows at a time, and sum over the rows of 2^(z - lse_row).
-// Thread = key: the sum runs along the thread's TMEM lane, so no value crosses
-// threads and the order of the additions is fixed.  K stays in shared memory
+// Thread = key and half of the rows: the sum runs along the thread's TMEM lane in
+// a fixed order.  K stays in shared memory
 // for the whole CTA; the rows come by TMA, their lse beside them; two TMEM
 // buffers a tile let the next product run during the exponentials, which bound
 // the kernel (one a logit, on the special-function unit or the FP32 pipe).
@@ -675,7 +685,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
     extern __shared__ __align__(16) char smem_raw[];
     char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2][2], s_free[2][2];
-    __shared__ __align__(16) float lse[kStages][I8 ? 2 : 1][kTile];   // -lse of the rows, INT8: their factors
+    __shared__ __align__(16) float lse[kStages][I8 ? 2 : 1][kTile];   // minus the rows' lse, INT8: their factors
     __shared__ uint32_t tmem_at;
     __shared__ int abort_at;
     volatile int *abort_flag = &abort_at;
@@ -694,16 +704,16 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 1 + 32);
-            mbar_init(&empty[i], 1 + 2 * kTile);
+            mbar_init(&empty[i], 1 + 4 * kTile);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i >> 1][i & 1], 1);
-            mbar_init(&s_free[i >> 1][i & 1], kTile);
+            mbar_init(&s_free[i >> 1][i & 1], 2 * kTile);
         }
         abort_at = 0;
         fence_barrier_init();
     }
-    if (warp == 8) tc::alloc(&tmem_at, 512);
+    if (warp == kProductWarp) tc::alloc(&tmem_at, 512);
     pdl_enter();
     if (n > 0) {
         // two tiles of keys (zeros where there are none)
@@ -735,7 +745,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
                 }
             }
         }
-        // rows behind a short tile stay what they are here: zeros
+        // rows behind a short tile stay what they are here: zeros, and weightless
+        for (int i = threadIdx.x; i < kStages * kTile; i += kTileThreads) {
+            lse[i / kTile][0][i % kTile] = kNegInf;
+            if constexpr (I8) lse[i / kTile][1][i % kTile] = 0.f;
+        }
         if (tile_rows < kTile) {
             char *q = smem + G::kRing;
             for (int i = threadIdx.x; i < kStages * G::kStageBytes / 16; i += kTileThreads)
@@ -748,33 +762,15 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
     tc::fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp >= 8) {
-        if (warp == 9) {
-            // ---- query rows and their lse
-            int issued = 0;
-            const long long lrow = (long long)b * p.tokens;
-            for (int i = 0; i < n; ++i) {
-                const int s = i % kStages, mi = m0 + i * tile_rows, left = rows - i * tile_rows;
-                // (the loads ahead of the wait for the stage)
-                float l[kTile / 32], f[kTile / 32];
-#pragma unroll
-                for (int e = 0; e < kTile / 32; ++e) {
-                    const int x = lane + 32 * e, m = mi + x;
-                    l[e] = kNegInf;
-                    f[e] = 0.f;
-                    if (x < tile_rows && x < left) {
-                        l[e] = -p.row_lse[(lrow + m / R) * p.heads + g * R + m % R];
-                        if constexpr (I8) f[e] = p.q16_scale[(long long)unit * TR + m];
-                    }
-                }
-                if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
-#pragma unroll
-                for (int e = 0; e < kTile / 32; ++e) {
-                    lse[s][0][lane + 32 * e] = l[e];
-                    if constexpr (I8) lse[s][1][lane + 32 * e] = f[e];
-                }
-                mbar_arrive(&full[s]);
-                if (lane == 0) {
+    if (warp >= kMathWarps) {
+        fewer_registers();
+        if (warp == kCopyWarp) {
+            // ---- query rows
+            if (lane == 0) {
+                int issued = 0;
+                for (int i = 0; i < n; ++i) {
+                    const int s = i % kStages, mi = m0 + i * tile_rows;
+                    if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
                     char *dst = smem + G::kRing + s * G::kStageBytes;
                     mbar_arrive_expect_tx(&full[s], G::kPieces * HD * 2 * tile_rows);
                     for (int x = 0; x < G::kPieces; ++x)
@@ -786,14 +782,33 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
                             else
                                 tma_load_4d(d, &mq, 64 * c, g * R, mi / R, b, &full[s]);
                         }
+                    ++issued;
                 }
-                ++issued;
-            }
-            if (lane == 0)
                 for (int i = max(0, issued - kStages); i < issued; ++i)
                     mbar_wait(&full[i % kStages], (uint32_t)(i / kStages) & 1);
+            }
             __syncwarp();
-        } else if (warp == 8) {
+        } else if (warp == kConvertWarp) {
+            // ---- their lse (and INT8 factors)
+            const float *src = p.neg_lse + (long long)unit * TR + m0, *fac = nullptr;
+            if constexpr (I8) fac = p.q16_scale + (long long)unit * TR + m0;
+            for (int i = 0; i < n; ++i) {
+                const int s = i % kStages, at = i * tile_rows;
+                if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+#pragma unroll
+                for (int e = 0; e < kTile / 32; ++e) {
+                    const int x = lane + 32 * e, m = min(at + x, rows - 1);   // (rows behind the last: not counted)
+                    if (x < tile_rows) {
+                        cp_async<4>(&lse[s][0][x], src + m);
+                        if constexpr (I8) cp_async<4>(&lse[s][1][x], fac + m);
+                    }
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[s]))
+                             : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+        } else if (warp == kProductWarp) {
             // ---- products
             constexpr uint32_t ids = idesc(BF, false, kTile);
             const uint32_t k0 = smem_addr(smem), q0 = smem_addr(smem) + G::kRing;
@@ -825,8 +840,10 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
         }
         __syncwarp();
     } else {
-        // ---- thread = key
-        const int w = warp >> 2, j = key0 + w * kTile + (threadIdx.x & (kTile - 1));
+        more_registers();
+        // ---- thread = key and half of the rows
+        constexpr int kCols = kTile / 2;
+        const int w = warp >> 3, half = (warp >> 2) & 1, j = key0 + w * kTile + (threadIdx.x & (kTile - 1));
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         float ks = p.scale2;
         if constexpr (I8) {
@@ -845,52 +862,52 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
             // (the rows' lse: written before the products' wait for the same phase)
             if (!wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag)) break;
             tc::fence_after();
-            const uint32_t ts = tmem + (2 * w + (i & 1)) * kTile + lanes;
-            uint32_t raw[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
+            const uint32_t ts = tmem + (2 * w + (i & 1)) * kTile + half * kCols + lanes;
+            uint32_t raw[2][32];
+            tc::ld32(ts, raw[0]);
+            tc::ld32(ts + 32, raw[1]);
             tc::wait_ld();
             tc::fence_before();
             mbar_arrive(&s_free[w][i & 1]);
-            const int x0 = (int)max(0LL, min((long long)kTile, from - (long long)i * tile_rows));
-            const int x1 = (int)max(0LL, min((long long)kTile, to - (long long)i * tile_rows));
+            const long long at = (long long)i * tile_rows + half * kCols;
+            const int x0 = (int)max(0LL, min((long long)kCols, from - at));
+            const int x1 = (int)max(0LL, min((long long)kCols, to - at));
+            const float *ls = &lse[s][0][half * kCols], *fs = &lse[s][I8 ? 1 : 0][half * kCols];
             float2 part[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) part[c] = make_float2(0.f, 0.f);
-            const bool whole = x0 == 0 && x1 == kTile;
-            if (__all_sync(0xffffffffu, whole)) {
+            if (__all_sync(0xffffffffu, x0 == 0 && x1 == kCols)) {
 #pragma unroll
-                for (int c = 0; c < kTile; c += 4) {
-                    const float4 l4 = *(const float4 *)&lse[s][0][c];
+                for (int c = 0; c < kCols; c += 4) {
+                    const float4 l4 = *(const float4 *)(ls + c);
                     float2 a = make_float2(__uint_as_float(raw[c / 32][c % 32]),
                                            __uint_as_float(raw[c / 32][c % 32 + 1]));
                     float2 d = make_float2(__uint_as_float(raw[c / 32][c % 32 + 2]),
                                            __uint_as_float(raw[c / 32][c % 32 + 3]));
                     if constexpr (I8) {
-                        const float4 f4 = *(const float4 *)&lse[s][1][c];
+                        const float4 f4 = *(const float4 *)(fs + c);
                         a = fma2(a, mul2(k2, make_float2(f4.x, f4.y)), make_float2(l4.x, l4.y));
                         d = fma2(d, mul2(k2, make_float2(f4.z, f4.w)), make_float2(l4.z, l4.w));
                     } else {
                         a = fma2(a, k2, make_float2(l4.x, l4.y));
                         d = fma2(d, k2, make_float2(l4.z, l4.w));
                     }
-                    if ((c / 4) % 8 < kWeightFmaOf8)
+                    if ((c / 4) % 8 < kWeightFmaOf8) {
                         a = ex2_fma2(a);
-                    else
-                        a = make_float2(ex2(a.x), ex2(a.y));
-                    if ((c / 4) % 8 < kWeightFmaOf8)
                         d = ex2_fma2(d);
-                    else
+                    } else {
+                        a = make_float2(ex2(a.x), ex2(a.y));
                         d = make_float2(ex2(d.x), ex2(d.y));
+                    }
                     part[(c / 4) & 1] = add2(part[(c / 4) & 1], a);
                     part[2 + ((c / 4) & 1)] = add2(part[2 + ((c / 4) & 1)], d);
                 }
-            } else {
+            } else if (x0 < x1) {
 #pragma unroll
-                for (int c = 0; c < kTile; ++c) {
+                for (int c = 0; c < kCols; ++c) {
                     float f = ks;
-                    if constexpr (I8) f *= lse[s][1][c];
-                    const float y = ex2(fmaf(__uint_as_float(raw[c / 32][c % 32]), f, lse[s][0][c]));
+                    if constexpr (I8) f *= fs[c];
+                    const float y = ex2(fmaf(__uint_as_float(raw[c / 32][c % 32]), f, ls[c]));
                     if (c >= x0 && c < x1) part[c & 3].x += y;
                 }
             }
@@ -898,14 +915,20 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
             part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
             total += part[0].x + part[0].y;
         }
-        if (j < p.capacity)
+        float *halves = &lse[0][0][0];                 // (free once every thread is past its rows)
+        static_assert(kStages >= 2, "room for the sums");
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        if (half) halves[w * kTile + (threadIdx.x & (kTile - 1))] = total;
+        tile_sync(2 + w);
+        if (!half && j < p.capacity)
             p.weights_out[b * p.wos[0] + g * p.wos[1] + j * p.wos[2]] =
-                p.weights[b * p.ws[0] + g * p.ws[1] + j * p.ws[2]] + total;
+                p.weights[b * p.ws[0] + g * p.ws[1] + j * p.ws[2]] +
+                (total + halves[w * kTile + (threadIdx.x & (kTile - 1))]);
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 8) tc::dealloc(tmem, 512);
+    if (warp == kProductWarp) tc::dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
 }
 

@@ -181,8 +181,18 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
 constexpr uint32_t kWaitLimit = 1u << 22;
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t a = smem_addr(bar);
+    uint32_t done;
+    // most phases have ended by the time they are asked for: a test first, since
+    // try_wait may suspend the thread for longer
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
-        uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -197,11 +207,16 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volat
     return false;
 }
 
-// Registers move between the warpgroups of a CTA of 384 threads of 168: two
-// softmax warpgroups of 208 and one of 88, 64512 in all as at the launch.
-constexpr int kTileThreads = 384;
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+// A CTA of the tile kernels: four warpgroups for the exponentials (two a tile of
+// 128 rows: thread = row and half of the columns) and one for products, copies and
+// conversions.  Registers move between them: of the 96 a thread at the launch,
+// 104 to the first four and 64 to the last, 61440 in all as before.
+constexpr int kTileThreads = 640;
+constexpr int kMathWarps = 16, kProductWarp = 16, kCopyWarp = 17, kConvertWarp = 18;
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+// The 256 threads of one tile.
+__device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); }
 
 }  // namespace tile
 }  // namespace nb200
