@@ -3,15 +3,19 @@
 // chunk or prompt against its own keys.  Formulas and the row and
 // partial-result conventions: prefix_attention.cuh.
 //
-// One CTA attends up to 256 rows (two tiles of 128) to one key range, 128 keys
-// at a time.  A warp feeds K and V by TMA, one thread issues the products
-// S = Q K^T (into TMEM) and O += P V (P from TMEM, V from shared memory), and
-// each tile has two warpgroups, whose threads own a row and half of its columns:
-// they read their 64 logits back, settle the row's maximum through shared memory,
-// keep maximum and sum in registers, write the weights over the logits and, where
-// the maximum grew by more than 2^8, rescale their half of the row of O.  While
-// one tile is in its softmax the tensor core works for the other.  Up to 128 rows
-// run with both tiles on the same rows and alternate key tiles, as two key ranges.
+// One CTA attends up to 256 rows (two tiles of 128) to one key range, 128 keys at
+// a time.  A warp feeds K and V by TMA, one thread issues the products S = Q K^T
+// (into TMEM) and O += P V (P from TMEM, V from shared memory), and each tile has
+// a warpgroup whose thread i owns row i: it reads its 128 logits back, keeps the
+// row's maximum and sum in registers, writes the weights over the logits (the
+// first half's product starts while the second is computed) and, where the
+// maximum grew by more than 2^8, rescales its row of O.  While one tile is in its
+// softmax the tensor core works for the other.  TMEM holds the two tiles' O and
+// two (128 dimensions) or three (64) buffers of logits; with three, a tile's next
+// logits are computed during its softmax.  Steps of 64 keys with four buffers
+// were slower (480 against 345 us for two prompts of 4096 tokens): a product of
+// 64 columns takes nearly the time of one of 128.  Up to 128 rows run with both
+// tiles on the same rows and alternate key steps, as two key ranges.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -34,24 +38,45 @@ constexpr int kFmaOf8 = 2;                       // of 8 powers of two, those on
 constexpr int kWeightFmaOf8 = 3;                 // the same of the key weights
 constexpr float kGrow = 8.f;                     // log2 growth of a maximum that is left to the weights
 
+constexpr int kStep = 128;                       // keys of a step
+constexpr int kTileThreads = 384;                // two warpgroups of rows, one of products, copies, conversions
+constexpr int kMathWarps = 8, kProductWarp = 8, kCopyWarp = 9, kConvertWarp = 10;
+// 2 * 128 * 208 + 128 * 88 = 384 * 168
+constexpr int kMathRegisters = 208, kOtherRegisters = 88;
+
 template <int TYPE, int HD>
 struct TileGeom {
     static constexpr bool I8 = TYPE == kCacheI8;
     static constexpr int kPieces = I8 ? 2 : 1;                    // FP32 queries and weights as FP16 pairs
-    static constexpr int kTileBytes = kTile * HD * 2;             // a Q, K or V tile of 16-bit values
+    static constexpr int kQBytes = kTile * HD * 2;                // a piece of a tile of queries
+    static constexpr int kKVBytes = kStep * HD * 2;               // a step's K or V in 16 bits
     // the FP32 queries' pairs of two 128-dimension tiles would fill the shared memory
     static constexpr int kQTiles = I8 && HD == 128 ? 1 : 2;
     static constexpr int kStages = HD == 64 ? (I8 ? 4 : 6) : (I8 ? 3 : 4);
-    static constexpr int kRaw = I8 ? (HD == 64 ? 4 : 2) : 0;      // INT8 tiles on their way
-    static constexpr int kRawBytes = kTile * HD;
-    static constexpr int kScaleRing = 4;
-    static constexpr int kRing = kQTiles * kPieces * kTileBytes;
-    static constexpr int kRawAt = kRing + kStages * kTileBytes;
+    static constexpr int kBuffers = HD == 64 ? 3 : 2;             // of logits
+    // whether a step's K can be there before the weights of kBuffers items earlier
+    static constexpr bool kEarly = kStages >= (kBuffers == 3 ? 6 : 4);
+    static constexpr int kRaw = I8 ? (HD == 64 ? 4 : 2) : 0;      // INT8 steps on their way
+    static constexpr int kRawBytes = kStep * HD;
+    static constexpr int kScaleRing = 8;                          // steps whose scales are held
+    static constexpr int kRing = kQTiles * kPieces * kQBytes;
+    static constexpr int kRawAt = kRing + kStages * kKVBytes;
     static constexpr int kScaleAt = kRawAt + kRaw * kRawBytes;
-    static constexpr int kSmem = kScaleAt + (I8 ? kScaleRing * 2 * kTile * 4 : 0) + 1024;
+    static constexpr int kSmem = kScaleAt + (I8 ? kScaleRing * 2 * kStep * 4 : 0) + 1024;
     static constexpr int kConverters = I8 ? 2 : 0;                // warps
-    static constexpr int kThreads = kTileThreads;
     static_assert(kSmem <= 232448 - 4096, "shared memory of a CTA");
+    // a step's scales are written when the stage of the K kStages / 2 steps before is
+    // free, at which time softmaxes of the kBuffers - 1 steps before that may be running
+    static_assert(kScaleRing >= kStages / 2 + kBuffers, "scales in use");
+};
+
+// The buffers of logits in turn, and the phase of their barriers.
+struct Turn {
+    int buffer = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void on(int items, int buffers) {
+        for (buffer += items; buffer >= buffers; buffer -= buffers) phase ^= 1;
+    }
 };
 
 // Units of work: (range, row tiles, KV head[, sequence]).
@@ -64,7 +89,7 @@ struct TileGrid {
 };
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_kernel(
+__global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
     const PrefixAttn p, const TileGrid grid, const __grid_constant__ CUtensorMap mk,
     const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mpk,
     const __grid_constant__ CUtensorMap mpv) {
@@ -74,12 +99,11 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     extern __shared__ __align__(16) char smem_raw[];
     char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     char *ring = smem + G::kRing;
-    float *scales = (float *)(smem + G::kScaleAt);               // [kScaleRing][K, V][kTile]
+    float *scales = (float *)(smem + G::kScaleAt);               // [kScaleRing][K, V][kStep]
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], raw_full[4], raw_empty[4];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], q_full;
+    __shared__ __align__(8) uint64_t s_full[3], p_full[3][2], o_done[2], o_full[2], q_full;
     __shared__ float qscale[I8 ? 256 : 1];
     __shared__ float vmost[G::kScaleRing][2];
-    __shared__ float half_max[2][2][2][kTile];                   // [turn][tile][half][row]
     __shared__ const char *qrow[256];
     __shared__ uint32_t tmem_at;
     __shared__ int abort_at;
@@ -110,7 +134,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
         hi = max(0, min(len, len - nq + t1 + 1));
         lo = p.window ? max(0, len - nq + t0 - p.window + 1) : 0;
         if (t0 >= nq) rows = 0;
-        const int n = max(0, hi - lo), each = (ceil_div(n, grid.own_ranges) + kTile - 1) / kTile * kTile;
+        const int n = max(0, hi - lo), each = (ceil_div(n, grid.own_ranges) + kStep - 1) / kStep * kStep;
         const int a = min(hi, lo + slot * each);
         hi = min(hi, a + each);
         lo = a;
@@ -134,7 +158,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
         g = unit / grid.prefix_tiles;
         m0 = tile * grid.prefix_rows;
         rows = min(grid.prefix_rows, p.batch * TR - m0);
-        const int each = (ceil_div(p.prefix, grid.prefix_ranges) + kTile - 1) / kTile * kTile;
+        const int each = (ceil_div(p.prefix, grid.prefix_ranges) + kStep - 1) / kStep * kStep;
         lo = min(p.prefix, slot * each);
         hi = min(p.prefix, lo + each);
         slot = alt ? 2 * slot : slot;
@@ -151,8 +175,12 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     // the streaming kernel of the same call works on other keys: it may start beside this one
     if (grid.stream_next) pdl_launch_dependents();
     if (rows <= 0) return;                        // the whole CTA
-    const int n = ceil_div(max(0, hi - lo), kTile);              // key tiles
+    const int n = ceil_div(max(0, hi - lo), kStep);              // steps of keys
     const int tiles = alt ? 1 : (rows > kTile ? 2 : 1);          // row tiles
+    // item k: step and tile; its logits in buffer k % ahead, so that they follow the
+    // output product of the item `ahead` before: one of its tile's last two, and the
+    // products of its tile's items before that have ended when they are there
+    const int each = alt ? 1 : tiles, items = n * each, ahead = alt || tiles == 2 ? G::kBuffers : 2;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
@@ -163,9 +191,13 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             mbar_init(&raw_full[i], 1);
             mbar_init(&raw_empty[i], 32 * G::kConverters);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 3; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 2 * kTile);
+            mbar_init(&p_full[i][0], kTile);
+            mbar_init(&p_full[i][1], kTile);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&o_done[i], 1);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(&q_full, 32 * kMathWarps);
@@ -174,7 +206,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     }
     if (warp == kProductWarp) tc::alloc(&tmem_at, 512);
 
-    for (int r = threadIdx.x; r < tiles * kTile; r += G::kThreads) {
+    for (int r = threadIdx.x; r < tiles * kTile; r += kTileThreads) {
         const int m = m0 + r, b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
         qrow[r] = r < rows ? (const char *)p.q + (b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) * (I8 ? 4 : 2) : nullptr;
     }
@@ -184,14 +216,14 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
     const uint32_t tmem = tmem_at;
 
     if (warp >= kMathWarps) {
-        fewer_registers();
+        fewer_registers<kOtherRegisters>();
         if (warp == kCopyWarp) {
             // ---- copies: tile j's K, then its V
             if (lane == 0) {
                 int issued = 0;
                 for (int i = 0; i < 2 * n; ++i) {
                     const CUtensorMap *map = i & 1 ? vm : km;
-                    const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kTile;
+                    const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kStep;
                     if constexpr (I8) {
                         const int s = i % G::kRaw;
                         if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
@@ -200,10 +232,10 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     } else {
                         const int s = i % kStages;
                         if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
-                        mbar_arrive_expect_tx(&full[s], G::kTileBytes);
+                        mbar_arrive_expect_tx(&full[s], G::kKVBytes);
     #pragma unroll
                         for (int c = 0; c < HD / 64; ++c)
-                            tma_load_4d(ring + s * G::kTileBytes + c * (kTile * 128), map, 64 * c, key, z, w, &full[s]);
+                            tma_load_4d(ring + s * G::kKVBytes + c * (kStep * 128), map, 64 * c, key, z, w, &full[s]);
                     }
                     ++issued;
                 }
@@ -215,115 +247,88 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             __syncwarp();
         } else if (warp == kProductWarp) {
             // ---- products
-            const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring);
-            constexpr uint32_t ids = idesc(BF, false, kTile), ido = idesc(BF, true, HD);
-            auto logits = [&](int w, int j) {             // S_w = Q_w K_j^T
-                const uint32_t k = r0 + ((2 * j) % kStages) * G::kTileBytes;
-                const uint32_t q = q0 + (alt ? 0 : w) * (G::kPieces * G::kTileBytes);
-    #pragma unroll
-                for (int x = 0; x < G::kPieces; ++x)
-    #pragma unroll
-                    for (int c = 0; c < HD / 16; ++c) {
-                        const uint32_t at = (c / 4) * (kTile * 128) + (c % 4) * 32;
-                        tc::mma_bf16_ss(tmem + w * kTile, desc_k(q + x * G::kTileBytes + at), desc_k(k + at), ids,
-                                        x + c > 0);
-                    }
-                tc::commit(&s_full[w]);
-            };
-            auto values = [&](int w, int j, bool first) {  // O_w += P_w V_j
-                const uint32_t v = r0 + ((2 * j + 1) % kStages) * G::kTileBytes;
-    #pragma unroll
-                for (int x = 0; x < G::kPieces; ++x)
-    #pragma unroll
-                    for (int c = 0; c < kTile / 16; ++c)
-                        mma_ts(tmem + 2 * kTile + w * HD, tmem + w * kTile + x * (kTile / 2) + c * 8, desc_mn(v + c * 2048),
-                               ido, !first || x + c > 0);
-            };
+            const uint32_t q0 = smem_addr(smem), r0 = smem_addr(ring), s0 = tmem + 2 * HD;
+            constexpr uint32_t ids = idesc(BF, false, kStep), ido = idesc(BF, true, HD);
+            auto step_of = [&](int k) { return each == 2 ? k >> 1 : k; };
+            auto tile_of = [&](int k) { return alt || each == 2 ? k & 1 : 0; };
             auto have = [&](int i) { return wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
+            auto logits = [&](int k, int buffer) {        // S_k = Q K^T
+                const int i = 2 * step_of(k), w = tile_of(k);
+                const uint32_t kt = r0 + (i % kStages) * G::kKVBytes;
+                const uint32_t q = q0 + (alt ? 0 : w) * (G::kPieces * G::kQBytes);
+                __syncwarp();
+                if (elect_one()) {
+                    tc::fence_after();
+#pragma unroll
+                    for (int x = 0; x < G::kPieces; ++x)
+#pragma unroll
+                        for (int c = 0; c < HD / 16; ++c)
+                            tc::mma_bf16_ss(s0 + buffer * kStep,
+                                            desc_k(q + x * G::kQBytes + (c / 4) * (kTile * 128) + (c % 4) * 32),
+                                            desc_k(kt + (c / 4) * (kStep * 128) + (c % 4) * 32), ids, x + c > 0);
+                    tc::commit(&s_full[buffer]);
+                    if (each == 1 || w == 1) tc::commit(&empty[i % kStages]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int k, int buffer, int half) {   // O += P_k V, half of the keys
+                const int i = 2 * step_of(k) + 1, w = tile_of(k);
+                const uint32_t v = r0 + (i % kStages) * G::kKVBytes, pk = s0 + buffer * kStep;
+                const bool first = k < (alt ? 2 : each) && half == 0;
+                __syncwarp();
+                if (elect_one()) {
+                    tc::fence_after();
+#pragma unroll
+                    for (int x = 0; x < G::kPieces; ++x)
+#pragma unroll
+                        for (int e = 0; e < kStep / 32; ++e) {
+                            const int c = half * (kStep / 32) + e;
+                            mma_ts(tmem + w * HD, pk + x * (kStep / 2) + c * 8, desc_mn<kStep>(v + c * 2048), ido,
+                                   !first || x + e > 0);
+                        }
+                    if (half) {
+                        tc::commit(&o_done[w]);
+                        if (k + (alt ? 2 : each) >= items) tc::commit(&o_full[w]);
+                        if (each == 1 || w == 1) tc::commit(&empty[i % kStages]);
+                    }
+                }
+                __syncwarp();
+            };
             auto have_v = [&](int j) {
                 if (!have(2 * j + 1)) return false;
-                const int valid = hi - lo - j * kTile;
-                if (!I8 && valid < kTile) {               // rows behind the range: whatever they hold, zeros
-                    char *v = ring + ((2 * j + 1) % kStages) * G::kTileBytes;
-                    for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
-    #pragma unroll
+                const int valid = hi - lo - j * kStep;
+                if (!I8 && valid < kStep) {               // rows behind the range: whatever they hold, zeros
+                    char *v = ring + ((2 * j + 1) % kStages) * G::kKVBytes;
+                    for (int i = valid * 8 + lane; i < kStep * 8; i += 32)
+#pragma unroll
                         for (int c = 0; c < HD / 64; ++c)
-                            *(uint4 *)(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                            *(uint4 *)(v + c * (kStep * 128) + i * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async();
-                    __syncwarp();
                 }
+                __syncwarp();
                 return true;
             };
-            // (K is waited for ahead of the weights where the ring allows it)
             bool ok = n > 0 && wait_phase(&q_full, 0, abort_flag);
-            constexpr bool kAhead = kStages >= 4;
-            if (alt) {
-                for (int j = 0; ok && j < min(n, 2); ++j) {
-                    ok = have(2 * j);
-                    __syncwarp();
-                    if (ok && elect_one()) {
-                        tc::fence_after();
-                        logits(j, j);
-                        tc::commit(&empty[(2 * j) % kStages]);
-                    }
-                    __syncwarp();
+            for (int k = 0; ok && k < min(items, ahead); ++k) {
+                ok = have(2 * step_of(k));
+                if (ok) logits(k, k);
+            }
+            Turn turn;
+            for (int k = 0; ok && k < items; ++k) {
+                const bool more = k + ahead < items;
+                ok = ((each == 2 && (k & 1)) || have_v(step_of(k))) &&
+                     (!G::kEarly || !more || have(2 * step_of(k + ahead))) &&
+                     wait_phase(&p_full[turn.buffer][0], turn.phase, abort_flag);
+                if (!ok) break;
+                values(k, turn.buffer, 0);
+                ok = wait_phase(&p_full[turn.buffer][1], turn.phase, abort_flag);
+                if (!ok) break;
+                values(k, turn.buffer, 1);
+                if (more) {
+                    ok = G::kEarly || have(2 * step_of(k + ahead));
+                    if (ok) logits(k + ahead, turn.buffer);
                 }
-                for (int j = 0; ok && j < n; ++j) {
-                    const int w = j & 1;
-                    ok = have_v(j) && (!kAhead || j + 2 >= n || have(2 * j + 4)) &&
-                         wait_phase(&p_full[w], (uint32_t)(j >> 1) & 1, abort_flag);
-                    if (!ok) break;
-                    __syncwarp();
-                    if (elect_one()) {
-                        tc::fence_after();
-                        values(w, j, j < 2);
-                        tc::commit(&empty[(2 * j + 1) % kStages]);
-                        if (j + 2 >= n) tc::commit(&o_full[w]);
-                    }
-                    __syncwarp();
-                    if (j + 2 < n) {
-                        ok = kAhead || have(2 * j + 4);
-                        __syncwarp();
-                        if (ok && elect_one()) {
-                            tc::fence_after();
-                            logits(w, j + 2);
-                            tc::commit(&empty[(2 * j + 4) % kStages]);
-                        }
-                        __syncwarp();
-                    }
-                }
-            } else {
-                ok = ok && have(0);
-                __syncwarp();
-                if (ok && elect_one()) {
-                    tc::fence_after();
-                    for (int w = 0; w < tiles; ++w) logits(w, 0);
-                    tc::commit(&empty[0]);
-                }
-                __syncwarp();
-                for (int j = 0; ok && j < n; ++j) {
-                    ok = have_v(j) && (j + 1 >= n || have(2 * j + 2));
-                    for (int w = 0; ok && w < tiles; ++w) {
-                        ok = wait_phase(&p_full[w], (uint32_t)j & 1, abort_flag);
-                        if (!ok) break;
-                        __syncwarp();
-                        if (elect_one()) {
-                            tc::fence_after();
-                            values(w, j, j == 0);
-                            if (w == tiles - 1) tc::commit(&empty[(2 * j + 1) % kStages]);
-                            if (j == n - 1) tc::commit(&o_full[w]);
-                        }
-                        __syncwarp();
-                        if (j + 1 < n) {
-                            if (elect_one()) {
-                                tc::fence_after();
-                                logits(w, j + 1);
-                                if (w == tiles - 1) tc::commit(&empty[(2 * j + 2) % kStages]);
-                            }
-                            __syncwarp();
-                        }
-                    }
-                }
+                turn.on(1, ahead);
             }
             __syncwarp();
         } else if (warp >= kConvertWarp) {
@@ -334,24 +339,23 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 for (int i = 0; i < 2 * n; ++i) {
                     const int s = i % kStages, rs = i % G::kRaw, j = i >> 1;
                     if (!(i & 1)) {
-                        // both scales of the tile's keys (V's zero behind the range), and V's largest
-                        float *sk = scales + (j % G::kScaleRing) * 2 * kTile, most = 0.f;
-                        float kx[kTile / kN], vx[kTile / kN];
+                        // both scales of the step's keys (V's zero behind the range), and V's largest
+                        float *sk = scales + (j % G::kScaleRing) * 2 * kStep, most = 0.f;
+                        float kx[kStep / kN], vx[kStep / kN];
     #pragma unroll
-                        for (int e = 0; e < kTile / kN; ++e) {
-                            const int key = lo + j * kTile + me + e * kN;
+                        for (int e = 0; e < kStep / kN; ++e) {
+                            const int key = lo + j * kStep + me + e * kN;
                             kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
                             vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
                             most = fmaxf(most, fabsf(vx[e]));
                         }
     #pragma unroll
                         for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                        // the tile kScaleRing before has been attended: its V was consumed for this stage
                         if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
     #pragma unroll
-                        for (int e = 0; e < kTile / kN; ++e) {
+                        for (int e = 0; e < kStep / kN; ++e) {
                             sk[me + e * kN] = kx[e];
-                            sk[kTile + me + e * kN] = vx[e];
+                            sk[kStep + me + e * kN] = vx[e];
                         }
                         if (lane == 0) vmost[j % G::kScaleRing][warp - kConvertWarp] = most;
                     } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
@@ -359,14 +363,14 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     }
                     if (!wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag)) break;
                     const char *src = smem + G::kRawAt + rs * G::kRawBytes;
-                    char *dst = ring + s * G::kTileBytes;
+                    char *dst = ring + s * G::kKVBytes;
     #pragma unroll 4
-                    for (int x = me; x < kTile * kChunks; x += kN) {
+                    for (int x = me; x < kStep * kChunks; x += kN) {
                         const int r = x / kChunks, c = x % kChunks;
                         uint4 a, b;
                         i8x16_to_f16(*(const uint4 *)(src + x * 16), a, b);
-                        *(uint4 *)(dst + piece_at(r, 2 * c)) = a;
-                        *(uint4 *)(dst + piece_at(r, 2 * c + 1)) = b;
+                        *(uint4 *)(dst + piece_at<kStep>(r, 2 * c)) = a;
+                        *(uint4 *)(dst + piece_at<kStep>(r, 2 * c + 1)) = b;
                     }
                     fence_proxy_async();
                     mbar_arrive(&raw_empty[rs]);
@@ -375,7 +379,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             }
         }
     } else {
-        more_registers();
+        more_registers<kMathRegisters>();
         // the queries, in the products' layout; rows that do not exist are zeros
         constexpr int kN = 32 * kMathWarps;
         if constexpr (I8) {
@@ -403,9 +407,9 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     split2(x[e].z * up, x[e].w * up, h.y, lo2.y);
                     if (r < tiles * kTile) {
                         if (l == 0) qscale[r] = p.scale2 * down;
-                        char *q = smem + (r / kTile) * 2 * G::kTileBytes + piece_at(r % kTile, l / 2) + (l & 1) * 8;
+                        char *q = smem + (r / kTile) * 2 * G::kQBytes + piece_at<kTile>(r % kTile, l / 2) + (l & 1) * 8;
                         *(uint2 *)q = h;
-                        *(uint2 *)(q + G::kTileBytes) = lo2;
+                        *(uint2 *)(q + G::kQBytes) = lo2;
                     }
                 }
             }
@@ -424,17 +428,16 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 for (int e = 0; e < 6; ++e) {
                     const int r = r0 + e * kPer;
                     if (r < tiles * kTile)
-                        *(uint4 *)(smem + (r / kTile) * G::kTileBytes + piece_at(r % kTile, c)) = x[e];
+                        *(uint4 *)(smem + (r / kTile) * G::kQBytes + piece_at<kTile>(r % kTile, c)) = x[e];
                 }
             }
         }
         fence_proxy_async();
         mbar_arrive(&q_full);
 
-        // ---- softmax: thread = row and half of the columns
-        constexpr int kCols = kTile / 2;
-        const int w = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & (kTile - 1);
-        const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // key tiles of this row tile
+        // ---- softmax: thread = row
+        const int w = warp >> 2, r = threadIdx.x & (kTile - 1);
+        const int mine = alt ? (n - w + 1) >> 1 : (w < tiles ? n : 0);   // steps of this tile
         const int m = m0 + (alt ? r : w * kTile + r);
         const bool row_ok = (alt ? r : w * kTile + r) < rows;
         const int b = m / TR, t = (m - b * TR) / R, h = g * R + m % R;
@@ -444,7 +447,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             if (p.window) first = len - nq + t - p.window + 1;
         }
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + w * kTile + lanes, to = tmem + 2 * kTile + w * HD + lanes + half * (HD / 2);
+        const uint32_t s0 = tmem + 2 * HD + lanes, to = tmem + w * HD + lanes;
         float zs = p.scale2;
         if constexpr (I8) {
             wait_phase(&q_full, 0, abort_flag);
@@ -452,36 +455,40 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
         }
         float top = kNegInf, sum = 0.f, vnorm = 0.f;
         bool ok = true;
-        for (int i = 0; i < mine; ++i) {
-            const int j = alt ? 2 * i + w : i, j0 = lo + j * kTile + half * kCols;
-            ok = wait_phase(&s_full[w], (uint32_t)i & 1, abort_flag);
+        Turn turn;
+        turn.on(w, ahead);
+        for (int i = 0; i < mine; ++i, turn.on(each == 2 || alt ? 2 : 1, ahead)) {
+            const int j = alt ? 2 * i + w : i, j0 = lo + j * kStep;
+            ok = wait_phase(&s_full[turn.buffer], turn.phase, abort_flag);
             if (I8) {
-                const int v = 2 * j + 1;                  // (and the tile's scales)
-                ok = wait_phase(&full[v % kStages], (uint32_t)(v / kStages) & 1, abort_flag) && ok;
+                const int v = 2 * j + 1;                  // (and the step's scales)
+                ok = ok && wait_phase(&full[v % kStages], (uint32_t)(v / kStages) & 1, abort_flag);
             }
+            if (!ok) break;
             tc::fence_after();
-            uint32_t raw[2][32];
-            tc::ld32(ts + half * kCols, raw[0]);
-            tc::ld32(ts + half * kCols + 32, raw[1]);
-            tc::wait_ld();
-            float2 z[kCols / 2];
-            const float *sk = scales + (j % G::kScaleRing) * 2 * kTile + half * kCols;
+            const uint32_t ts = s0 + turn.buffer * kStep;
+            uint32_t raw[4][32];
 #pragma unroll
-            for (int c = 0; c < kCols / 2; ++c)
+            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
+            tc::wait_ld();
+            float2 z[kStep / 2];
+            const float *sk = scales + (j % G::kScaleRing) * 2 * kStep;
+#pragma unroll
+            for (int c = 0; c < kStep / 2; ++c)
                 z[c] = make_float2(__uint_as_float(raw[c / 16][2 * (c % 16)]),
                                    __uint_as_float(raw[c / 16][2 * (c % 16) + 1]));
             if constexpr (I8) {
 #pragma unroll
-                for (int c = 0; c < kCols / 2; c += 2) {
+                for (int c = 0; c < kStep / 2; c += 2) {
                     const float4 s4 = *(const float4 *)(sk + 2 * c);
                     z[c] = mul2(z[c], make_float2(s4.x, s4.y));
                     z[c + 1] = mul2(z[c + 1], make_float2(s4.z, s4.w));
                 }
             }
-            if (j0 < first || j0 + kCols - 1 > last) {
+            if (j0 < first || j0 + kStep - 1 > last) {
                 const int x0 = first - j0, x1 = last - j0;
 #pragma unroll
-                for (int c = 0; c < kCols / 2; ++c) {
+                for (int c = 0; c < kStep / 2; ++c) {
                     if (2 * c < x0 || 2 * c > x1) z[c].x = kNegInf;
                     if (2 * c + 1 < x0 || 2 * c + 1 > x1) z[c].y = kNegInf;
                 }
@@ -489,13 +496,10 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             float best[4] = {fmaxf(z[0].x, z[0].y), fmaxf(z[1].x, z[1].y), fmaxf(z[2].x, z[2].y),
                              fmaxf(z[3].x, z[3].y)};
 #pragma unroll
-            for (int c = 4; c < kCols / 2; c += 4)
+            for (int c = 4; c < kStep / 2; c += 4)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) best[e] = max3(best[e], z[c + e].x, z[c + e].y);
-            const float part_max = max3(fmaxf(best[0], best[1]), best[2], best[3]);
-            half_max[i & 1][w][half][r] = part_max;
-            tile_sync(w);
-            const float now = fmaxf(part_max, half_max[i & 1][w][half ^ 1][r]) * zs;
+            const float now = max3(fmaxf(best[0], best[1]), best[2], best[3]) * zs;
             float keep = 1.f;
             if (now > top + kGrow || (top == kNegInf && now > kNegInf)) {
                 keep = ex2(top - now);                // top = -inf: 0
@@ -516,21 +520,25 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 vinv = 64.f / vnorm;
             }
             if (i > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+                // O holds the steps before: the last one's product has to end first (the
+                // ones before that had ended when these logits were computed)
+                ok = wait_phase(&o_done[w], (uint32_t)(i - 1) & 1, abort_flag);
+                tc::fence_after();
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 16) {
-                    uint32_t o[16];
-                    tc::ld16(to + c, o);
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tc::ld32(to + c, o);
                     tc::wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                    tc::st16(to + c, o);
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                    tc::st32(to + c, o);
                 }
             }
             const float base = top == kNegInf ? 0.f : -top;
             const float2 zs2 = make_float2(zs, zs), base2 = make_float2(base, base);
             float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < kCols / 2; c += 16) {      // 16 columns of TMEM a store takes
+            for (int c = 0; c < kStep / 2; c += 16) {      // 16 columns of TMEM a store takes
                 uint32_t hi16[16], lo16[I8 ? 16 : 1];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -543,7 +551,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                     }
                     part[e & 1] = add2(part[e & 1], x);
                     if constexpr (I8) {
-                        const float2 v2 = *(const float2 *)(sk + kTile + 2 * (c + e));
+                        const float2 v2 = *(const float2 *)(sk + kStep + 2 * (c + e));
                         x = mul2(x, mul2(v2, make_float2(vinv, vinv)));
                         split2(x.x, x.y, hi16[e], lo16[e]);
                     } else {
@@ -552,21 +560,19 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                         hi16[e] = pack2<BF>(x.x, x.y);
                     }
                 }
-                // (over the logits: every thread of the tile has read its own, tile_sync above)
-                tc::st16(ts + half * (kCols / 2) + c, hi16);
-                if constexpr (I8) tc::st16(ts + kTile / 2 + half * (kCols / 2) + c, lo16);
+                tc::st16(ts + c, hi16);                    // over the logits
+                if constexpr (I8) tc::st16(ts + kStep / 2 + c, lo16);
+                if (c == kStep / 4 - 16 || c == kStep / 2 - 16) {
+                    tc::wait_st();
+                    tc::fence_before();
+                    mbar_arrive(&p_full[turn.buffer][c >= kStep / 4]);
+                }
             }
             part[0] = add2(part[0], part[1]);
             sum += part[0].x + part[0].y;
-            tc::wait_st();
-            tc::fence_before();
-            if (ok) mbar_arrive(&p_full[w]);
         }
-        if (mine > 0) ok = wait_phase(&o_full[w], 0, abort_flag) && ok;
+        if (mine > 0) ok = ok && wait_phase(&o_full[w], 0, abort_flag);
         tc::fence_after();
-        half_max[mine & 1][w][half][r] = sum;
-        tile_sync(w);
-        sum += half_max[mine & 1][w][half ^ 1][r];
         if (top == kNegInf && sum == sum) sum = 0.f;  // no visible key (its weights counted as 2^-126 each)
         if (ok && (alt || w < tiles)) {
             const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
@@ -576,7 +582,7 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
             const bool direct = p.prefix_slots + p.own_slots == 1;
             const long long part = (slot + (alt ? w : 0)) * nrows + row;
             const bool write = row_ok && (!direct || t < own_tokens(p, b));
-            if (row_ok && half == 0) {
+            if (row_ok) {
                 if (!direct) {
                     p.part_lse[part] = lse;
                 } else {
@@ -585,30 +591,29 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
                 }
             }
 #pragma unroll
-            for (int c = 0; c < HD / 2; c += 16) {
-                uint32_t o[16];
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
                 if (mine > 0) {
-                    tc::ld16(to + c, o);
+                    tc::ld32(to + c, o);
                     tc::wait_ld();
                 }
-                float v[16];
+                float v[32];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+                for (int e = 0; e < 32; ++e) v[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
                 if (!write) continue;
-                const int d = half * (HD / 2) + c;
                 if (!direct) {
-                    float4 *dst = (float4 *)(p.part_o + part * HD + d);
+                    float4 *dst = (float4 *)(p.part_o + part * HD + c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                 } else {
-                    char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + d) * (I8 ? 4 : 2);
+                    char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + c) * (I8 ? 4 : 2);
                     if constexpr (I8) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 8; ++e)
                             ((float4 *)dst)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                        for (int e = 0; e < 4; ++e)
                             ((uint4 *)dst)[e] = make_uint4(
                                 pack2<BF>(v[8 * e], v[8 * e + 1]), pack2<BF>(v[8 * e + 2], v[8 * e + 3]),
                                 pack2<BF>(v[8 * e + 4], v[8 * e + 5]), pack2<BF>(v[8 * e + 6], v[8 * e + 7]));
@@ -633,6 +638,11 @@ __global__ __launch_bounds__(TileGeom<TYPE, HD>::kThreads, 1) void prefix_tile_k
 // for the whole CTA; the rows come by TMA, their lse beside them; two TMEM
 // buffers a tile let the next product run during the exponentials, which bound
 // the kernel (one a logit, on the special-function unit or the FP32 pipe).
+
+// four warpgroups of keys, two a tile, and one of products and copies:
+// 4 * 128 * 104 + 128 * 64 = 640 * 96
+constexpr int kWeightThreads = 640, kWeightWarps = 16;
+constexpr int kWeightRegisters = 104, kWeightOthers = 64;
 
 template <int TYPE, int HD>
 struct WeightGeom {
@@ -677,7 +687,7 @@ __global__ __launch_bounds__(256) void split_queries_kernel(const PrefixAttn p) 
 }
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const PrefixAttn p, int tile_rows,
+__global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const PrefixAttn p, int tile_rows,
                                                                       const __grid_constant__ CUtensorMap mq) {
     using G = WeightGeom<TYPE, HD>;
     constexpr bool I8 = G::I8, BF = TYPE == kCacheBF16;
@@ -713,11 +723,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
         abort_at = 0;
         fence_barrier_init();
     }
-    if (warp == kProductWarp) tc::alloc(&tmem_at, 512);
+    if (warp == kWeightWarps) tc::alloc(&tmem_at, 512);
     pdl_enter();
     if (n > 0) {
         // two tiles of keys (zeros where there are none)
-        constexpr int kChunks = HD * (I8 ? 1 : 2) / 16, kPer = kTileThreads / kChunks;
+        constexpr int kChunks = HD * (I8 ? 1 : 2) / 16, kPer = kWeightThreads / kChunks;
         const long long crow = p.cache_row ? p.cache_row[b] : b;
         const char *k = (const char *)p.k + (crow * p.ks[0] + g * p.ks[1]) * (I8 ? 1 : 2);
         const long long step = p.ks[2] * (I8 ? 1 : 2);
@@ -738,21 +748,21 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
                 if constexpr (I8) {
                     uint4 a, d;
                     i8x16_to_f16(x[e], a, d);
-                    *(uint4 *)(t + piece_at(r % kTile, 2 * c)) = a;
-                    *(uint4 *)(t + piece_at(r % kTile, 2 * c + 1)) = d;
+                    *(uint4 *)(t + piece_at<kTile>(r % kTile, 2 * c)) = a;
+                    *(uint4 *)(t + piece_at<kTile>(r % kTile, 2 * c + 1)) = d;
                 } else {
-                    *(uint4 *)(t + piece_at(r % kTile, c)) = x[e];
+                    *(uint4 *)(t + piece_at<kTile>(r % kTile, c)) = x[e];
                 }
             }
         }
         // rows behind a short tile stay what they are here: zeros, and weightless
-        for (int i = threadIdx.x; i < kStages * kTile; i += kTileThreads) {
+        for (int i = threadIdx.x; i < kStages * kTile; i += kWeightThreads) {
             lse[i / kTile][0][i % kTile] = kNegInf;
             if constexpr (I8) lse[i / kTile][1][i % kTile] = 0.f;
         }
         if (tile_rows < kTile) {
             char *q = smem + G::kRing;
-            for (int i = threadIdx.x; i < kStages * G::kStageBytes / 16; i += kTileThreads)
+            for (int i = threadIdx.x; i < kStages * G::kStageBytes / 16; i += kWeightThreads)
                 *(uint4 *)(q + i * 16) = make_uint4(0, 0, 0, 0);
         }
     }
@@ -762,9 +772,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
     tc::fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp >= kMathWarps) {
-        fewer_registers();
-        if (warp == kCopyWarp) {
+    if (warp >= kWeightWarps) {
+        fewer_registers<kWeightOthers>();
+        if (warp == kWeightWarps + 1) {
             // ---- query rows
             if (lane == 0) {
                 int issued = 0;
@@ -788,7 +798,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
                     mbar_wait(&full[i % kStages], (uint32_t)(i / kStages) & 1);
             }
             __syncwarp();
-        } else if (warp == kConvertWarp) {
+        } else if (warp == kWeightWarps + 2) {
             // ---- their lse (and INT8 factors)
             const float *src = p.neg_lse + (long long)unit * TR + m0, *fac = nullptr;
             if constexpr (I8) fac = p.q16_scale + (long long)unit * TR + m0;
@@ -808,7 +818,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
-        } else if (warp == kProductWarp) {
+        } else if (warp == kWeightWarps) {
             // ---- products
             constexpr uint32_t ids = idesc(BF, false, kTile);
             const uint32_t k0 = smem_addr(smem), q0 = smem_addr(smem) + G::kRing;
@@ -840,7 +850,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
         }
         __syncwarp();
     } else {
-        more_registers();
+        more_registers<kWeightRegisters>();
         // ---- thread = key and half of the rows
         constexpr int kCols = kTile / 2;
         const int w = warp >> 3, half = (warp >> 2) & 1, j = key0 + w * kTile + (threadIdx.x & (kTile - 1));
@@ -928,7 +938,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void weight_tile_kernel(const Pref
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == kProductWarp) tc::dealloc(tmem, 512);
+    if (warp == kWeightWarps) tc::dealloc(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_tile_fault, 1);
 }
 
@@ -947,7 +957,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-// Map of a cache [seqs][heads][keys][hd] in tiles of kTile keys: 128-byte
+// Map of a cache [seqs][heads][keys][hd] in steps of kStep keys: 128-byte
 // swizzled chunks of 64 16-bit values, or whole INT8 rows.  Axes of stride 0
 // (or one element) get extent 1 and their flag 0: the kernel's coordinate stays 0.
 bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long keys, long long heads, long long seqs,
@@ -968,7 +978,7 @@ bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long k
     const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)keys, (cuuint64_t)heads, (cuuint64_t)seqs};
     const cuuint64_t strides[3] = {(cuuint64_t)ks, (cuuint64_t)(*head_flag ? head_stride * size : row),
                                    (cuuint64_t)(*seq_flag ? seq_stride * size : row)};
-    const cuuint32_t box[4] = {(cuuint32_t)(i8 ? hd : 64), (cuuint32_t)kTile, 1, 1};
+    const cuuint32_t box[4] = {(cuuint32_t)(i8 ? hd : 64), (cuuint32_t)kStep, 1, 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r =
         fn(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims,
@@ -1048,7 +1058,7 @@ bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const P
             NB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
             if (dev >= 0 && dev < 64) configured[dev] = true;
         }
-        kernel<<<blocks, G::kThreads, G::kSmem, st>>>(p, grid, mk, mv, mpk, mpv);
+        kernel<<<blocks, kTileThreads, G::kSmem, st>>>(p, grid, mk, mv, mpk, mpv);
         NB_CUDA_TRY(cudaGetLastError());
         return true;
     };
@@ -1109,7 +1119,7 @@ bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st) {
         }
         const int blocks = p.batch * p.kvheads * ceil_div(p.capacity, 2 * kTile);
         if (blocks == 0) return true;
-        NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kTileThreads), (size_t)G::kSmem, st, p, tile_rows, mq));
+        NB_CUDA_TRY(launch_pdl(kernel, dim3(blocks), dim3(kWeightThreads), (size_t)G::kSmem, st, p, tile_rows, mq));
         return true;
     };
     return by_geometry(p, run);

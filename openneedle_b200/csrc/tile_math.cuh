@@ -122,7 +122,7 @@ __device__ __forceinline__ void i8x16_to_f16(uint4 w, uint4 &a, uint4 &b) {
                    i8x2_to_f16<0x4342>(u[3]));
 }
 
-constexpr int kTile = 128;   // rows of a tile, keys of a step
+constexpr int kTile = 128;   // rows of a tile
 
 // 128-byte swizzled operands: rows of 128 bytes in atoms of 8 rows, a 16-byte
 // piece c of row r at piece c ^ (r % 8).  K-major (Q, K): SBO = 1024 between
@@ -133,13 +133,15 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t a) {
     return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
+template <int ROWS>
 __device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(kTile * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(ROWS * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
 }
-// Byte of 16-byte piece c of row r in a tile of kTile rows of HD 16-bit values.
+// Byte of 16-byte piece c of row r in a tile of ROWS rows of 16-bit values.
+template <int ROWS>
 __device__ __forceinline__ int piece_at(int r, int c) {
-    return (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    return (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 // kind::f16, M = 128, f32 accumulator: types at bits 7 and 10 (0 f16, 1 bf16), B
 // MN-major at bit 16, N / 8 at bit 17, M / 16 at bit 24.
@@ -178,7 +180,7 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
 
 // Bounded wait; on its end the CTA's warps give up (and the kernel raises its
 // fault flag).
-constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr uint32_t kWaitLimit = 1u << 16;
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t a = smem_addr(bar);
     uint32_t done;
@@ -207,14 +209,16 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volat
     return false;
 }
 
-// A CTA of the tile kernels: four warpgroups for the exponentials (two a tile of
-// 128 rows: thread = row and half of the columns) and one for products, copies and
-// conversions.  Registers move between them: of the 96 a thread at the launch,
-// 104 to the first four and 64 to the last, 61440 in all as before.
-constexpr int kTileThreads = 640;
-constexpr int kMathWarps = 16, kProductWarp = 16, kCopyWarp = 17, kConvertWarp = 18;
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+// Registers move from the warpgroup of products, copies and conversions to the
+// others; the sum over the CTA stays what it was at the launch.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 // The 256 threads of one tile.
 __device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); }
 
