@@ -9,7 +9,6 @@ CUDA tensors and do not synchronise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as ct
 import functools
 import struct
@@ -224,15 +223,13 @@ def _bind_operators():
     return lib, torch, types, getattr(torch._C, "_cuda_getCurrentRawStream", current_stream)
 
 
-_HERE = contextlib.nullcontext()
-
-
 def _on_stream(torch, device, stream):
-    """The context in which torch allocates and launches for `device` and `stream` (None: the current one)."""
+    """The context in which torch allocates and launches for `device` and `stream` (None: the current one); None
+    where that is the present one."""
     if device.type != "cuda":
         raise ValueError("the operators run on CUDA tensors")
     if stream is None:
-        return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
         handle = _stream_ptr(stream)
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
@@ -297,7 +294,7 @@ def _strides(axes, *tensors):
 
 
 def _layout(x):
-    return None if x is None else (x.shape, x.stride(), x.dtype, x.device)
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
 
 
 def _pointer(x):
@@ -401,20 +398,24 @@ def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales
             outs.append((weights_out, "weights_out"))
         _apart(outs, (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales,
                       prefix_v_scales, None if same else weights))
-    with _on_stream(torch, device, stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        lse = torch.empty(rows, dtype=torch.float32, device=device) if return_lse else None
-        if weights is not None and weights_out is None:
-            weights_out = torch.empty(weights.shape, dtype=torch.float32, device=device)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        args = sizes + _ATTENTION_POINTERS.pack(
-            q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales),
-            _pointer(prefix_k), _pointer(prefix_v), _pointer(prefix_k_scales), _pointer(prefix_v_scales),
-            lengths.data_ptr(), _pointer(tokens), 0, _pointer(lse), weights.data_ptr() if weigh else 0,
-            weights_out.data_ptr() if weigh else 0)
-        if lib.needle2_prefix_attention_device(args, _pointer(workspace), size, raw_stream(device.index)):
-            _check(-1, "prefix_attention")
+    context = _on_stream(torch, device, stream)
+    if context is not None:
+        with context:
+            return _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales,
+                           prefix_k_scales, prefix_v_scales, tokens, window, scale, out, return_lse, None)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(rows, dtype=torch.float32, device=device) if return_lse else None
+    if weights is not None and weights_out is None:
+        weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    args = sizes + _ATTENTION_POINTERS.pack(
+        q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales),
+        _pointer(prefix_k), _pointer(prefix_v), _pointer(prefix_k_scales), _pointer(prefix_v_scales),
+        lengths.data_ptr(), _pointer(tokens), 0, _pointer(lse), weights.data_ptr() if weigh else 0,
+        weights_out.data_ptr() if weigh else 0)
+    if lib.needle2_prefix_attention_device(args, _pointer(workspace), size, raw_stream(device.index)):
+        _check(-1, "prefix_attention")
     if return_lse and q.dim() == 3:
         lse = lse.squeeze(1)
     return out, lse, weights_out
@@ -485,28 +486,32 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     sizes, shape = plan
     _no_gradients(torch, k, v, weights)
     device = k.device
-    with _on_stream(torch, device, stream):
-        if in_place:
-            _apart([(x, "the cache") for x in (k, v, weights, k_scales, v_scales) if x is not None], (lengths,))
-            out = Evicted(k, v, weights, torch.empty(shape[:1], dtype=torch.int32, device=device),
-                          torch.empty(shape, dtype=torch.int32, device=device), k_scales, v_scales)
-        elif out is None:
-            f32 = {"dtype": torch.float32, "device": device}
-            out = Evicted(torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device),
-                          torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device), torch.empty(shape, **f32),
-                          torch.empty(shape[:1], dtype=torch.int32, device=device),
-                          torch.empty(shape, dtype=torch.int32, device=device),
-                          None if k_scales is None else torch.zeros(shape, **f32),
-                          None if v_scales is None else torch.zeros(shape, **f32))
-        else:
-            out = Evicted(*out)
-            _apart([(x, "out") for x in out if x is not None], (k, v, weights, lengths, k_scales, v_scales))
-        args = sizes + _EVICT_POINTERS.pack(
-            k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales), weights.data_ptr(), lengths.data_ptr(),
-            out.k.data_ptr(), out.v.data_ptr(), _pointer(out.k_scales), _pointer(out.v_scales), out.weights.data_ptr(),
-            out.indices.data_ptr(), out.lengths.data_ptr())
-        if lib.needle2_evict_device(args, raw_stream(device.index)):
-            _check(-1, "evict")
+    context = _on_stream(torch, device, stream)
+    if context is not None:
+        with context:
+            return evict(k, v, weights, lengths, keep, first=first, recent=recent, k_scales=k_scales, v_scales=v_scales,
+                         out=out, in_place=in_place)
+    if in_place:
+        _apart([(x, "the cache") for x in (k, v, weights, k_scales, v_scales) if x is not None], (lengths,))
+        out = Evicted(k, v, weights, torch.empty(shape[:1], dtype=torch.int32, device=device),
+                      torch.empty(shape, dtype=torch.int32, device=device), k_scales, v_scales)
+    elif out is None:
+        f32 = {"dtype": torch.float32, "device": device}
+        out = Evicted(torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device),
+                      torch.zeros((*shape, k.shape[3]), dtype=k.dtype, device=device), torch.empty(shape, **f32),
+                      torch.empty(shape[:1], dtype=torch.int32, device=device),
+                      torch.empty(shape, dtype=torch.int32, device=device),
+                      None if k_scales is None else torch.zeros(shape, **f32),
+                      None if v_scales is None else torch.zeros(shape, **f32))
+    else:
+        out = Evicted(*out)
+        _apart([(x, "out") for x in out if x is not None], (k, v, weights, lengths, k_scales, v_scales))
+    args = sizes + _EVICT_POINTERS.pack(
+        k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales), weights.data_ptr(), lengths.data_ptr(),
+        out.k.data_ptr(), out.v.data_ptr(), _pointer(out.k_scales), _pointer(out.v_scales), out.weights.data_ptr(),
+        out.indices.data_ptr(), out.lengths.data_ptr())
+    if lib.needle2_evict_device(args, raw_stream(device.index)):
+        _check(-1, "evict")
     return out
 
 

@@ -48,9 +48,11 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
     return true;
 }
 
+constexpr int kJointKeys = 512;
+
 struct Plan {
     PrefixSplit prefix, own;
-    bool logits, neg_lse, weight_tiles;
+    bool joint, logits, neg_lse, weight_tiles;
     long long part_o, part_lse, neg_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
 
@@ -81,13 +83,19 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         } else {
             const long long units = groups * ((group_rows + tile - 1) / tile);
             const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
-            s.ranges = (int)std::max(1LL, std::min({want, (keys + 127) / 128, 64LL}));
+            s.ranges = (int)std::max(1LL, std::min({want, (keys + 255) / 256, 64LL}));
         }
         return s;
     };
     const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
     if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span);
     if (a.prefix) p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix);
+    // few rows and keys: one kernel whose units take both key sets one after the other
+    p.joint = a.prefix && a.capacity && !p.own.tiles && !p.prefix.tiles && a.prefix + (long long)span <= kJointKeys;
+    if (p.joint) {
+        p.prefix.ranges = 0;
+        p.own.ranges = 1;
+    }
     if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros
         p.own = PrefixSplit{};
         p.own.ranges = 1;
@@ -185,7 +193,7 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
         if (tiles &&
             !launch_prefix_tiles(p, plan.prefix, plan.own, a.cache_rows ? 1LL << 30 : a.batch, stream, st))
             return false;
-        if (stream && !launch_prefix_stream(p, stream_prefix, stream_own, tiles, st)) return false;
+        if (stream && !launch_prefix_stream(p, stream_prefix, stream_own, plan.joint, tiles, st)) return false;
     }
     if (!launch_prefix_finish(p, st)) return false;
     if (!a.weights || plan.logits) return true;

@@ -95,6 +95,7 @@ struct KeySet {
 struct StreamGrid {
     int own_units, own_tiles, prefix_units, prefix_tiles;
     int own_slots, prefix_slots;
+    int joint;                                    // own units take the prefix too
 };
 
 // One lane's part of the copies of a warp's blocks: 16-byte pieces of K and V
@@ -108,7 +109,7 @@ struct BlockCopy {
     const float *ks, *vs;
     long long k_per, v_per, k_next, v_next, ks_next, vs_next;
 
-    __device__ __forceinline__ BlockCopy(const KeySet &s, int j0, int keys, int lane) {
+    __device__ __forceinline__ void set(const KeySet &s, int j0, int keys, int lane) {
         const long long r = j0 + lane / kChunks, piece = lane % kChunks * 16;
         k = s.k + r * s.k_step + piece;
         v = s.v + r * s.v_step + piece;
@@ -156,6 +157,23 @@ struct BlockCopy {
         }
     }
 };
+
+template <int TYPE, int HD>
+__device__ __forceinline__ KeySet prefix_set(const PrefixAttn &p, int g) {
+    constexpr int kSize = StreamGeom<TYPE, HD>::kSize;
+    KeySet s;
+    s.k = (const char *)p.pk + g * p.pks[0] * kSize;
+    s.v = (const char *)p.pv + g * p.pvs[0] * kSize;
+    s.k_step = p.pks[1] * kSize;
+    s.v_step = p.pvs[1] * kSize;
+    if constexpr (TYPE == kCacheI8) {
+        s.ks = p.pkscale + g * p.pkss[0];
+        s.vs = p.pvscale + g * p.pvss[0];
+        s.ks_step = p.pkss[1];
+        s.vs_step = p.pvss[1];
+    }
+    return s;
+}
 
 // W warps share a unit's keys: four where the ranges are long, one (and four
 // units a CTA, no merge between warps) where they are short.
@@ -215,16 +233,7 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         g = unit / grid.prefix_tiles;
         m0 = tile * G::kRows;
         rows = min(G::kRows, p.batch * TR - m0);
-        s.k = (const char *)p.pk + g * p.pks[0] * G::kSize;
-        s.v = (const char *)p.pv + g * p.pvs[0] * G::kSize;
-        s.k_step = p.pks[1] * G::kSize;
-        s.v_step = p.pvs[1] * G::kSize;
-        if constexpr (I8) {
-            s.ks = p.pkscale + g * p.pkss[0];
-            s.vs = p.pvscale + g * p.pvss[0];
-            s.ks_step = p.pkss[1];
-            s.vs_step = p.pvss[1];
-        }
+        s = prefix_set<TYPE, HD>(p, g);
         const int each = (ceil_div(p.prefix, grid.prefix_slots) + G::kKeys - 1) / G::kKeys * G::kKeys;
         lo = min(p.prefix, slot * each);
         hi = min(p.prefix, lo + each);
@@ -232,16 +241,21 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
     if (rows <= 0) return;
 
     // first copies, then the queries
-    const int blocks = ceil_div(max(0, hi - lo), G::kKeys);
-    const int mine = blocks > part ? (blocks - part + W - 1) / W : 0;
-    BlockCopy<TYPE, HD> copy(s, lo + part * G::kKeys, W * G::kKeys, lane);
-    int left = hi - lo - part * G::kKeys;            // keys from the next block to be copied on
+    int mine, left;                                  // this warp's blocks; keys from the next one to be copied on
+    BlockCopy<TYPE, HD> copy;
+    auto begin = [&] {
+        const int blocks = ceil_div(max(0, hi - lo), G::kKeys);
+        mine = blocks > part ? (blocks - part + W - 1) / W : 0;
+        left = hi - lo - part * G::kKeys;
+        copy.set(s, lo + part * G::kKeys, W * G::kKeys, lane);
 #pragma unroll
-    for (int i = 0; i < G::kStages - 1; ++i) {
-        if (i < mine) copy.block(ring + i * G::kStage, left, lane);
-        left -= W * G::kKeys;
-        cp_async_commit();
-    }
+        for (int i = 0; i < G::kStages - 1; ++i) {
+            if (i < mine) copy.block(ring + i * G::kStage, left, lane);
+            left -= W * G::kKeys;
+            cp_async_commit();
+        }
+    };
+    begin();
 
     // this lane's rows (g8 and, 16-bit, g8 + 8), their visible own keys [first, last]
     constexpr int kMine = I8 ? 1 : 2;
@@ -260,7 +274,7 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         }
         last[e] = min(last[e], hi - 1);
     }
-    const int all_from = max(first[0], first[kMine - 1]), all_to = min(last[0], last[kMine - 1]);
+    int all_from = max(first[0], first[kMine - 1]), all_to = min(last[0], last[kMine - 1]);
     uint32_t qa[KS][4];
     float qscale = p.scale2;
     if constexpr (I8) {
@@ -305,7 +319,23 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
     if (p.logits && seq >= 0)
         logits = p.logits + ((long long)(seq * p.kvheads + g) * TR + (m0 - seq * TR)) * p.capacity;
 
-    for (int i = 0; i < mine; ++i) {
+    for (int i = 0;; ++i) {
+        if (i == mine) {
+            if (seq < 0 || !grid.joint || s.k == (const char *)p.pk + g * p.pks[0] * G::kSize) break;
+            // then the prefix, on the same state; every query sees all of it
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            s = prefix_set<TYPE, HD>(p, g);
+            lo = all_from = 0;
+            hi = p.prefix;
+            all_to = hi - 1;
+#pragma unroll
+            for (int e = 0; e < kMine; ++e) first[e] = 0, last[e] = hi - 1;
+            logits = nullptr;
+            begin();
+            i = -1;
+            continue;
+        }
         cp_async_wait<G::kStages - 2>();
         __syncwarp();
         {   // the stage that was read last takes the copy two blocks ahead
@@ -563,7 +593,7 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
 }
 
 template <int TYPE, int HD, int W>
-__global__ __launch_bounds__(kWarps * 32) void prefix_stream_kernel(
+__global__ __launch_bounds__(kWarps * 32, HD == 64 ? 4 : 3) void prefix_stream_kernel(
     const __grid_constant__ PrefixAttn p, const __grid_constant__ StreamGrid grid) {
     stream_unit<TYPE, HD, W>(p, grid);
     pdl_enter();   // (at the end: what follows this kernel follows the tile kernel beside it too)
@@ -581,18 +611,34 @@ __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, in
     const long long bt = row / p.heads;
     const int t = (int)(bt % p.tokens), b = (int)(bt / p.tokens);
     if (t >= own_tokens(p, b)) return;
+    // four partial results in flight at a time
     float top = kNegInf;
-    for (int i = 0; i < slots; ++i) top = fmaxf(top, p.part_lse[i * nrows + row]);
+    for (int i = 0; i < slots; i += 4) {
+        float l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[e] = i + e < slots ? p.part_lse[(i + e) * nrows + row] : kNegInf;
+        top = fmaxf(max3(top, l[0], l[1]), fmaxf(l[2], l[3]));
+    }
     const float t0 = top == kNegInf ? 0.f : top;
     float total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < slots; ++i) {
-        const float l = p.part_lse[i * nrows + row];
-        if (l == kNegInf) continue;
-        const float f = ex2(l - t0);
-        total += f;
-        const float4 v = *(const float4 *)(p.part_o + (i * nrows + row) * HD + part);
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+    for (int i = 0; i < slots; i += 4) {
+        float l[4];
+        float4 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            l[e] = i + e < slots ? p.part_lse[(i + e) * nrows + row] : kNegInf;
+            v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (l[e] != kNegInf) v[e] = *(const float4 *)(p.part_o + ((i + e) * nrows + row) * HD + part);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float f = ex2(l[e] - t0);
+            total += f;
+            acc.x += f * v[e].x; acc.y += f * v[e].y; acc.z += f * v[e].z; acc.w += f * v[e].w;
+        }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
@@ -802,7 +848,7 @@ bool by_geometry(const PrefixAttn &p, F f) {
 
 }  // namespace
 
-bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after_tiles, cudaStream_t st) {
+bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint, bool after_tiles, cudaStream_t st) {
     return by_geometry(p, [&](auto type, auto hd) -> bool {
         using G = StreamGeom<type(), hd()>;
         StreamGrid grid{};
@@ -811,6 +857,7 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after
         grid.prefix_slots = std::max(1, p.prefix_slots);
         grid.own_tiles = ceil_div(rows, G::kRows);
         grid.prefix_tiles = ceil_div(p.batch * rows, G::kRows);
+        grid.joint = joint;
         grid.own_units = own ? p.batch * p.kvheads * grid.own_tiles * grid.own_slots : 0;
         grid.prefix_units = prefix ? p.kvheads * grid.prefix_tiles * grid.prefix_slots : 0;
         const int units = grid.own_units + grid.prefix_units;
@@ -834,7 +881,7 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool after
             return true;
         };
         const int span = p.window ? std::min<long long>(p.capacity, (long long)p.window + p.tokens) : p.capacity;
-        const int longest = std::max(own ? ceil_div(span, grid.own_slots) : 0,
+        const int longest = std::max(own ? ceil_div(span, grid.own_slots) + (joint ? p.prefix : 0) : 0,
                                      prefix ? ceil_div(p.prefix, grid.prefix_slots) : 0);
         return longest <= kShortRange ? launch(std::integral_constant<int, 1>())
                                       : launch(std::integral_constant<int, kWarps>());

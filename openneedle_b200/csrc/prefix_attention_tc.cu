@@ -34,8 +34,6 @@ using namespace tile;
 
 __device__ int g_tile_fault = 0;                 // a bounded wait ran out
 
-constexpr int kFmaOf8 = 2;                       // of 8 powers of two, those on the FP32 pipe
-constexpr int kWeightFmaOf8 = 3;                 // the same of the key weights
 constexpr float kGrow = 8.f;                     // log2 growth of a maximum that is left to the weights
 
 constexpr int kStep = 128;                       // keys of a step
@@ -543,12 +541,8 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     float2 x = fma2(z[c + e], zs2, base2);
-                    if ((e & 7) < kFmaOf8) {
-                        x = ex2_fma2(x);
-                    } else {
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
-                    }
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
                     part[e & 1] = add2(part[e & 1], x);
                     if constexpr (I8) {
                         const float2 v2 = *(const float2 *)(sk + kStep + 2 * (c + e));
@@ -573,7 +567,6 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
         }
         if (mine > 0) ok = ok && wait_phase(&o_full[w], 0, abort_flag);
         tc::fence_after();
-        if (top == kNegInf && sum == sum) sum = 0.f;  // no visible key (its weights counted as 2^-126 each)
         if (ok && (alt || w < tiles)) {
             const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
             const float lse = sum == 0.f ? kNegInf : (top == kNegInf ? 0.f : top) + log2f(sum);
@@ -637,7 +630,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
 // a fixed order.  K stays in shared memory
 // for the whole CTA; the rows come by TMA, their lse beside them; two TMEM
 // buffers a tile let the next product run during the exponentials, which bound
-// the kernel (one a logit, on the special-function unit or the FP32 pipe).
+// the kernel (one a logit).  Powers of two by a polynomial on the FP32 pipe, for a
+// part of them, did not pay: the more the slower (180 us for none or one of eight,
+// 217 for five of eight, two prompts of 4096 tokens).
 
 // four warpgroups of keys, two a tile, and one of products and copies:
 // 4 * 128 * 104 + 128 * 64 = 640 * 96
@@ -902,13 +897,8 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
                         a = fma2(a, k2, make_float2(l4.x, l4.y));
                         d = fma2(d, k2, make_float2(l4.z, l4.w));
                     }
-                    if ((c / 4) % 8 < kWeightFmaOf8) {
-                        a = ex2_fma2(a);
-                        d = ex2_fma2(d);
-                    } else {
-                        a = make_float2(ex2(a.x), ex2(a.y));
-                        d = make_float2(ex2(d.x), ex2(d.y));
-                    }
+                    a = make_float2(ex2(a.x), ex2(a.y));
+                    d = make_float2(ex2(d.x), ex2(d.y));
                     part[(c / 4) & 1] = add2(part[(c / 4) & 1], a);
                     part[2 + ((c / 4) & 1)] = add2(part[2 + ((c / 4) & 1)], d);
                 }

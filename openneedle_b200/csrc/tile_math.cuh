@@ -1,6 +1,5 @@
-// Arithmetic and tensor-core helpers of the attention tiles: paired FP32
-// instructions, powers of two, FP16 splits, swizzled operand descriptors,
-// bounded waits.
+// Arithmetic and tensor-core helpers of the attention kernels: paired FP32
+// instructions, FP16 splits, swizzled operand descriptors, bounded waits.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -52,28 +51,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
     return pair2(r);
-}
-
-// 2^x of two values on the FP32 pipe, which relieves the special-function unit:
-// x = n + f with n the nearest integer (the sum with 1.5 * 2^23 leaves it in the
-// low bits), 2^f by a polynomial of degree 5 whose relative error on
-// [-1/2, 1/2] is least (Remez exchange: 7.5e-8, 2.1e-7 with FP32 roundings), n
-// added to the exponent.  x below -126 counts as -126.
-__device__ __forceinline__ float2 ex2_fma2(float2 x) {
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const float2 big = make_float2(12582912.f, 12582912.f);
-    const float2 r = add2(x, big);
-    const float2 f = add2(x, mul2(add2(r, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f)));
-    float2 y = make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
-    y = fma2(y, f, make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
-    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
-    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
-    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
-    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
-    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
-    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
-    return y;
 }
 
 template <bool BF>

@@ -100,14 +100,14 @@ def test_evict_refuses(more, message):
 
 def pack(**change):
     """A valid call of two sequences on an INT8 cache; addresses that nothing reads."""
-    a = dict(batch=2, tokens=1, heads=8, kvheads=4, head_dim=64, prefix=16, capacity=32, window=0, cache_type=0,
+    a = dict(batch=2, tokens=1, heads=8, kvheads=4, head_dim=64, prefix=600, capacity=32, window=0, cache_type=0,
              scale=0.125, q=4096, out=8192, k=4096, v=4096, ks=4096, vs=4096, pk=4096, pv=4096, pks=4096, pvs=4096,
              lengths=4096, counts=0, rows=0, lse=0, weights=0, weights_out=0, kstride=64)
     a.update(change)
     three, flat, flat2 = (8192, 2048, a["kstride"]), (128, 32, 1), (16, 1)
     return attention._ATTENTION_SIZES.pack(
         a["batch"], a["tokens"], a["heads"], a["kvheads"], a["head_dim"], a["prefix"], a["capacity"], a["window"],
-        a["cache_type"], a["scale"], 512, 512, 64, 512, 512, 64, *three, 8192, 2048, 64, *flat, *flat, 1024, 64, 1024,
+        a["cache_type"], a["scale"], 512, 512, 64, 512, 512, 64, *three, 8192, 2048, 64, *flat, *flat, 38400, 64, 38400,
         64, *flat2, *flat2, *flat, *flat) + attention._ATTENTION_POINTERS.pack(
         a["q"], a["out"], a["k"], a["v"], a["ks"], a["vs"], a["pk"], a["pv"], a["pks"], a["pvs"], a["lengths"],
         a["counts"], a["rows"], a["lse"], a["weights"], a["weights_out"])
