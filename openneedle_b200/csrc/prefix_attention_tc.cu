@@ -281,8 +281,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
 #pragma unroll
                         for (int e = 0; e < kStep / 32; ++e) {
                             const int c = half * (kStep / 32) + e;
-                            mma_ts(tmem + w * HD, pk + x * (kStep / 2) + c * 8, desc_mn<kStep>(v + c * 2048), ido,
-                                   !first || x + e > 0);
+                            // 32 keys take 32 columns: 16 of their weights (hi), 16 of lo
+                            mma_ts(tmem + w * HD, pk + 32 * (c >> 1) + 8 * (c & 1) + 16 * x,
+                                   desc_mn<kStep>(v + c * 2048), ido, !first || x + e > 0);
                         }
                     if (half) {
                         tc::commit(&o_done[w]);
@@ -451,6 +452,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             wait_phase(&q_full, 0, abort_flag);
             zs = qscale[alt ? r : w * kTile + r];
         }
+        // columns of logits in registers: all of a step; INT8, whose weights take three
+        // times the instructions, reads them twice (for the maximum and for the weights),
+        // 32 at a time in loops: its code does not fit the instruction cache otherwise
+        // (20 against 26 us for a prefix of 384 keys)
+        constexpr int kRead = I8 ? 32 : kStep;
         float top = kNegInf, sum = 0.f, vnorm = 0.f;
         bool ok = true;
         Turn turn;
@@ -465,38 +471,43 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             if (!ok) break;
             tc::fence_after();
             const uint32_t ts = s0 + turn.buffer * kStep;
-            uint32_t raw[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, raw[c]);
-            tc::wait_ld();
-            float2 z[kStep / 2];
             const float *sk = scales + (j % G::kScaleRing) * 2 * kStep;
+            // kRead logits of the row from column c on, INT8: times K's scales; -inf where not seen
+            const bool edge = j0 < first || j0 + kStep - 1 > last;
+            float2 z[kRead / 2];
+            auto read = [&](int c) {
+                uint32_t raw[kRead / 32][32];
 #pragma unroll
-            for (int c = 0; c < kStep / 2; ++c)
-                z[c] = make_float2(__uint_as_float(raw[c / 16][2 * (c % 16)]),
-                                   __uint_as_float(raw[c / 16][2 * (c % 16) + 1]));
-            if constexpr (I8) {
+                for (int x = 0; x < kRead / 32; ++x) tc::ld32(ts + c + 32 * x, raw[x]);
+                tc::wait_ld();
 #pragma unroll
-                for (int c = 0; c < kStep / 2; c += 2) {
-                    const float4 s4 = *(const float4 *)(sk + 2 * c);
-                    z[c] = mul2(z[c], make_float2(s4.x, s4.y));
-                    z[c + 1] = mul2(z[c + 1], make_float2(s4.z, s4.w));
+                for (int e = 0; e < kRead / 2; ++e)
+                    z[e] = make_float2(__uint_as_float(raw[e / 16][2 * (e % 16)]),
+                                       __uint_as_float(raw[e / 16][2 * (e % 16) + 1]));
+                if constexpr (I8) {
+#pragma unroll
+                    for (int e = 0; e < kRead / 2; e += 2) {
+                        const float4 s4 = *(const float4 *)(sk + c + 2 * e);
+                        z[e] = mul2(z[e], make_float2(s4.x, s4.y));
+                        z[e + 1] = mul2(z[e + 1], make_float2(s4.z, s4.w));
+                    }
                 }
-            }
-            if (j0 < first || j0 + kStep - 1 > last) {
-                const int x0 = first - j0, x1 = last - j0;
+                if (edge) {
+                    const int x0 = first - j0 - c, x1 = last - j0 - c;
 #pragma unroll
-                for (int c = 0; c < kStep / 2; ++c) {
-                    if (2 * c < x0 || 2 * c > x1) z[c].x = kNegInf;
-                    if (2 * c + 1 < x0 || 2 * c + 1 > x1) z[c].y = kNegInf;
+                    for (int e = 0; e < kRead / 2; ++e) {
+                        if (2 * e < x0 || 2 * e > x1) z[e].x = kNegInf;
+                        if (2 * e + 1 < x0 || 2 * e + 1 > x1) z[e].y = kNegInf;
+                    }
                 }
+            };
+            float best[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll 1
+            for (int c = 0; c < kStep; c += kRead) {
+                read(c);
+#pragma unroll
+                for (int e = 0; e < kRead / 2; ++e) best[e & 3] = max3(best[e & 3], z[e].x, z[e].y);
             }
-            float best[4] = {fmaxf(z[0].x, z[0].y), fmaxf(z[1].x, z[1].y), fmaxf(z[2].x, z[2].y),
-                             fmaxf(z[3].x, z[3].y)};
-#pragma unroll
-            for (int c = 4; c < kStep / 2; c += 4)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) best[e] = max3(best[e], z[c + e].x, z[c + e].y);
             const float now = max3(fmaxf(best[0], best[1]), best[2], best[3]) * zs;
             float keep = 1.f;
             if (now > top + kGrow || (top == kNegInf && now > kNegInf)) {
@@ -533,33 +544,38 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                 }
             }
             const float base = top == kNegInf ? 0.f : -top;
-            const float2 zs2 = make_float2(zs, zs), base2 = make_float2(base, base);
+            const float2 zs2 = make_float2(zs, zs), base2 = make_float2(base, base), vinv2 = make_float2(vinv, vinv);
             float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+            for (int c0 = 0; c0 < kStep; c0 += kRead) {
+                if (kRead < kStep) read(c0);
 #pragma unroll
-            for (int c = 0; c < kStep / 2; c += 16) {      // 16 columns of TMEM a store takes
-                uint32_t hi16[16], lo16[I8 ? 16 : 1];
+                for (int x = 0; x < kRead; x += 32) {
+                    const int c = c0 + x;
+                    uint32_t hi16[16], lo16[I8 ? 16 : 1];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float2 x = fma2(z[c + e], zs2, base2);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    part[e & 1] = add2(part[e & 1], x);
-                    if constexpr (I8) {
-                        const float2 v2 = *(const float2 *)(sk + kStep + 2 * (c + e));
-                        x = mul2(x, mul2(v2, make_float2(vinv, vinv)));
-                        split2(x.x, x.y, hi16[e], lo16[e]);
-                    } else {
-                        // the softmax weights are rounded to the cache's type for the
-                        // product; their sum keeps 32 bits
-                        hi16[e] = pack2<BF>(x.x, x.y);
+                    for (int e = 0; e < 16; ++e) {
+                        float2 y = fma2(z[x / 2 + e], zs2, base2);
+                        y.x = ex2(y.x);
+                        y.y = ex2(y.y);
+                        part[e & 1] = add2(part[e & 1], y);
+                        if constexpr (I8) {
+                            const float2 v2 = *(const float2 *)(sk + kStep + c + 2 * e);
+                            y = mul2(y, mul2(v2, vinv2));
+                            split2(y.x, y.y, hi16[e], lo16[e]);
+                        } else {
+                            // the softmax weights are rounded to the cache's type for the
+                            // product; their sum keeps 32 bits
+                            hi16[e] = pack2<BF>(y.x, y.y);
+                        }
                     }
-                }
-                tc::st16(ts + c, hi16);                    // over the logits
-                if constexpr (I8) tc::st16(ts + kStep / 2 + c, lo16);
-                if (c == kStep / 4 - 16 || c == kStep / 2 - 16) {
-                    tc::wait_st();
-                    tc::fence_before();
-                    mbar_arrive(&p_full[turn.buffer][c >= kStep / 4]);
+                    tc::st16(ts + c, hi16);                // over the logits of these keys
+                    if constexpr (I8) tc::st16(ts + c + 16, lo16);
+                    if (c & 32) {                          // half of the keys
+                        tc::wait_st();
+                        tc::fence_before();
+                        mbar_arrive(&p_full[turn.buffer][c >> 6]);
+                    }
                 }
             }
             part[0] = add2(part[0], part[1]);
