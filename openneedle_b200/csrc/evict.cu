@@ -15,6 +15,7 @@ namespace nb200 {
 namespace {
 
 constexpr int kThreads = 1024;
+constexpr int kCopyRows = 296;   // rows (two a multiprocessor) from which the selecting CTAs copy
 
 // Order-preserving unsigned key of a weight; both zeros are one value.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -23,18 +24,62 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// kRowsOf kept rows, `step` apart from row i0 on, to the output, all in flight at
+// once: the thread's 16-byte piece of K and of V (a row has 1 << shift pieces).
+constexpr int kRowsOf = 2;
+
+__device__ __forceinline__ void copy_rows(const Evict &e, int unit, int i0, int step, int kept, int shift) {
+    const int g = unit % e.kvheads, b = unit / e.kvheads, piece = threadIdx.x & ((1 << shift) - 1);
+    const int *idx = e.indices + (long long)unit * e.keep;
+    long long j[kRowsOf];
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r) j[r] = i0 + r * step < kept ? idx[i0 + r * step] : -1;
+    const char *k = e.k + b * e.ks[0] + g * e.ks[1] + piece * 16, *v = e.v + b * e.vs[0] + g * e.vs[1] + piece * 16;
+    uint4 x[kRowsOf], y[kRowsOf];
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r)
+        if (j[r] >= 0) {
+            x[r] = __ldcs((const uint4 *)(k + j[r] * e.ks[2]));
+            y[r] = __ldcs((const uint4 *)(v + j[r] * e.vs[2]));
+        }
+    float s[kRowsOf];
+    const bool scales = e.kscale && piece < 2;       // piece 0 moves K's, piece 1 V's
+    if (scales) {
+        const float *sc = piece == 0 ? e.kscale + b * e.kss[0] + g * e.kss[1] : e.vscale + b * e.vss[0] + g * e.vss[1];
+        const long long next = piece == 0 ? e.kss[2] : e.vss[2];
+#pragma unroll
+        for (int r = 0; r < kRowsOf; ++r)
+            if (j[r] >= 0) s[r] = sc[j[r] * next];
+    }
+    char *ko = e.ko + b * e.kos[0] + g * e.kos[1] + piece * 16, *vo = e.vo + b * e.vos[0] + g * e.vos[1] + piece * 16;
+#pragma unroll
+    for (int r = 0; r < kRowsOf; ++r)
+        if (j[r] >= 0) {
+            const long long i = i0 + r * step;
+            *(uint4 *)(ko + i * e.kos[2]) = x[r];
+            *(uint4 *)(vo + i * e.vos[2]) = y[r];
+            if (scales) {
+                if (piece == 0)
+                    e.kscale_o[b * e.ksos[0] + g * e.ksos[1] + i * e.ksos[2]] = s[r];
+                else
+                    e.vscale_o[b * e.vsos[0] + g * e.vsos[1] + i * e.vsos[2]] = s[r];
+            }
+        }
+}
+
 // Selection with a row's weights in registers: a cluster of C CTAs per
 // (sequence, KV head), each thread up to kMine weights of its CTA's contiguous
 // segment.  The key of the last weight that stays is found eight bits at a time
 // from the top: the keys that still match are counted by digit in shared memory
-// (few of them after the first round, so that counting costs little), the counts
-// of a cluster's CTAs meet by distributed shared memory.  Then ties and kept
+// (few of them after the first round), the counts of a cluster's CTAs meet by
+// distributed shared memory, and the search ends where a digit's keys are just as
+// many as stay.  Then ties (where some of them stay and others not) and kept
 // positions are ranked in index order, and everything is written.  The weights
 // are read once; bound by the latency of the rounds.
 constexpr int kMine = 16;
 
-template <int C, int T>
-__global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
+template <int C, int T, bool COPY>
+__global__ __launch_bounds__(T, T == 256 ? 4 : 1) void evict_rank_kernel(const Evict e, int shift) {
     constexpr int kWarpsIn = T / 32;
     const int row = blockIdx.x / C, rank = blockIdx.x % C;
     const int g = row % e.kvheads, b = row / e.kvheads;
@@ -44,7 +89,7 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
     float *wo = e.weights_o + b * e.wos[0] + g * e.wos[1];
     int *idx = e.indices + (long long)row * e.keep;
     __shared__ int counts[4][256];
-    __shared__ int sums[8], found[2];
+    __shared__ int sums[8], found[3];
     __shared__ int ranks[2][kMine * kWarpsIn + 1];   // ties, kept: of (i, warp), then exclusive sums; last: their total
     for (int i = tid; i < 1024; i += T) (&counts[0][0])[i] = 0;
 
@@ -78,8 +123,9 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
     int need = e.keep - e.first - e.recent;          // of the keys equal to `prefix` so far
     const bool none = need == 0;
     uint32_t prefix = 0;
+    bool exact = false;                              // all keys from `prefix` on stay
     if (choose && !none) {                           // the same in every CTA of the row
-        for (int it = 0; it < 4; ++it) {
+        for (int it = 0; it < 4 && !exact; ++it) {
             const int shift = 24 - 8 * it;
             const uint32_t mask = it == 0 ? 0u : ~0u << (shift + 8);
 #pragma unroll
@@ -108,11 +154,13 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
                 if (above >= need && above - total < need) {
                     found[0] = 255 - tid;
                     found[1] = need - (above - total);
+                    found[2] = total;
                 }
             }
             __syncthreads();
             prefix |= (uint32_t)found[0] << shift;
             need = found[1];
+            exact = need == found[2];
         }
     }
 
@@ -141,7 +189,7 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
         return before;
     };
     int tie_base = 0;
-    if (choose && !none) {
+    if (choose && !none && !exact) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             if (i >= mine) break;
@@ -158,10 +206,12 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
         const int j = j0 + i * T + tid;
         const uint32_t u = weight_key(x[i]);
         const bool middle = choose && j >= lo && j < hi;
-        const bool tie = middle && !none && u == prefix;
-        const unsigned m = __ballot_sync(0xffffffffu, tie);
-        bool s = j < n && (!middle || (!none && u > prefix));
-        if (tie) s = tie_base + ranks[0][i * kWarpsIn + warp] + __popc(m & ((1u << lane) - 1)) < need;
+        bool s = j < n && (!middle || (!none && u >= prefix));
+        if (!exact) {                                // the first `need` of the ties stay
+            const bool tie = middle && !none && u == prefix;
+            const unsigned m = __ballot_sync(0xffffffffu, tie);
+            if (tie) s = tie_base + ranks[0][i * kWarpsIn + warp] + __popc(m & ((1u << lane) - 1)) < need;
+        }
         const unsigned k = __ballot_sync(0xffffffffu, s);
         if (lane == 0) ranks[1][i * kWarpsIn + warp] = __popc(k);
         stays |= (uint32_t)s << i;
@@ -182,6 +232,11 @@ __global__ __launch_bounds__(T) void evict_rank_kernel(const Evict e) {
     for (int i = kept + rank * T + tid; i < e.out_capacity; i += C * T) wo[i * e.wos[2]] = 0.f;
     if (g == 0 && rank == 0 && tid == 0) e.lengths_o[b] = kept;
     if constexpr (C > 1) all_sync();                 // no CTA ends while another reads its counts
+    if constexpr (COPY) {
+        __syncthreads();                             // (the indexes)
+        const int step = T >> shift;
+        for (int i = tid >> shift; i < kept; i += kRowsOf * step) copy_rows(e, row, i, step, kept, shift);
+    }
 }
 
 // Selection of rows too long for that: one CTA per (sequence, KV head) reads the
@@ -278,51 +333,13 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const Evict e) {
     if (g == 0 && tid == 0) e.lengths_o[b] = kept;
 }
 
-// Kept rows to other memory: 16-byte pieces of K and of V, kRowsOf rows of a
-// thread in flight at once.
-constexpr int kRowsOf = 4;
-
-__global__ __launch_bounds__(256) void evict_gather_kernel(const Evict e, int chunks, int pieces, int shift) {
-    const int unit = blockIdx.x / chunks, g = unit % e.kvheads, b = unit / e.kvheads;
-    const int rows = 256 >> shift, piece = threadIdx.x & (pieces - 1);
-    const int i0 = blockIdx.x % chunks * (kRowsOf * rows) + (threadIdx.x >> shift);
+// Kept rows to other memory by a grid of their own.
+__global__ __launch_bounds__(256) void evict_gather_kernel(const Evict e, int chunks, int shift) {
+    const int unit = blockIdx.x / chunks;
     pdl_enter();
-    const int kept = min(max(0, min(e.lengths[b], e.capacity)), e.keep);
-    const int *idx = e.indices + (long long)unit * e.keep;
-    long long j[kRowsOf];
-#pragma unroll
-    for (int r = 0; r < kRowsOf; ++r) j[r] = i0 + r * rows < kept ? idx[i0 + r * rows] : -1;
-    const char *k = e.k + b * e.ks[0] + g * e.ks[1] + piece * 16, *v = e.v + b * e.vs[0] + g * e.vs[1] + piece * 16;
-    uint4 x[kRowsOf], y[kRowsOf];
-#pragma unroll
-    for (int r = 0; r < kRowsOf; ++r)
-        if (j[r] >= 0) {
-            x[r] = __ldcs((const uint4 *)(k + j[r] * e.ks[2]));
-            y[r] = __ldcs((const uint4 *)(v + j[r] * e.vs[2]));
-        }
-    float s[kRowsOf];
-    const bool scales = e.kscale && piece < 2;       // piece 0 moves K's, piece 1 V's
-    if (scales) {
-        const float *sc = piece == 0 ? e.kscale + b * e.kss[0] + g * e.kss[1] : e.vscale + b * e.vss[0] + g * e.vss[1];
-        const long long step = piece == 0 ? e.kss[2] : e.vss[2];
-#pragma unroll
-        for (int r = 0; r < kRowsOf; ++r)
-            if (j[r] >= 0) s[r] = sc[j[r] * step];
-    }
-    char *ko = e.ko + b * e.kos[0] + g * e.kos[1] + piece * 16, *vo = e.vo + b * e.vos[0] + g * e.vos[1] + piece * 16;
-#pragma unroll
-    for (int r = 0; r < kRowsOf; ++r)
-        if (j[r] >= 0) {
-            const long long i = i0 + r * rows;
-            *(uint4 *)(ko + i * e.kos[2]) = x[r];
-            *(uint4 *)(vo + i * e.vos[2]) = y[r];
-            if (scales) {
-                if (piece == 0)
-                    e.kscale_o[b * e.ksos[0] + g * e.ksos[1] + i * e.ksos[2]] = s[r];
-                else
-                    e.vscale_o[b * e.vsos[0] + g * e.vsos[1] + i * e.vsos[2]] = s[r];
-            }
-        }
+    const int kept = min(max(0, min(e.lengths[unit / e.kvheads], e.capacity)), e.keep);
+    copy_rows(e, unit, blockIdx.x % chunks * (kRowsOf * (256 >> shift)) + (threadIdx.x >> shift), 256 >> shift, kept,
+              shift);
 }
 
 // The same in place: one CTA moves a (sequence, KV head) front to back, a
@@ -367,8 +384,8 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const Evict e) {
 
 namespace {
 
-template <int C, int T>
-bool launch_rank(const Evict &e, int rows, cudaStream_t st) {
+template <int C, int T, bool COPY = false>
+bool launch_rank(const Evict &e, int rows, int shift, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * C);
     cfg.blockDim = dim3(T);
@@ -379,7 +396,7 @@ bool launch_rank(const Evict &e, int rows, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    NB_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_rank_kernel<C, T>, e));
+    NB_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_rank_kernel<C, T, COPY>, e, shift));
     return true;
 }
 
@@ -388,17 +405,21 @@ bool launch_rank(const Evict &e, int rows, cudaStream_t st) {
 bool launch_evict(const Evict &e, cudaStream_t st) {
     const int units = e.batch * e.kvheads;
     if (units == 0) return true;
-    // a row's weights in registers: as few CTAs as hold them
+    const int pieces = e.row_bytes / 16, shift = pieces == 4 ? 2 : pieces == 8 ? 3 : 4;
     const int n = e.capacity;
+    // where the rows fill the machine, each CTA copies its own (one's selection runs
+    // beside another's copies: 69 -> 65 us for 1024 rows of 3712 INT8 keys)
+    if (!e.in_place && n <= 256 * kMine && units >= kCopyRows) return launch_rank<1, 256, true>(e, units, shift, st);
+    // a row's weights in registers: as few CTAs as hold them
     bool ok;
     if (n <= 256 * kMine)
-        ok = launch_rank<1, 256>(e, units, st);
+        ok = launch_rank<1, 256>(e, units, shift, st);
     else if (n <= 1024 * kMine)
-        ok = launch_rank<1, 1024>(e, units, st);
+        ok = launch_rank<1, 1024>(e, units, shift, st);
     else if (n <= 4 * 1024 * kMine)
-        ok = launch_rank<4, 1024>(e, units, st);
+        ok = launch_rank<4, 1024>(e, units, shift, st);
     else if (n <= 8 * 1024 * kMine)
-        ok = launch_rank<8, 1024>(e, units, st);
+        ok = launch_rank<8, 1024>(e, units, shift, st);
     else {
         evict_select_kernel<<<units, kThreads, 0, st>>>(e);
         NB_CUDA_TRY(cudaGetLastError());
@@ -409,10 +430,9 @@ bool launch_evict(const Evict &e, cudaStream_t st) {
         NB_CUDA_TRY(launch_pdl(evict_move_kernel, dim3(units), dim3(kThreads), 0, st, e));
         return true;
     }
-    const int pieces = e.row_bytes / 16, shift = pieces == 4 ? 2 : pieces == 8 ? 3 : 4;
     const int chunks = ceil_div(e.keep, kRowsOf * (256 >> shift));
     if (chunks == 0) return true;
-    NB_CUDA_TRY(launch_pdl(evict_gather_kernel, dim3(units * chunks), dim3(256), 0, st, e, chunks, pieces, shift));
+    NB_CUDA_TRY(launch_pdl(evict_gather_kernel, dim3(units * chunks), dim3(256), 0, st, e, chunks, shift));
     return true;
 }
 

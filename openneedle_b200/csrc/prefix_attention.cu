@@ -611,16 +611,9 @@ __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, in
     const long long bt = row / p.heads;
     const int t = (int)(bt % p.tokens), b = (int)(bt / p.tokens);
     if (t >= own_tokens(p, b)) return;
-    // four partial results in flight at a time
-    float top = kNegInf;
-    for (int i = 0; i < slots; i += 4) {
-        float l[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) l[e] = i + e < slots ? p.part_lse[(i + e) * nrows + row] : kNegInf;
-        top = fmaxf(max3(top, l[0], l[1]), fmaxf(l[2], l[3]));
-    }
-    const float t0 = top == kNegInf ? 0.f : top;
-    float total = 0.f;
+    // four partial results in flight at a time, merged as they come (o of an empty
+    // range was not written: it is read and not used)
+    float top = kNegInf, total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < slots; i += 4) {
         float l[4];
@@ -628,18 +621,22 @@ __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, in
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             l[e] = i + e < slots ? p.part_lse[(i + e) * nrows + row] : kNegInf;
-            v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            v[e] = *(const float4 *)(p.part_o + (min(i + e, slots - 1) * nrows + row) * HD + part);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (l[e] != kNegInf) v[e] = *(const float4 *)(p.part_o + ((i + e) * nrows + row) * HD + part);
+        const float now = fmaxf(max3(top, l[0], l[1]), fmaxf(l[2], l[3]));
+        const float base = now == kNegInf ? 0.f : now, keep = ex2(top - base);
+        total *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+        top = now;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float f = ex2(l[e] - t0);
+            if (l[e] == kNegInf) continue;
+            const float f = ex2(l[e] - base);
             total += f;
             acc.x += f * v[e].x; acc.y += f * v[e].y; acc.z += f * v[e].z; acc.w += f * v[e].w;
         }
     }
+    const float t0 = top == kNegInf ? 0.f : top;
     const float inv = total == 0.f ? 0.f : 1.f / total;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + part) * (I8 ? 4 : 2);
