@@ -211,6 +211,14 @@ int needle2_attention_query(void *kv, const int *session_ids, const int *positio
                             int count);
 int needle2_attention_query_device(void *kv, const int *session_ids, const int *positions, const float *q, float *out,
                                    int count, void *stream);
+/* The same with the shared prefix attended once for all entries (the queries as
+ * the rows of one matrix product on the tensor cores) instead of once for each;
+ * head_dim 64 or 128, positions behind the prefix.  Outputs agree with
+ * needle2_attention_query within FP32 rounding. */
+int needle2_attention_query_shared(void *kv, const int *session_ids, const int *positions, const float *q, float *out,
+                                   int count);
+int needle2_attention_query_shared_device(void *kv, const int *session_ids, const int *positions, const float *q,
+                                          float *out, int count, void *stream);
 /* Decode step: store each session's new K/V at its position, then attend. */
 int needle2_attention_decode(void *kv, const int *session_ids, const int *positions, const float *q, const float *k,
                              const float *v, float *out, int count);

@@ -38,6 +38,8 @@ def _bind():
     lib.needle2_kv_store_device.argtypes = [_p, _p, _p, _p, _p, _i, _p]
     lib.needle2_attention_query.argtypes = [_p, _p, _p, _p, _p, _i]
     lib.needle2_attention_query_device.argtypes = [_p, _p, _p, _p, _p, _i, _p]
+    lib.needle2_attention_query_shared.argtypes = [_p, _p, _p, _p, _p, _i]
+    lib.needle2_attention_query_shared_device.argtypes = [_p, _p, _p, _p, _p, _i, _p]
     lib.needle2_attention_decode.argtypes = [_p, _p, _p, _p, _p, _p, _p, _i]
     lib.needle2_attention_decode_device.argtypes = [_p, _p, _p, _p, _p, _p, _p, _i, _p]
     lib.needle2_attention_prefill.argtypes = [_p, _p, _p, _i, _p, _p, _p, _p, _i]
@@ -45,6 +47,7 @@ def _bind():
     lib.needle2_kv_export.argtypes = [_p, _i, _p, _p, _p, _p]
     for name in ("needle2_kv_set_prefix", "needle2_kv_set_prefix_device", "needle2_kv_store",
                  "needle2_kv_store_device", "needle2_attention_query", "needle2_attention_query_device",
+                 "needle2_attention_query_shared", "needle2_attention_query_shared_device",
                  "needle2_attention_decode", "needle2_attention_decode_device", "needle2_attention_prefill",
                  "needle2_attention_prefill_device", "needle2_kv_export"):
         getattr(lib, name).restype = _i
@@ -107,12 +110,21 @@ class KVCache:
                                           v.ctypes.data, ids.size), "kv_store")
 
     def query(self, session_ids, positions, q):
+        return self._query(self._lib.needle2_attention_query, session_ids, positions, q)
+
+    def query_shared(self, session_ids, positions, q):
+        """``query`` with the shared prefix attended once for all the sessions of
+        the call (head_dim 64 or 128, positions behind the prefix): for long
+        prefixes and many sessions."""
+        return self._query(self._lib.needle2_attention_query_shared, session_ids, positions, q)
+
+    def _query(self, call, session_ids, positions, q):
         ids, pos, q = _i32(session_ids), _i32(positions), _f32(q)
         if q.shape != (ids.size, self.heads * self.head_dim) or pos.size != ids.size:
             raise ValueError("query: q must be [count, heads*head_dim]")
         out = np.empty_like(q)
-        _check(self._lib.needle2_attention_query(self._handle, ids.ctypes.data, pos.ctypes.data, q.ctypes.data,
-                                                 out.ctypes.data, ids.size), "attention_query")
+        _check(call(self._handle, ids.ctypes.data, pos.ctypes.data, q.ctypes.data, out.ctypes.data, ids.size),
+               "attention_query")
         return out
 
     def decode(self, session_ids, positions, q, k, v):
@@ -172,6 +184,12 @@ class KVCache:
         _check(self._lib.needle2_attention_query_device(self._handle, ids.ctypes.data, pos.ctypes.data, q.data_ptr(),
                                                         out.data_ptr(), ids.size, _stream_ptr(stream)),
                "attention_query_device")
+
+    def query_shared_device(self, session_ids, positions, q, out, stream=None) -> None:
+        ids, pos = _i32(session_ids), _i32(positions)
+        _check(self._lib.needle2_attention_query_shared_device(self._handle, ids.ctypes.data, pos.ctypes.data,
+                                                               q.data_ptr(), out.data_ptr(), ids.size,
+                                                               _stream_ptr(stream)), "attention_query_shared_device")
 
     def prefill_device(self, session_ids, start_positions, tokens, q, k, v, out, stream=None) -> None:
         ids, pos = _i32(session_ids), _i32(start_positions)

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/needle2_b200.h"
+#include "cache_ops.cuh"
 #include "common.cuh"
 #include "evict.cuh"
 #include "prefix_attention.cuh"
@@ -262,6 +263,14 @@ bool evict(const needle2_evict_args &a, cudaStream_t st) {
 }
 
 }  // namespace
+
+long long prefix_attention_workspace(const needle2_prefix_attention_args &a) {
+    return sizes_ok(a) ? plan_of(a).bytes : -1;
+}
+bool prefix_attention(const needle2_prefix_attention_args &a, void *workspace, long long bytes, cudaStream_t st) {
+    return attention(a, workspace, bytes, st);
+}
+
 }  // namespace nb200
 
 namespace {
@@ -287,13 +296,13 @@ long long entry(const void *args, F f) {
 extern "C" {
 
 long long needle2_prefix_attention_workspace(const needle2_prefix_attention_args *args) {
-    return entry(args, [&]() -> long long { return nb200::sizes_ok(*args) ? nb200::plan_of(*args).bytes : -1; });
+    return entry(args, [&] { return nb200::prefix_attention_workspace(*args); });
 }
 
 int needle2_prefix_attention_device(const needle2_prefix_attention_args *args, void *workspace,
                                     long long workspace_bytes, void *stream) {
     return (int)entry(args, [&]() -> long long {
-        return nb200::attention(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? 0 : -1;
+        return nb200::prefix_attention(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? 0 : -1;
     });
 }
 

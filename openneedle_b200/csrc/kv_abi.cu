@@ -13,6 +13,7 @@
 
 #include "../../include/needle2_b200.h"
 #include "attention.cuh"
+#include "cache_ops.cuh"
 #include "common.cuh"
 #include "cq_gemv.cuh"
 #include "kv_pool.cuh"
@@ -56,6 +57,7 @@ struct KVPool {
     Buf<float> pks, pvs, sks, svs, stks, stvs, pm, pl, pacc, hq, hk, hv, hout;
     Buf<float> pkf, pvf, skf, svf, stkf, stvf;   // FP32 cache
     Buf<int> ids, pos;
+    Buf<int8_t> shared_ws;                       // workspace of the shared-prefix query
     ~KVPool() {
         cudaSetDevice(device);
         if (stream) cudaStreamSynchronize(stream);
@@ -64,6 +66,7 @@ struct KVPool {
         for (auto *b : {&pkf, &pvf, &skf, &svf, &stkf, &stvf}) b->release();
         ids.release();
         pos.release();
+        shared_ws.release();
         if (stream) cudaStreamDestroy(stream);
     }
     int capacity() const { return window ? window + prefix : max_seq; }
@@ -221,6 +224,49 @@ bool stage(KVPool &kv, const float *k, const float *v, int rows, cudaStream_t st
 }
 
 KVPool *pool(void *h) { return static_cast<KVPool *>(h); }
+
+// One query per entry, the pool's prefix attended once for all of them.  An entry
+// sees the whole prefix and its slots [0, own): the slots of a window's ring hold
+// exactly the window, in another order (positions enter no formula).
+bool query_shared(KVPool &kv, const int *session_ids, const int *positions, int count, const float *q, float *out,
+                  cudaStream_t st) {
+    if (kv.fp32) { set_error("the shared-prefix query reads INT8 pools"); return false; }
+    std::vector<int> own(count);
+    int most = 1;
+    for (int i = 0; i < count; ++i) {
+        own[i] = positions[i] - kv.prefix + 1;
+        if (kv.window) own[i] = std::min(own[i], kv.window);
+        most = std::max(most, own[i]);
+    }
+    if (!upload_index(kv, session_ids, own.data(), count, st)) return false;
+    needle2_prefix_attention_args a{};
+    a.batch = count; a.tokens = 1; a.heads = kv.heads; a.kvheads = kv.kvheads; a.head_dim = kv.hd;
+    a.prefix = kv.prefix;
+    a.capacity = most;                           // the longest entry decides how the keys are split
+    a.cache_type = 0;
+    a.scale = 1 / std::sqrt((float)kv.hd);
+    const long long width = (long long)kv.heads * kv.hd, row = kv.hd;
+    const long long query[3] = {width, width, row};
+    const long long rows[3] = {(long long)kv.kvheads * kv.cs * row, (long long)kv.cs * row, row};
+    const long long flat[3] = {(long long)kv.kvheads * kv.cs, kv.cs, 1};
+    for (int i = 0; i < 3; ++i) {
+        a.q_stride[i] = a.out_stride[i] = query[i];
+        a.k_stride[i] = a.v_stride[i] = rows[i];
+        a.k_scale_stride[i] = a.v_scale_stride[i] = flat[i];
+    }
+    a.prefix_k_stride[0] = a.prefix_v_stride[0] = kv.prefix * row;
+    a.prefix_k_stride[1] = a.prefix_v_stride[1] = row;
+    a.prefix_k_scale_stride[0] = a.prefix_v_scale_stride[0] = kv.prefix;
+    a.prefix_k_scale_stride[1] = a.prefix_v_scale_stride[1] = 1;
+    a.q = q; a.out = out;
+    a.k = kv.sk.ptr; a.v = kv.sv.ptr; a.k_scales = kv.sks.ptr; a.v_scales = kv.svs.ptr;
+    a.prefix_k = kv.pk.ptr; a.prefix_v = kv.pv.ptr; a.prefix_k_scales = kv.pks.ptr; a.prefix_v_scales = kv.pvs.ptr;
+    a.lengths = kv.pos.ptr;
+    a.cache_rows = kv.ids.ptr;
+    const long long bytes = prefix_attention_workspace(a);
+    if (bytes < 0 || !kv.shared_ws.reserve((size_t)bytes)) return false;
+    return prefix_attention(a, kv.shared_ws.ptr, bytes, st);
+}
 
 }  // namespace
 
@@ -384,7 +430,8 @@ int needle2_kv_set_prefix(void *h, const float *k, const float *v) {
     return 0;
 }
 
-// mode: 0 = store only, 1 = store then attend (decode), 2 = attend only.
+// mode: 0 = store only, 1 = store then attend (decode), 2 = attend only, 4 =
+// attend only, the prefix once for all entries (3 is the host calls' prefill).
 static int decode_device(void *h, const int *session_ids, const int *positions, const float *q, const float *k,
                          const float *v, float *out, int count, void *stream, int mode) {
     nb200::clear_error();
@@ -394,6 +441,7 @@ static int decode_device(void *h, const int *session_ids, const int *positions, 
     if (!nb200::validate(*kv, session_ids, positions, count, 1, mode == 2)) return -1;
     if (cudaSetDevice(kv->device) != cudaSuccess) { nb200::set_error("cudaSetDevice failed"); return -1; }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (mode == 4) return nb200::query_shared(*kv, session_ids, positions, count, q, out, st) ? 0 : -1;
     if (!nb200::upload_index(*kv, session_ids, positions, count, st)) return -1;
     const nb200::KVOp op = mode == 0 ? nb200::kStore : mode == 1 ? nb200::kDecode : nb200::kQuery;
     const int len = nb200::kv_max_visible(kv->prefix, kv->window, positions, count, 1);
@@ -411,6 +459,11 @@ int needle2_kv_store_device(void *h, const int *session_ids, const int *position
 int needle2_attention_query_device(void *h, const int *session_ids, const int *positions, const float *q, float *out,
                                    int count, void *stream) {
     return decode_device(h, session_ids, positions, q, nullptr, nullptr, out, count, stream, 2);
+}
+
+int needle2_attention_query_shared_device(void *h, const int *session_ids, const int *positions, const float *q,
+                                          float *out, int count, void *stream) {
+    return decode_device(h, session_ids, positions, q, nullptr, nullptr, out, count, stream, 4);
 }
 
 int needle2_attention_prefill_device(void *h, const int *session_ids, const int *start_positions, int tokens,
@@ -473,6 +526,10 @@ int needle2_kv_store(void *h, const int *session_ids, const int *positions, cons
 int needle2_attention_query(void *h, const int *session_ids, const int *positions, const float *q, float *out,
                             int count) {
     return host_call(h, session_ids, positions, q, nullptr, nullptr, out, count, 1, 2);
+}
+int needle2_attention_query_shared(void *h, const int *session_ids, const int *positions, const float *q, float *out,
+                                   int count) {
+    return host_call(h, session_ids, positions, q, nullptr, nullptr, out, count, 1, 4);
 }
 int needle2_attention_prefill(void *h, const int *session_ids, const int *start_positions, int tokens, const float *q,
                               const float *k, const float *v, float *out, int count) {

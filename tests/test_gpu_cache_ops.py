@@ -303,6 +303,80 @@ def test_evict_into_strided_outputs(ops):
     check_evicted(e, c, 150, 5, 10, behind=behind)
 
 
+@pytest.mark.parametrize("cache,d,s", [("int8", 64, 40), ("bf16", 128, 33), ("int8", 64, 4100)])
+def test_evict_many_rows(ops, cache, d, s):
+    """More rows than the machine has places for: selection and copies in one kernel, and (4100) in two."""
+    b, kv = 75, 4
+    c = evict_inputs(cache, b, kv, d, s, [s - (i * 7) % s for i in range(b)], seed=s)
+    e, _ = evicted(ops, c, s // 3, 2, 5)
+    check_evicted(e, c, s // 3, 2, 5)
+
+
+@pytest.mark.parametrize("s,lengths", [(20000, [20000, 70]), (70000, [70000, 66000]), (140000, [140000, 139999])])
+def test_evict_long_rows(ops, s, lengths):
+    """One CTA, four, eight a row, and rows beyond their registers; against a stable sort."""
+    g = torch.Generator("cuda").manual_seed(s)
+    b, kv, d, keep, first, recent = 2, 2, 64, 5000, 16, 700
+    k = torch.randint(-127, 128, (b, kv, s, d), generator=g, device="cuda", dtype=torch.int8)
+    v = torch.randint(-127, 128, (b, kv, s, d), generator=g, device="cuda", dtype=torch.int8)
+    ks, vs = (torch.rand(b, kv, s, generator=g, device="cuda") for _ in range(2))
+    w = torch.exp(4 * torch.randn(b, kv, s, generator=g, device="cuda"))
+    w[torch.rand(b, kv, s, generator=g, device="cuda") < 0.4] = 0.0
+    w = torch.where(torch.rand(b, kv, s, generator=g, device="cuda") < 0.3, w.round(), w)
+    e = ops.evict(k, v, w, torch.tensor(lengths, dtype=torch.int32, device="cuda"), keep, first=first, recent=recent,
+                  k_scales=ks, v_scales=vs)
+    for i, n in enumerate(lengths):
+        assert int(e.lengths[i]) == min(n, keep)
+        for h in range(kv):
+            if n <= keep:
+                at = torch.arange(n, device="cuda")
+            else:
+                x = w[i, h, :n].clone()
+                x[:first] = math.inf
+                x[n - recent:] = math.inf
+                at = torch.sort(x, descending=True, stable=True).indices[:keep].sort().values
+            m = len(at)
+            assert torch.equal(e.indices[i, h, :m], at.int()) and (e.indices[i, h, m:] == -1).all()
+            for x, y in ((e.k, k), (e.v, v), (e.k_scales, ks), (e.v_scales, vs), (e.weights, w)):
+                assert torch.equal(x[i, h, :m], y[i, h][at])
+            assert (e.weights[i, h, m:] == 0).all()
+
+
+# ---- the KV pool's shared-prefix query -------------------------------------------
+
+@pytest.mark.parametrize("heads,kvheads,hd,window,prefix,sessions", [
+    (8, 4, 64, 0, 24, 3), (8, 4, 64, 16, 7, 5), (8, 8, 64, 0, 5, 4), (4, 1, 128, 9, 33, 40), (4, 2, 128, 0, 0, 3),
+    (16, 2, 64, 0, 300, 70), (8, 4, 64, 24, 700, 33)])
+def test_pool_query_shared(ops, heads, kvheads, hd, window, prefix, sessions):
+    """KVCache.query_shared against KVCache.query on the same pool (whose outputs the oracle pins): ring windows
+    before and after they are full, sessions in another order and left out."""
+    import numpy as np
+    from util import FP32_REL_TOL, rel_err
+    rng = np.random.default_rng(prefix + sessions)
+    kv = ops.KVCache(sessions, heads, kvheads, hd, prefix + 64, window, prefix)
+    if prefix:
+        kv.set_prefix(*(rng.normal(size=(prefix, kvheads * hd)).astype(np.float32) for _ in range(2)))
+    for step in range(40):
+        ids = rng.permutation(sessions)
+        k, v = (rng.normal(size=(sessions, kvheads * hd)).astype(np.float32) for _ in range(2))
+        kv.store(ids, [prefix + step] * sessions, k, v)
+        if step in (0, 10, 39):
+            some = rng.permutation(sessions)[:max(1, sessions - 2)]
+            q = rng.normal(size=(len(some), heads * hd)).astype(np.float32)
+            got = kv.query_shared(some, [prefix + step] * len(some), q)
+            assert rel_err(got, kv.query(some, [prefix + step] * len(some), q)) <= FP32_REL_TOL
+            qd = torch.from_numpy(q).cuda()
+            out = torch.empty_like(qd)
+            kv.query_shared_device(some, [prefix + step] * len(some), qd, out)
+            torch.cuda.synchronize()
+            np.testing.assert_array_equal(out.cpu().numpy(), got)
+    with pytest.raises(RuntimeError, match="appears twice"):
+        kv.query_shared([0, 0], [prefix] * 2, np.zeros((2, heads * hd), np.float32))
+    if prefix:
+        with pytest.raises(RuntimeError, match="inside the shared prefix"):
+            kv.query_shared([0], [prefix - 1], np.zeros((1, heads * hd), np.float32))
+
+
 # ---- a run of them together, streams and graphs -------------------------------------
 
 @pytest.mark.parametrize("cache", CACHES)
