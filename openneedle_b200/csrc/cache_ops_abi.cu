@@ -50,10 +50,11 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
 }
 
 constexpr int kJointKeys = 512;
+constexpr long long kMaxLogits = 1LL << 26;   // kept for the weights
 
 struct Plan {
     PrefixSplit prefix, own;
-    bool joint, logits, neg_lse, weight_tiles;
+    bool joint, joint_tiles, logits, neg_lse, weight_tiles;
     long long part_o, part_lse, neg_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
 
@@ -72,21 +73,28 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     const int sms = sm_count();
     const int R = a.heads / a.kvheads, tile = a.cache_type == kCacheI8 ? 8 : 16;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
-    // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys
+    // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys.
+    // Tiles or streaming by their times, fitted to measurements (us): a tile CTA has its
+    // multiprocessor to itself and takes 9 beside 0.9 for 128 keys of one tile (1.8 of
+    // two), a streaming unit 1.2 of one beside its keys, of which the 16-bit caches'
+    // 128 dimensions take longest.  (358 sequences of 16 rows and 88 INT8 keys: 500 by
+    // tiles, 100 streaming; two prompts of 4096 tokens: 5100 streaming, 340 by tiles.)
+    const double key = (a.cache_type == kCacheI8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
     auto split = [&](long long groups, long long group_rows, long long keys) {
-        PrefixSplit s;
-        s.tiles = group_rows > tile;
-        if (s.tiles) {
-            s.alt = group_rows <= 128 || (a.cache_type == kCacheI8 && a.head_dim == 128);
-            const long long units = groups * ((group_rows + (s.alt ? 127 : 255)) / (s.alt ? 128 : 256));
-            const long long most = (keys + (s.alt ? 511 : 255)) / (s.alt ? 512 : 256);
-            s.ranges = (int)std::max(1LL, std::min({sms / std::max(1LL, units), most, 32LL}));
-        } else {
-            const long long units = groups * ((group_rows + tile - 1) / tile);
-            const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
-            s.ranges = (int)std::max(1LL, std::min({want, (keys + 255) / 256, 64LL}));
-        }
-        return s;
+        PrefixSplit s, t;
+        t.tiles = true;
+        t.alt = group_rows <= 128 || (a.cache_type == kCacheI8 && a.head_dim == 128);
+        const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
+        const long long most = (keys + (t.alt ? 511 : 255)) / (t.alt ? 512 : 256);
+        t.ranges = (int)std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL}));
+        const long long units = groups * ((group_rows + tile - 1) / tile);
+        const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
+        s.ranges = (int)std::max(1LL, std::min({want, (keys + 255) / 256, 64LL}));
+        if (group_rows <= tile) return s;
+        const double waves = std::max(1.0, (double)tiles * t.ranges / sms);
+        const double by_tiles = waves * (9.0 + (t.alt ? 7e-3 : 14e-3) * (double)keys / t.ranges);
+        const double streaming = 4.0 + units * (1.2 + key * (double)keys) / sms;
+        return by_tiles < streaming ? t : s;
     };
     const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
     if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span);
@@ -97,13 +105,19 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.prefix.ranges = 0;
         p.own.ranges = 1;
     }
+    // tiles of the sequences' own rows that fill the machine take the prefix first, in
+    // the same accumulators: no partial results
+    p.joint_tiles = a.prefix && p.own.tiles && p.prefix.tiles && p.own.ranges == 1 &&
+                    (long long)a.batch * a.kvheads * ((a.tokens * R + 255) / 256) * 5 >= 4LL * sms;
+    if (p.joint_tiles) p.prefix = PrefixSplit{};
     if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros
         p.own = PrefixSplit{};
         p.own.ranges = 1;
     }
-    p.logits = a.weights && a.tokens > 0 && !p.own.tiles;     // (the tile kernel's rows are too many to keep)
+    p.logits = a.weights && a.tokens > 0 && !p.own.tiles && a.tokens * R <= kMaxLogitRows &&
+               (long long)a.batch * a.kvheads * a.tokens * R * a.capacity <= kMaxLogits;
     p.neg_lse = a.weights != nullptr;
-    p.weight_tiles = a.weights && p.own.tiles && R <= 128;
+    p.weight_tiles = a.weights && !p.logits && a.tokens > 0 && R <= 128;
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long r = at;
@@ -192,7 +206,8 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
         const bool tiles = plan.prefix.tiles || plan.own.tiles, stream = stream_prefix || stream_own;
         // the first axis of a cache addressed by cache_rows has an extent that only the caller knows
         if (tiles &&
-            !launch_prefix_tiles(p, plan.prefix, plan.own, a.cache_rows ? 1LL << 30 : a.batch, stream, st))
+            !launch_prefix_tiles(p, plan.prefix, plan.own, plan.joint_tiles, a.cache_rows ? 1LL << 30 : a.batch, stream,
+                                 st))
             return false;
         if (stream && !launch_prefix_stream(p, stream_prefix, stream_own, plan.joint, tiles, st)) return false;
     }

@@ -652,7 +652,6 @@ __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, in
 }
 
 constexpr int kWeightKeys = 512;   // keys of one CTA of the weights from kept logits
-constexpr int kMaxLogitRows = 16;
 
 template <int TYPE, int HD>
 __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, int merge_blocks) {

@@ -19,6 +19,8 @@
 
 namespace nb200 {
 
+constexpr int kMaxLogitRows = 64;   // query rows of a KV head up to which the weights may come from kept logits
+
 enum CacheType { kCacheI8 = 0, kCacheBF16 = 1, kCacheF16 = 2 };
 
 struct PrefixAttn {
@@ -84,10 +86,11 @@ bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
 // beside it, and has ended when it ends; joint: the own keys' units take the
 // prefix too (prefix_slots 0).
 bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint, bool after_tiles, cudaStream_t st);
-// Tile kernel for the sets whose split says `tiles`; cache_rows: extent of the
-// first axis of k and v.
-bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
-                         bool stream_next, cudaStream_t st);
+// Tile kernel for the sets whose split says `tiles`; joint: the own keys' units
+// take the prefix too (prefix_slots 0); cache_rows: extent of the first axis of k
+// and v; stream_next: the streaming kernel of the same call follows.
+bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, bool joint,
+                         long long cache_rows, bool stream_next, cudaStream_t st);
 // Weights of many rows from neg_lse (and, INT8, q16): group up to 128.
 bool launch_weight_tiles(const PrefixAttn &p, cudaStream_t st);
 // 1 if a bounded wait of the tile kernels ran out since the last call, -1 if

@@ -82,6 +82,7 @@ struct TileGrid {
     int own_units, own_tiles, own_ranges, own_alt, own_rows;          // rows of a unit
     int prefix_units, prefix_tiles, prefix_ranges, prefix_alt, prefix_rows;
     int stream_next;
+    int joint;                                                        // own units take the prefix first
     // whether the cache's head and sequence axes advance in the tensor maps
     int k_head, k_seq, v_head, v_seq, pk_head, pv_head;
 };
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
     int unit = blockIdx.x, g, m0, rows, lo, hi, slot, seq = -1, len = 0, nq = 0, alt;
     const float *ksc = nullptr, *vsc = nullptr;
     long long ksc_step = 0, vsc_step = 0;
-    int kz, kw, vz, vw;
+    int kz, kw, vz, vw, before = 0;                              // before: steps of the prefix ahead of [lo, hi)
     const CUtensorMap *km, *vm;
     if (unit < grid.own_units) {
         alt = grid.own_alt;
@@ -147,6 +148,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             ksc_step = p.kss[2];
             vsc_step = p.vss[2];
         }
+        if (grid.joint) before = ceil_div(p.prefix, kStep);
     } else {
         alt = grid.prefix_alt;
         unit -= grid.own_units;
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
     // the streaming kernel of the same call works on other keys: it may start beside this one
     if (grid.stream_next) pdl_launch_dependents();
     if (rows <= 0) return;                        // the whole CTA
-    const int n = ceil_div(max(0, hi - lo), kStep);              // steps of keys
+    const int n = before + ceil_div(max(0, hi - lo), kStep);     // steps of keys
     const int tiles = alt ? 1 : (rows > kTile ? 2 : 1);          // row tiles
     // item k: step and tile; its logits in buffer k % ahead, so that they follow the
     // output product of the item `ahead` before: one of its tile's last two, and the
@@ -220,8 +222,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             if (lane == 0) {
                 int issued = 0;
                 for (int i = 0; i < 2 * n; ++i) {
-                    const CUtensorMap *map = i & 1 ? vm : km;
-                    const int z = i & 1 ? vz : kz, w = i & 1 ? vw : kw, key = lo + (i >> 1) * kStep;
+                    const bool shared = (i >> 1) < before, v = i & 1;
+                    const CUtensorMap *map = shared ? (v ? &mpv : &mpk) : (v ? vm : km);
+                    const int key = shared ? (i >> 1) * kStep : lo + ((i >> 1) - before) * kStep;
+                    const int z = shared ? g * (v ? grid.pv_head : grid.pk_head) : (v ? vz : kz);
+                    const int w = shared ? 0 : (v ? vw : kw);
                     if constexpr (I8) {
                         const int s = i % G::kRaw;
                         if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             };
             auto have_v = [&](int j) {
                 if (!have(2 * j + 1)) return false;
-                const int valid = hi - lo - j * kStep;
+                const int valid = j < before ? p.prefix - j * kStep : hi - lo - (j - before) * kStep;
                 if (!I8 && valid < kStep) {               // rows behind the range: whatever they hold, zeros
                     char *v = ring + ((2 * j + 1) % kStages) * G::kKVBytes;
                     for (int i = valid * 8 + lane; i < kStep * 8; i += 32)
@@ -343,12 +348,19 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                         float kx[kStep / kN], vx[kStep / kN];
     #pragma unroll
                         for (int e = 0; e < kStep / kN; ++e) {
-                            const int key = lo + j * kStep + me + e * kN;
-                            kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
-                            vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
+                            const int x = me + e * kN;
+                            if (j < before) {
+                                const int key = j * kStep + x;
+                                kx[e] = key < p.prefix ? p.pkscale[g * p.pkss[0] + key * p.pkss[1]] : 0.f;
+                                vx[e] = key < p.prefix ? p.pvscale[g * p.pvss[0] + key * p.pvss[1]] : 0.f;
+                            } else {
+                                const int key = lo + (j - before) * kStep + x;
+                                kx[e] = key < hi ? ksc[key * ksc_step] : 0.f;
+                                vx[e] = key < hi ? vsc[key * vsc_step] : 0.f;
+                            }
                             most = fmaxf(most, fabsf(vx[e]));
                         }
-    #pragma unroll
+#pragma unroll
                         for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
                         if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
     #pragma unroll
@@ -446,7 +458,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             if (p.window) first = len - nq + t - p.window + 1;
         }
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s0 = tmem + 2 * HD + lanes, to = tmem + w * HD + lanes;
+        const uint32_t s0 = tmem + 2 * HD + lanes, ot = tmem + w * HD + lanes;
         float zs = p.scale2;
         if constexpr (I8) {
             wait_phase(&q_full, 0, abort_flag);
@@ -462,7 +474,9 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
         Turn turn;
         turn.on(w, ahead);
         for (int i = 0; i < mine; ++i, turn.on(each == 2 || alt ? 2 : 1, ahead)) {
-            const int j = alt ? 2 * i + w : i, j0 = lo + j * kStep;
+            const int j = alt ? 2 * i + w : i;
+            const int j0 = j < before ? j * kStep : lo + (j - before) * kStep;
+            const int from = j < before ? 0 : first, to = j < before ? p.prefix - 1 : last;   // keys the row sees
             ok = wait_phase(&s_full[turn.buffer], turn.phase, abort_flag);
             if (I8) {
                 const int v = 2 * j + 1;                  // (and the step's scales)
@@ -473,7 +487,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             const uint32_t ts = s0 + turn.buffer * kStep;
             const float *sk = scales + (j % G::kScaleRing) * 2 * kStep;
             // kRead logits of the row from column c on, INT8: times K's scales; -inf where not seen
-            const bool edge = j0 < first || j0 + kStep - 1 > last;
+            const bool edge = j0 < from || j0 + kStep - 1 > to;
             float2 z[kRead / 2];
             auto read = [&](int c) {
                 uint32_t raw[kRead / 32][32];
@@ -493,7 +507,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                     }
                 }
                 if (edge) {
-                    const int x0 = first - j0 - c, x1 = last - j0 - c;
+                    const int x0 = from - j0 - c, x1 = to - j0 - c;
 #pragma unroll
                     for (int e = 0; e < kRead / 2; ++e) {
                         if (2 * e < x0 || 2 * e > x1) z[e].x = kNegInf;
@@ -536,11 +550,11 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
-                    tc::ld32(to + c, o);
+                    tc::ld32(ot + c, o);
                     tc::wait_ld();
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                    tc::st32(to + c, o);
+                    tc::st32(ot + c, o);
                 }
             }
             const float base = top == kNegInf ? 0.f : -top;
@@ -603,7 +617,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 if (mine > 0) {
-                    tc::ld32(to + c, o);
+                    tc::ld32(ot + c, o);
                     tc::wait_ld();
                 }
                 float v[32];
@@ -1021,12 +1035,13 @@ int read_and_clear_tile_fault() {
     return v ? 1 : 0;
 }
 
-bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, long long cache_rows,
+bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, bool joint, long long cache_rows,
                          bool stream_next, cudaStream_t st) {
     auto run = [&](auto type, auto hd) -> bool {
         using G = TileGeom<type(), hd()>;
         TileGrid grid{};
         grid.stream_next = stream_next;
+        grid.joint = joint;
         const int rows = p.tokens * p.group;
         CUtensorMap mk{}, mv{}, mpk{}, mpv{};
         int unused;
@@ -1048,6 +1063,8 @@ bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const P
             grid.prefix_tiles = ceil_div(p.batch * rows, grid.prefix_rows);
             grid.prefix_ranges = prefix.ranges;
             grid.prefix_units = p.kvheads * grid.prefix_tiles * prefix.ranges;
+        }
+        if (prefix.tiles || joint) {
             if (!cache_map(&mpk, p.pk, type(), hd(), p.prefix, p.kvheads, 1, p.pks[1], p.pks[0], 0, &grid.pk_head,
                            &unused) ||
                 !cache_map(&mpv, p.pv, type(), hd(), p.prefix, p.kvheads, 1, p.pvs[1], p.pvs[0], 0, &grid.pv_head,
