@@ -64,6 +64,7 @@ __device__ __forceinline__ void cp4z(uint32_t dst, const void *src, bool valid) 
 
 constexpr int kWarps = 4;
 constexpr int kShortRange = 64;   // keys of a range that one warp takes by itself
+constexpr int kManyUnits = 2368;  // 16 a multiprocessor
 
 template <int TYPE, int HD>
 struct StreamGeom {
@@ -879,7 +880,8 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint
         const int span = p.window ? std::min<long long>(p.capacity, (long long)p.window + p.tokens) : p.capacity;
         const int longest = std::max(own ? ceil_div(span, grid.own_slots) + (joint ? p.prefix : 0) : 0,
                                      prefix ? ceil_div(p.prefix, grid.prefix_slots) : 0);
-        return longest <= kShortRange ? launch(std::integral_constant<int, 1>())
+        // one warp a unit on short ranges, and on longer ones where the units are many
+        return longest <= kShortRange || (longest <= 4 * kShortRange && units >= kManyUnits) ? launch(std::integral_constant<int, 1>())
                                       : launch(std::integral_constant<int, kWarps>());
     });
 }

@@ -266,8 +266,10 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                     for (int x = 0; x < G::kPieces; ++x)
 #pragma unroll
                         for (int c = 0; c < HD / 16; ++c)
+                            // (INT8: the small lo pieces first, the sum grows last)
                             tc::mma_bf16_ss(s0 + buffer * kStep,
-                                            desc_k(q + x * G::kQBytes + (c / 4) * (kTile * 128) + (c % 4) * 32),
+                                            desc_k(q + (G::kPieces - 1 - x) * G::kQBytes + (c / 4) * (kTile * 128) +
+                                                   (c % 4) * 32),
                                             desc_k(kt + (c / 4) * (kStep * 128) + (c % 4) * 32), ids, x + c > 0);
                     tc::commit(&s_full[buffer]);
                     if (each == 1 || w == 1) tc::commit(&empty[i % kStages]);
