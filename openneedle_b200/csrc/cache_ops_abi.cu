@@ -42,9 +42,9 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
     if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return refuse("prefix attention: scale must be positive and finite");
     const long long rows = (long long)a.batch * a.tokens;
     // units of work and row numbers are 32-bit
-    if (rows * a.heads > kMaxUnits / 64 || (long long)a.batch * a.kvheads > kMaxUnits / 64 ||
-        (long long)a.batch * a.kvheads * ((a.capacity + 63) / 64) > kMaxUnits || a.capacity > 0x7fffff00 ||
-        a.prefix > 0x7fffff00)
+    if (a.capacity > 0x7fffff00 || a.prefix > 0x7fffff00 || rows * a.heads > kMaxUnits / 4 ||
+        (long long)a.batch * a.kvheads > kMaxUnits / 64 ||
+        (long long)a.batch * a.kvheads * (((long long)a.capacity + 63) / 64) > kMaxUnits)
         return refuse("prefix attention: the call is too large");
     return true;
 }

@@ -80,6 +80,88 @@ def test_several_tokens(ops, cache, d, b, t, heads, kv, p, s, lengths, window):
 
 
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("d", (64, 128))
+@pytest.mark.parametrize("b,t,heads,kv,p,s,window", [
+    (20, 130, 8, 8, 200, 140, 0),                           # own row tiles that fill the machine take the prefix
+    (20, 130, 8, 8, 129, 300, 70),
+    (170, 90, 1, 1, 260, 100, 0),                           # ... both tiles of a CTA on the same rows
+    (3, 12, 40, 8, 30, 40, 0),                              # 60 rows: weights from kept logits
+    (2, 3, 130, 1, 20, 50, 0)])                             # more query heads a KV head than a tile has rows
+def test_many_rows(ops, cache, d, b, t, heads, kv, p, s, window):
+    """Larger calls, against the definition on the GPU in 64 bits with the bounds of cache_ops_reference."""
+    lengths = [t + (7 * i) % (s - t + 1) for i in range(b)]
+    c = R.make_inputs(cache, b, t, heads, kv, d, p, s, lengths, seed=t)
+    g = cuda(c)
+    r = heads // kv
+    wide = lambda x, sc: x.double() if sc is None else x.double() * sc.double().unsqueeze(-1)   # noqa: E731
+    k, v = wide(g["k"], g["k_scales"]), wide(g["v"], g["v_scales"])
+    pk = wide(g["prefix_k"], g["prefix_k_scales"]).expand(b, -1, -1, -1)
+    pv = wide(g["prefix_v"], g["prefix_v_scales"]).expand(b, -1, -1, -1)
+    k, v = torch.cat((pk, k), 2), torch.cat((pv, v), 2)
+    q = g["q"].double().view(b, t, kv, r, d).permute(0, 2, 1, 3, 4)                 # [B, KV, T, R, D]
+    at = (g["lengths"].view(b, 1) - t + torch.arange(t, device="cuda")).view(b, 1, t, 1, 1)
+    j = torch.arange(-p, s, device="cuda")
+    seen = (j < 0) | ((j <= at) & (j > at - window if window else j >= 0))
+    z = torch.einsum("bgtrd,bgkd->bgtrk", q, k) * d ** -0.5
+    z = z.masked_fill(~seen, -math.inf)
+    soft = torch.softmax(z, -1)
+    back = lambda x: x.permute(0, 2, 1, 3, *range(4, x.dim())).reshape(b, t, heads, *x.shape[4:]).cpu()   # noqa: E731
+    gained = soft[..., p:].sum((2, 3)).cpu()
+    count = seen.expand_as(z).sum(-1)
+    most = (127 * count * torch.cat((g["prefix_v_scales"].expand(b, -1, -1), g["v_scales"]), 2).abs().amax(-1)
+            .view(b, kv, 1, 1)).double() if cache == "int8" else torch.zeros_like(z[..., 0])
+    ref = {"out": back(torch.einsum("bgtrk,bgkd->bgtrd", soft, v)), "lse": back(torch.logsumexp(z, -1)),
+           "weights": c["weights"].double() + gained, "gained": gained,
+           "mix": back(torch.einsum("bgtrk,bgkd->bgtrd", soft, v.abs())), "most_v": back(most),
+           "total_v": back(torch.einsum("bgtrk,bgkd->bgtrd", seen.expand_as(z).double(), v.abs())),
+           "dz": back(torch.where(seen, torch.einsum("bgtrd,bgkd->bgtrk", q.abs(), k.abs()) * d ** -0.5,
+                                  torch.zeros_like(z)).amax(-1))}
+    bound = R.bounds(c, ref)
+    out, lse = call(ops, c, window=window)
+    R.check(out, ref["out"], bound["out"], "out")
+    R.check(lse, ref["lse"], bound["lse"], "lse")
+    out, weights = call(ops, c, weigh=True, window=window)
+    R.check(out, ref["out"], bound["out"], "out of accumulate_attention")
+    R.check(weights, ref["weights"], bound["weights"], "weights")
+
+
+@pytest.mark.parametrize("t", (1, 100))
+def test_offsets_beyond_32_bits(ops, t):
+    """The last keys of a cache of 34 million INT8 rows (2.2 GB), in a window."""
+    s, n = 34_000_000, 34_000_000 - 3
+    g = torch.Generator("cuda").manual_seed(1)
+    k = torch.zeros(1, 1, s, 64, dtype=torch.int8, device="cuda")
+    k[:, :, -400:] = torch.randint(-127, 128, (1, 1, 400, 64), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.full((1, 1, s), 0.01, device="cuda")
+    q = torch.randn(1, t, 2, 64, generator=g, device="cuda")
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    out, lse = ops.prefix_attention(q, k, k, lengths, k_scales=scales, v_scales=scales, window=64, return_lse=True)
+    tail = slice(s - 400, s)
+    near = {"k_scales": scales[:, :, tail].clone(), "v_scales": scales[:, :, tail].clone(), "window": 64,
+            "return_lse": True}
+    out2, lse2 = ops.prefix_attention(q, k[:, :, tail].clone(), k[:, :, tail].clone(), lengths - (s - 400), **near)
+    # the same keys from the front of a small cache: only the order of the sums may differ
+    assert (out - out2).abs().max() <= 1e-5 * out2.abs().max() and (lse - lse2).abs().max() <= 1e-5
+
+
+def test_lengths_are_clamped(ops):
+    c = R.make_inputs("bf16", 3, 1, 8, 4, 64, 20, 60, [60, 0, 60], seed=3)
+    want = call(ops, c) + call(ops, c, weigh=True)
+    c["lengths"] = torch.tensor([2 ** 31 - 1, -5, 61], dtype=torch.int32)
+    for x, y in zip(want, call(ops, c) + call(ops, c, weigh=True)):
+        assert torch.equal(x, y)
+    c = R.make_inputs("bf16", 2, 40, 8, 4, 64, 20, 60, [60, 60], seed=3)
+    want = call(ops, c)
+    got = call(ops, c, tokens=torch.tensor([1000, 40], dtype=torch.int32).cuda())
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    e = evict_inputs("bf16", 2, 2, 64, 50, [50, 0], seed=4)
+    first, _ = evicted(ops, e, 20, 1, 2)
+    e["lengths"] = torch.tensor([5000, -3], dtype=torch.int32)
+    for x, y in zip(first, evicted(ops, e, 20, 1, 2)[0]):
+        assert x is y is None or torch.equal(x, y)
+
+
+@pytest.mark.parametrize("cache", CACHES)
 def test_rows_that_see_nothing(ops, cache):
     c = R.make_inputs(cache, 3, 1, 8, 4, 64, 0, 16, [0, 5, 0])
     out, lse, weights = both(ops, c)
