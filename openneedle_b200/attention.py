@@ -495,8 +495,8 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     to the inputs themselves (``in_place``; lengths and indices are new), or to
     new tensors of ``keep`` slots, zero behind the kept keys."""
     lib, torch, types, raw_stream = _bind_operators()
-    key = (_layout(k), _layout(v), _layout(weights), _layout(lengths), _layout(k_scales), _layout(v_scales), keep, first,
-           recent, in_place, None if out is None else tuple(map(_layout, out)))
+    key = (_layout(k), _layout(v), _layout(weights), _layout(lengths), _layout(k_scales), _layout(v_scales), keep,
+           first, recent, in_place, None if out is None else tuple(map(_layout, out)))
     plan = _plans.get(key)
     if plan is None:
         plan = _remember(key, _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales,

@@ -30,7 +30,7 @@ bool rows_ok(const void *p, const long long *stride, std::initializer_list<int> 
     if (!p) return refuse((std::string(what) + " is null").c_str());
     bool ok = aligned16(p);
     for (int n : extent) ok = ok && (n <= 1 || (*stride * size) % 16 == 0), ++stride;
-    return ok ? true : refuse((std::string(what) + ": the pointer and the strides must be multiples of 16 bytes").c_str());
+    return ok || refuse((std::string(what) + ": the pointer and the strides must be multiples of 16 bytes").c_str());
 }
 
 bool sizes_ok(const needle2_prefix_attention_args &a) {
@@ -39,7 +39,8 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
     if (a.heads % a.kvheads) return refuse("prefix attention: heads must be a multiple of kvheads");
     if (a.head_dim != 64 && a.head_dim != 128) return refuse("prefix attention: head_dim must be 64 or 128");
     if (a.cache_type < 0 || a.cache_type > 2) return refuse("prefix attention: unknown cache type");
-    if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return refuse("prefix attention: scale must be positive and finite");
+    if (!(a.scale > 0.f) || !std::isfinite(a.scale))
+        return refuse("prefix attention: scale must be positive and finite");
     const long long rows = (long long)a.batch * a.tokens;
     // units of work and row numbers are 32-bit
     if (a.capacity > 0x7fffff00 || a.prefix > 0x7fffff00 || rows * a.heads > kMaxUnits / 4 ||
@@ -236,11 +237,18 @@ bool evict(const needle2_evict_args &a, cudaStream_t st) {
     const int size = a.cache_type == kCacheI8 ? 1 : 2;
     if (!a.lengths || !a.lengths_out || (a.keep && !a.indices)) return refuse("evict: null pointer");
     if (a.lengths == a.lengths_out) return refuse("evict: lengths_out must not be lengths");
-    if (a.capacity && (!rows_ok(a.k, a.k_stride, {a.batch, a.kvheads, a.capacity}, size, "k") || !rows_ok(a.v, a.v_stride, {a.batch, a.kvheads, a.capacity}, size, "v") || !a.weights))
-        return a.weights ? false : refuse("evict: weights is null");
-    if (a.out_capacity && (!rows_ok(a.k_out, a.k_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "k_out") ||
-                           !rows_ok(a.v_out, a.v_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "v_out") || !a.weights_out))
-        return a.weights_out ? false : refuse("evict: weights_out is null");
+    if (a.capacity) {
+        if (!rows_ok(a.k, a.k_stride, {a.batch, a.kvheads, a.capacity}, size, "k") ||
+            !rows_ok(a.v, a.v_stride, {a.batch, a.kvheads, a.capacity}, size, "v"))
+            return false;
+        if (!a.weights) return refuse("evict: weights is null");
+    }
+    if (a.out_capacity) {
+        if (!rows_ok(a.k_out, a.k_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "k_out") ||
+            !rows_ok(a.v_out, a.v_out_stride, {a.batch, a.kvheads, a.out_capacity}, size, "v_out"))
+            return false;
+        if (!a.weights_out) return refuse("evict: weights_out is null");
+    }
     const bool i8 = a.cache_type == kCacheI8;
     if (i8 && ((a.capacity && (!a.k_scales || !a.v_scales)) ||
                (a.out_capacity && (!a.k_scales_out || !a.v_scales_out))))

@@ -54,17 +54,28 @@ __device__ __forceinline__ void cp4z(uint32_t dst, const void *src, bool valid) 
 
 // ---- the streaming kernel --------------------------------------------------
 //
-// One CTA attends one tile of rows to one key range: 16 rows of a 16-bit cache
+// A unit attends one tile of rows to one key range: 16 rows of a 16-bit cache
 // (an m16n8k16 A operand), or 8 rows of an INT8 cache, whose FP32 queries and
 // softmax weights fill the 16 rows of A as FP16 pairs hi + lo (the codes
 // themselves are exact in FP16), so that INT8 costs no further products and
-// keeps FP32 accuracy.  Each of the four warps walks its own blocks of keys
-// (one pass, running maximum and sum), fed by its own ring of asynchronous
-// copies; the four states meet in shared memory at the end.
+// keeps FP32 accuracy.  Each warp of a unit walks its own blocks of keys (one
+// pass, running maximum and sum), fed by its own ring of asynchronous copies;
+// the states of a unit's warps meet in shared memory at the end.
+//
+// Bound by HBM where keys are long and many: 256 sessions of 3712 INT8 keys and 4
+// KV heads behind 384 shared ones (518 MB) 106 us, 4.9 TB/s, of the 79 us that a
+// copy of the bytes would take.  What is left is instructions: 64 % of the issue
+// slots, half of them on the integer pipe, which turns the codes into FP16 (three
+// of its instructions for four codes of K, eight for eight of V).  Two stages a
+// ring: three were slower (121 against 113 us), fewer CTAs fit.
 
 constexpr int kWarps = 4;
-constexpr int kShortRange = 64;   // keys of a range that one warp takes by itself
-constexpr int kManyUnits = 2368;  // 16 a multiprocessor
+// Keys of a range that one warp takes by itself (1024 sessions of 64 INT8 slots: 36 us
+// against 48 with four warps a unit; two sequences of 200 keys: 11 against 5.3), and
+// four times as many where the units are 16 a multiprocessor or more (1019 sessions
+// of 135 slots and 8 KV heads: 94 against 125 us).
+constexpr int kShortRange = 64;
+constexpr int kManyUnits = 2368;
 
 template <int TYPE, int HD>
 struct StreamGeom {
@@ -284,12 +295,11 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         const float *q = (const float *)qrow[0];
         float x[KS][4], most = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[k][e] = q[64 * (k / 4) + 16 * c + 4 * (k % 4) + e];
-                most = fmaxf(most, fabsf(x[k][e]));
-            }
+        for (int k = 0; k < KS; ++k) {
+            const float4 f = *(const float4 *)(q + 64 * (k / 4) + 16 * c + 4 * (k % 4));
+            x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
+            most = fmaxf(fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         float up, down;
@@ -386,7 +396,7 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         float best[kMine];
 #pragma unroll
         for (int e = 0; e < kMine; ++e) best[e] = kNegInf;
-        float vs[NT][2], vmax = 0.f;
+        float vs[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if constexpr (I8) {
@@ -394,7 +404,6 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
                 const float2 v2 = *(const float2 *)(stage + G::kSOff + 128 + (8 * n + 2 * c) * 4);
                 vs[n][0] = v2.x;
                 vs[n][1] = v2.y;
-                vmax = fmaxf(vmax, fmaxf(fabsf(v2.x), fabsf(v2.y)));
                 z[n][0] = (z[n][0] + z[n][2]) * (ks.x * qscale);
                 z[n][1] = (z[n][1] + z[n][3]) * (ks.y * qscale);
             } else {
@@ -440,9 +449,10 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
         // scale so far (a power of two), with 2^12 above FP16's small numbers
         float vinv = 1.f;
         if constexpr (I8) {
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-            vmax = __uint_as_float(__float_as_uint(fmaxf(vmax, 1e-30f)) & 0x7f800000u);
+            // (a scale a lane; sizes of floats order as their bits)
+            const uint32_t size = *(const uint32_t *)(stage + G::kSOff + 128 + lane * 4) & 0x7fffffffu;
+            const uint32_t most = __reduce_max_sync(0xffffffffu, size);
+            const float vmax = __uint_as_float(max(most, 0x0da24260u) & 0x7f800000u);   // at least 1e-30
             if (vmax > vnorm) {                              // the same in every lane
                 const float f = vnorm / vmax;
 #pragma unroll
@@ -602,7 +612,9 @@ __global__ __launch_bounds__(kWarps * 32, HD == 64 ? 4 : 3) void prefix_stream_k
 
 // ---- merge -----------------------------------------------------------------
 
-// HD / 4 threads a row: L over the row's partial results, then their weighted sum.
+// HD / 4 threads a row: the weighted sum of the row's partial results.  Bound by
+// their bytes, mostly out of L2: 4096 rows of 128 dimensions with 10 each (21 MB)
+// 5.8 us.
 template <int TYPE, int HD>
 __device__ __forceinline__ void merge_row(const PrefixAttn &p, long long row, int part) {
     constexpr bool I8 = TYPE == kCacheI8, BF = TYPE == kCacheBF16;
@@ -729,7 +741,10 @@ __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, 
 //
 // Keys are the rows of the product K Q^T: a warp holds 16 keys as the A operand
 // and walks the sequence's query rows, eight columns at a time, adding
-// 2^(z - L_row) of the rows that see the key.
+// 2^(z - L_row) of the rows that see the key.  Only for more query heads a KV head
+// than a tile of the tensor-core kernel has rows (it took 3200 us for two prompts
+// of 4096 tokens, the tiles take 182), and to copy the weights of calls without
+// tokens.
 
 template <int TYPE, int HD>
 __global__ __launch_bounds__(128) void key_weights_kernel(const PrefixAttn p) {
@@ -831,18 +846,6 @@ __global__ __launch_bounds__(128) void key_weights_kernel(const PrefixAttn p) {
     }
 }
 
-template <typename F>
-bool by_geometry(const PrefixAttn &p, F f) {
-    if (p.hd == 64) {
-        if (p.type == kCacheI8) return f(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 64>());
-        if (p.type == kCacheBF16) return f(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 64>());
-        return f(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 64>());
-    }
-    if (p.type == kCacheI8) return f(std::integral_constant<int, kCacheI8>(), std::integral_constant<int, 128>());
-    if (p.type == kCacheBF16) return f(std::integral_constant<int, kCacheBF16>(), std::integral_constant<int, 128>());
-    return f(std::integral_constant<int, kCacheF16>(), std::integral_constant<int, 128>());
-}
-
 }  // namespace
 
 bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint, bool after_tiles, cudaStream_t st) {
@@ -881,8 +884,8 @@ bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint
         const int longest = std::max(own ? ceil_div(span, grid.own_slots) + (joint ? p.prefix : 0) : 0,
                                      prefix ? ceil_div(p.prefix, grid.prefix_slots) : 0);
         // one warp a unit on short ranges, and on longer ones where the units are many
-        return longest <= kShortRange || (longest <= 4 * kShortRange && units >= kManyUnits) ? launch(std::integral_constant<int, 1>())
-                                      : launch(std::integral_constant<int, kWarps>());
+        const bool alone = longest <= kShortRange || (longest <= 4 * kShortRange && units >= kManyUnits);
+        return alone ? launch(std::integral_constant<int, 1>()) : launch(std::integral_constant<int, kWarps>());
     });
 }
 

@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace nb200 {
 
 constexpr int kMaxLogitRows = 64;   // query rows of a KV head up to which the weights may come from kept logits
@@ -66,6 +68,19 @@ __device__ __forceinline__ long long neg_lse_at(const PrefixAttn &p, int b, int 
 }
 __device__ __forceinline__ int own_tokens(const PrefixAttn &p, int b) {
     return p.ntokens ? max(0, min(p.ntokens[b], p.tokens)) : p.tokens;
+}
+
+// f of the cache type and the head dimension as compile-time constants.
+template <typename F>
+bool by_geometry(const PrefixAttn &p, F f) {
+    using I8 = std::integral_constant<int, kCacheI8>;
+    using BF = std::integral_constant<int, kCacheBF16>;
+    using F16 = std::integral_constant<int, kCacheF16>;
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (p.hd == 64)
+        return p.type == kCacheI8 ? f(I8(), D64()) : p.type == kCacheBF16 ? f(BF(), D64()) : f(F16(), D64());
+    return p.type == kCacheI8 ? f(I8(), D128()) : p.type == kCacheBF16 ? f(BF(), D128()) : f(F16(), D128());
 }
 
 // How one set of keys is attended: by the streaming kernel or by tiles, in how

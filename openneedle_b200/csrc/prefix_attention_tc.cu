@@ -12,10 +12,20 @@
 // maximum grew by more than 2^8, rescales its row of O.  While one tile is in its
 // softmax the tensor core works for the other.  TMEM holds the two tiles' O and
 // two (128 dimensions) or three (64) buffers of logits; with three, a tile's next
-// logits are computed during its softmax.  Steps of 64 keys with four buffers
-// were slower (480 against 345 us for two prompts of 4096 tokens): a product of
-// 64 columns takes nearly the time of one of 128.  Up to 128 rows run with both
-// tiles on the same rows and alternate key steps, as two key ranges.
+// logits are computed during its softmax.  Up to 128 rows run with both tiles on
+// the same rows and alternate key steps, as two key ranges.
+//
+// Two prompts of 4096 tokens, 32 heads, 128 dimensions, causal: 340 us, 810 TFLOP/s
+// (bf16).  A step of 128 keys takes about 3500 cycles: the products 2200 (a product
+// S of 128 columns 80 cycles an instruction rather than 64, as both operands come
+// from shared memory), a tile's softmax 1700, of which the exponentials 1000, and the
+// chain softmax - O - next logits leaves the tensor core idle in between, as TMEM has
+// no room for another buffer beside two O of 128 columns.  Steps of 64 keys with four
+// buffers took 480 us (a product of 64 columns takes nearly the time of one of 128),
+// four warpgroups of softmax 345, a part of the exponentials as polynomials on the
+// FP32 pipe 347 to 362.  Short calls pay about 9 us a CTA beside its steps: queries,
+// first copies, and the output (a 16k document asked about by 128 users: 47 us for
+// 15 steps).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -229,7 +239,8 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                     const int w = shared ? 0 : (v ? vw : kw);
                     if constexpr (I8) {
                         const int s = i % G::kRaw;
-                        if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag)) break;
+                        if (i >= G::kRaw && !wait_phase(&raw_empty[s], (uint32_t)(i / G::kRaw - 1) & 1, abort_flag))
+                            break;
                         mbar_arrive_expect_tx(&raw_full[s], G::kRawBytes);
                         tma_load_4d(smem + G::kRawAt + s * G::kRawBytes, map, 0, key, z, w, &raw_full[s]);
                     } else {
@@ -629,7 +640,8 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                 if (!direct) {
                     float4 *dst = (float4 *)(p.part_o + part * HD + c);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    for (int e = 0; e < 8; ++e)
+                        dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                 } else {
                     char *dst = (char *)p.out + (b * p.os[0] + t * p.os[1] + h * p.os[2] + c) * (I8 ? 4 : 2);
                     if constexpr (I8) {
@@ -1004,28 +1016,13 @@ bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long k
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r =
         fn(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims,
-           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("prefix attention: the cache's strides cannot be described to the copy engine");
         return false;
     }
     return true;
-}
-
-}  // namespace
-
-namespace {
-
-template <typename F>
-bool by_geometry(const PrefixAttn &p, F f) {
-    using I8 = std::integral_constant<int, kCacheI8>;
-    using BF = std::integral_constant<int, kCacheBF16>;
-    using F16 = std::integral_constant<int, kCacheF16>;
-    using D64 = std::integral_constant<int, 64>;
-    using D128 = std::integral_constant<int, 128>;
-    if (p.hd == 64) return p.type == kCacheI8 ? f(I8(), D64()) : p.type == kCacheBF16 ? f(BF(), D64()) : f(F16(), D64());
-    return p.type == kCacheI8 ? f(I8(), D128()) : p.type == kCacheBF16 ? f(BF(), D128()) : f(F16(), D128());
 }
 
 }  // namespace
@@ -1037,8 +1034,8 @@ int read_and_clear_tile_fault() {
     return v ? 1 : 0;
 }
 
-bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, bool joint, long long cache_rows,
-                         bool stream_next, cudaStream_t st) {
+bool launch_prefix_tiles(const PrefixAttn &p, const PrefixSplit &prefix, const PrefixSplit &own, bool joint,
+                         long long cache_rows, bool stream_next, cudaStream_t st) {
     auto run = [&](auto type, auto hd) -> bool {
         using G = TileGeom<type(), hd()>;
         TileGrid grid{};

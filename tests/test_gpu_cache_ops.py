@@ -380,7 +380,8 @@ def test_evict_into_strided_outputs(ops):
                       torch.zeros(2, 4, 150, dtype=torch.int32, device="cuda"), ks.transpose(1, 2), vs.transpose(1, 2))
     e = ops.evict(d["k"], d["v"], d["weights"], d["lengths"], 150, first=5, recent=10, k_scales=d["k_scales"],
                   v_scales=d["v_scales"], out=out)
-    behind = {"k": torch.full((2, 4, 200, 64), 9, dtype=torch.int8), "v": torch.full((2, 4, 200, 64), 9, dtype=torch.int8),
+    nines = torch.full((2, 4, 200, 64), 9, dtype=torch.int8)
+    behind = {"k": nines, "v": nines,
               "k_scales": torch.full((2, 4, 200), 9.0), "v_scales": torch.full((2, 4, 200), 9.0)}
     check_evicted(e, c, 150, 5, 10, behind=behind)
 
