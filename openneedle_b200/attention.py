@@ -264,28 +264,28 @@ def _want(x, name, shape, dtype, device, last=True):
         raise ValueError(f"{name}: the last axis must be contiguous")
 
 
-def _span(x):
-    """First and past-the-last byte that a tensor's elements take."""
-    size = x.nbytes
-    if not size:
-        return 0, 0
-    a = x.data_ptr()
-    if not x.is_contiguous():
-        size = (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
-    return a, a + size
+def _extent(x, name=None):
+    """The bytes from a tensor's first element to behind its last (0 for None); outputs, which are named, must not
+    be expanded."""
+    if x is None or not x.numel():
+        return 0
+    if x.is_contiguous():
+        return x.nbytes
+    if name and any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride())):
+        raise ValueError(f"{name} must not be expanded")
+    return (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
 
 
-def _apart(outs, inputs):
-    """Refuse outputs [(tensor, name)] that share memory with an input, with one another, or with themselves."""
-    taken = [_span(x) for x in inputs if x is not None]
-    for x, name in outs:
-        if not x.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride())):
-            raise ValueError(f"{name} must not be expanded")
-        a, b = _span(x)
-        for c, d in taken:
-            if a < d and c < b:
-                raise ValueError(f"{name} overlaps an input or another output")
-        taken.append((a, b))
+def _apart(outs, ins):
+    """Refuse outputs that share memory with an input or with one another; (tensor, bytes, name) and (tensor, bytes)."""
+    spans = sorted([(x.data_ptr(), n, name) for x, n, name in outs if n] + [(x.data_ptr(), n, "") for x, n in ins if n])
+    end = end_out = 0                                      # of all spans, of the outputs' so far
+    for start, n, name in spans:
+        if start < (end if name else end_out):
+            raise ValueError(f"{name or 'an output'} overlaps an input or another output")
+        end = max(end, start + n)
+        if name:
+            end_out = max(end_out, start + n)
 
 
 def _no_gradients(torch, *tensors):
@@ -334,7 +334,7 @@ def _remember(key, plan):
 
 def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales,
                     prefix_k_scales, prefix_v_scales, tokens, window, scale, out):
-    """Check a call; its packed sizes, its workspace's bytes, its result's type."""
+    """Check a call; its packed sizes, its workspace's bytes and what follows from its shapes."""
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
@@ -391,7 +391,12 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
     size = lib.needle2_prefix_attention_workspace(sizes + _ATTENTION_POINTERS.pack(*[4096] * 14, one, one))
     if size < 0:
         raise ValueError(last_error())
-    return sizes, size, (batch, count, heads), weigh
+    extents = None
+    if out is not None or weights_out is not None:
+        extents = ([_extent(out, "out"), _extent(weights_out, "weights_out")],
+                   [_extent(x) for x in (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales,
+                                         prefix_k_scales, prefix_v_scales, weights)])
+    return sizes, size, (batch, count, heads), weigh, extents
 
 
 def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
@@ -405,17 +410,16 @@ def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales
         plan = _remember(key, _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, prefix_k,
                                               prefix_v, k_scales, v_scales, prefix_k_scales, prefix_v_scales, tokens,
                                               window, scale, out))
-    sizes, size, rows, weigh = plan
+    sizes, size, rows, weigh, extents = plan
     _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights)
     device = k.device
-    if out is not None or weights_out is not None:
+    if extents is not None:
         same = weights_out is not None and weights_out.data_ptr() == weights.data_ptr() and \
             weights_out.stride() == weights.stride()
-        outs = [] if out is None else [(out, "out")]
-        if weights_out is not None:
-            outs.append((weights_out, "weights_out"))
-        _apart(outs, (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales,
-                      prefix_v_scales, None if same else weights))
+        (n_out, n_weights), n_in = extents
+        _apart([(out, n_out, "out"), (weights_out, n_weights, "weights_out")],
+               zip((q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales, prefix_k_scales, prefix_v_scales,
+                    weights), n_in[:-1] if same else n_in))
     context = _on_stream(torch, device, stream)
     if context is not None:
         with context:
@@ -501,7 +505,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     if plan is None:
         plan = _remember(key, _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales,
                                           out, in_place))
-    sizes, shape = plan
+    sizes, shape, (n_out, n_in) = plan
     _no_gradients(torch, k, v, weights)
     device = k.device
     context = _on_stream(torch, device, stream)
@@ -510,7 +514,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
             return evict(k, v, weights, lengths, keep, first=first, recent=recent, k_scales=k_scales, v_scales=v_scales,
                          out=out, in_place=in_place)
     if in_place:
-        _apart([(x, "the cache") for x in (k, v, weights, k_scales, v_scales) if x is not None], (lengths,))
+        _apart([(x, n, "the cache") for x, n in zip((k, v, weights, k_scales, v_scales), n_out)], [(lengths, n_in[0])])
         out = Evicted(k, v, weights, torch.empty(shape[:1], dtype=torch.int32, device=device),
                       torch.empty(shape, dtype=torch.int32, device=device), k_scales, v_scales)
     elif out is None:
@@ -523,7 +527,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
                       None if v_scales is None else torch.zeros(shape, **f32))
     else:
         out = Evicted(*out)
-        _apart([(x, "out") for x in out if x is not None], (k, v, weights, lengths, k_scales, v_scales))
+        _apart([(x, n, "out") for x, n in zip(out, n_out)], zip((k, v, weights, lengths, k_scales, v_scales), n_in))
     args = sizes + _EVICT_POINTERS.pack(
         k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales), weights.data_ptr(), lengths.data_ptr(),
         out.k.data_ptr(), out.v.data_ptr(), _pointer(out.k_scales), _pointer(out.v_scales), out.weights.data_ptr(),
@@ -534,7 +538,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
 
 
 def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales, out, in_place):
-    """Check an eviction; its packed sizes and [batch, kvheads, keep]."""
+    """Check an eviction; its packed sizes, [batch, kvheads, keep], and the tensors' extents in bytes."""
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
@@ -567,5 +571,11 @@ def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_sca
         if not out.indices.is_contiguous() or not out.lengths.is_contiguous():
             raise ValueError("out.indices and out.lengths must be contiguous")
         to = _strides(3, out.k, out.v, out.k_scales, out.v_scales, out.weights)
+    extents = [], []
+    if in_place:
+        extents = [_extent(x, "the cache") for x in (k, v, weights, k_scales, v_scales)], [_extent(lengths)]
+    elif out is not None:
+        extents = ([_extent(x, "out") for x in out],
+                   [_extent(x) for x in (k, v, weights, lengths, k_scales, v_scales)])
     return _EVICT_SIZES.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
-                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep)
+                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep), extents

@@ -694,10 +694,18 @@ __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, 
                 l = -p.neg_lse[neg_lse_at(p, b, t, h)];
             } else {
                 float top = kNegInf, total = 0.f;
-                for (int i = 0; i < slots; ++i) top = fmaxf(top, p.part_lse[i * nrows + row]);
-                const float t0 = top == kNegInf ? 0.f : top;
-                for (int i = 0; i < slots; ++i) total += ex2(p.part_lse[i * nrows + row] - t0);
-                l = total == 0.f ? 0.f : t0 + log2f(total);
+                for (int i = 0; i < slots; i += 4) {       // four in flight at a time
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = i + e < slots ? p.part_lse[(i + e) * nrows + row] : kNegInf;
+                    const float now = fmaxf(max3(top, x[0], x[1]), fmaxf(x[2], x[3]));
+                    const float base = now == kNegInf ? 0.f : now;
+                    total *= ex2(top - base);
+                    top = now;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) total += ex2(x[e] - base);
+                }
+                l = total == 0.f ? 0.f : (top == kNegInf ? 0.f : top) + log2f(total);
             }
             if (l == kNegInf) l = 0.f;
         }
