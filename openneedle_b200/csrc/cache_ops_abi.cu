@@ -136,7 +136,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.q16_at = take(rows * a.head_dim * 4);
         p.q16_scale_at = take(rows * 4);
     }
-    p.bytes = at;
+    p.bytes = n > 1 ? at + 16 : at;              // partial rows lie on 32 bytes, the workspace on 16
     return p;
 }
 
@@ -196,6 +196,7 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
     char *base = static_cast<char *>(workspace);
     const int n = p.own_slots + p.prefix_slots;
     if (n > 1) {
+        base += reinterpret_cast<uintptr_t>(base) % 32;
         p.part_o = reinterpret_cast<float *>(base + plan.part_o);
         p.part_lse = reinterpret_cast<float *>(base + plan.part_lse);
     }

@@ -510,6 +510,48 @@ def test_prefill_evict_decode(ops, cache):
         c["weights"] = w.cpu()
 
 
+@pytest.mark.parametrize("cache", CACHES)
+def test_workspace_on_sixteen_bytes(ops, monkeypatch, cache):
+    """A workspace that starts on an odd multiple of 16 bytes: nothing outside it is written."""
+    c = R.make_inputs(cache, 40, 1, 8, 4, 64, 600, 300, [(11 * i) % 301 for i in range(40)], seed=51)
+    plain = call(ops, c) + call(ops, c, weigh=True)
+    empty, around = torch.empty, []
+
+    def shifted(*size, **more):
+        if more.get("dtype") != torch.uint8:
+            return empty(*size, **more)
+        around.append(torch.full((size[0] + 64,), 77, **more))
+        return around[-1][16:16 + size[0]]
+
+    monkeypatch.setattr(torch, "empty", shifted)
+    got = call(ops, c) + call(ops, c, weigh=True)
+    assert len(around) == 2
+    for x, y in zip(got, plain):
+        assert torch.equal(x, y)
+    for x in around:
+        assert x.data_ptr() % 32 == 0 and bool((x[:16] == 77).all()) and bool((x[-48:] == 77).all())
+
+
+@pytest.mark.parametrize("d", (64, 128))
+def test_long_sums_keep_their_bits(ops, d):
+    """Equal weights over 16000 INT8 keys of one sign: the means, where each sum that is cut and not rounded
+    shows. Products: 3 steps of 16 sums, 2^-23 each; weights as pairs: 2^-21; the sums of the steps, of the
+    weights and the rest: 150 roundings of 2^-24. Together 2^-16."""
+    g = torch.Generator().manual_seed(d)
+    b, t, heads, kv, keys = 4, 600, 16, 4, 16000
+    v = torch.randint(1, 128, (kv, keys, d), generator=g, dtype=torch.int8)
+    scales = torch.rand(kv, keys, generator=g) + 0.5
+    mean = (v.double() * scales.double()[..., None]).mean(1)
+    none = torch.zeros(b, kv, 8, d, dtype=torch.int8, device="cuda")
+    out = ops.prefix_attention(torch.zeros(b, t, heads, d, device="cuda"), none, none,
+                               torch.zeros(b, dtype=torch.int32, device="cuda"), prefix_k=v.cuda(), prefix_v=v.cuda(),
+                               k_scales=none[..., 0].float(), v_scales=none[..., 0].float(),
+                               prefix_k_scales=scales.cuda(), prefix_v_scales=scales.cuda())
+    want = mean.repeat_interleave(heads // kv, 0)
+    off = (out.double().cpu() - want).abs() / want
+    assert float(off.max()) <= 2.0 ** -16, float(off.max())
+
+
 @pytest.mark.parametrize("t", (1, 40))
 def test_streams_and_graphs(ops, t):
     """Calls on a side stream, and two captured graphs replayed in turn with new inputs: each keeps its own
