@@ -72,22 +72,28 @@ int sm_count() {
 Plan plan_of(const needle2_prefix_attention_args &a) {
     Plan p{};
     const int sms = sm_count();
-    const int R = a.heads / a.kvheads, tile = a.cache_type == kCacheI8 ? 8 : 16;
+    const bool i8 = a.cache_type == kCacheI8;
+    const int R = a.heads / a.kvheads, tile = i8 ? 8 : 16;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
+    // Keys of a tile CTA: its products cut their sums to 24 bits towards zero, eight times
+    // 128 keys, by up to 2^-23 and 2^-25 on the average. So many keys stay within half a
+    // step of FP16.  (INT8's sums leave the accumulator long before.)
+    const long long kTileKeys = i8 ? 1LL << 40 : 32768;
     // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys.
     // Tiles or streaming by their times, fitted to measurements (us): a tile CTA has its
     // multiprocessor to itself and takes 9 beside 0.9 for 128 keys of one tile (1.8 of
     // two), a streaming unit 1.2 of one beside its keys, of which the 16-bit caches'
     // 128 dimensions take longest.  (358 sequences of 16 rows and 88 INT8 keys: 500 by
     // tiles, 100 streaming; two prompts of 4096 tokens: 5100 streaming, 340 by tiles.)
-    const double key = (a.cache_type == kCacheI8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
+    const double key = (i8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
     auto split = [&](long long groups, long long group_rows, long long keys) {
         PrefixSplit s, t;
         t.tiles = true;
-        t.alt = group_rows <= 128 || (a.cache_type == kCacheI8 && a.head_dim == 128);
+        t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
         const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
         const long long most = (keys + (t.alt ? 511 : 255)) / (t.alt ? 512 : 256);
-        t.ranges = (int)std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL}));
+        t.ranges = (int)std::max((keys + kTileKeys - 1) / kTileKeys,
+                                 std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL})));
         const long long units = groups * ((group_rows + tile - 1) / tile);
         const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
         s.ranges = (int)std::max(1LL, std::min({want, (keys + 255) / 256, 64LL}));
@@ -109,6 +115,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     // tiles of the sequences' own rows that fill the machine take the prefix first, in
     // the same accumulators: no partial results
     p.joint_tiles = a.prefix && p.own.tiles && p.prefix.tiles && p.own.ranges == 1 &&
+                    (i8 || a.prefix + (long long)span <= kTileKeys) &&
                     (long long)a.batch * a.kvheads * ((a.tokens * R + 255) / 256) * 5 >= 4LL * sms;
     if (p.joint_tiles) p.prefix = PrefixSplit{};
     if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros

@@ -74,9 +74,10 @@ struct TileGeom {
     static constexpr int kConverters = I8 ? 2 : 0;                // warps
     // A product's sums are cut to 24 bits towards zero, 16 times a step for the pairs: O
     // shrinks by up to 2^-19 a step. So after every kHold steps it is added to sums that the
-    // row's thread holds, and starts at zero. 16000 shared keys, 1200 tokens, 64 / 128
-    // dimensions: error 9e-6 / 14e-6 in 183 / 459 us without, 1.2e-6 in 188 / 494 with 4
-    // steps, 0.8e-6 in 194 / 536 with 2 (elementary operations in 32 bits: 2.4e-6)
+    // row's thread holds (in local memory), and starts at zero. 16000 shared keys, 1200
+    // tokens, 64 / 128 dimensions: 9e-6 / 14e-6 off in 183 / 459 us without, 0.8e-6 / 1.0e-6
+    // in 174 / 452 so (elementary operations in 32 bits: 2.4e-6); 2 steps for 128
+    // dimensions: 0.8e-6 in 471. 16-bit outputs need it only after many more keys: ranges.
     static constexpr int kHold = HD == 64 ? 2 : 3;
     static_assert(kSmem <= 232448 - 4096, "shared memory of a CTA");
     // a step's scales are written when the stage of the K kStages / 2 steps before is
@@ -494,7 +495,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
         float top = kNegInf, sum = 0.f, vnorm = 0.f;
         // INT8: O leaves for these sums every kHold steps, held * hold + O is the whole
         // (see kHold)
-        float held[I8 ? HD : 1], hold = 0.f;
+        float held[HD], hold = 0.f;
         bool ok = true;
         Turn turn;
         turn.on(w, ahead);
@@ -573,24 +574,31 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                 // ones before that had ended when these logits were computed)
                 ok = wait_phase(&o_done[w], (uint32_t)(i - 1) & 1, abort_flag);
                 tc::fence_after();
-                if constexpr (I8) hold *= keep;
+                hold *= keep;
+                if (leave) {
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tc::ld32(ot + c, o);
+                        tc::wait_ld();
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t o[32];
-                    tc::ld32(ot + c, o);
-                    tc::wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float x = __uint_as_float(o[e]) * keep;
-                        if constexpr (I8) {
-                            if (leave) {
-                                held[c + e] = hold == 0.f ? x : fmaf(held[c + e], hold, x);
-                                x = 0.f;
-                            }
+                        for (int e = 0; e < 32; ++e) {
+                            const float x = __uint_as_float(o[e]) * keep;
+                            held[c + e] = hold == 0.f ? x : fmaf(held[c + e], hold, x);
+                            o[e] = 0;
                         }
-                        o[e] = __float_as_uint(x);
+                        tc::st32(ot + c, o);
                     }
-                    tc::st32(ot + c, o);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tc::ld32(ot + c, o);
+                        tc::wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tc::st32(ot + c, o);
+                    }
                 }
                 if (I8 && leave) hold = 1.f;
             }

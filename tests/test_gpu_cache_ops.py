@@ -552,6 +552,30 @@ def test_long_sums_keep_their_bits(ops, d):
     assert float(off.max()) <= 2.0 ** -16, float(off.max())
 
 
+@pytest.mark.parametrize("d", (64, 128))
+@pytest.mark.parametrize("shared", (True, False))
+def test_long_sums_in_sixteen_bits(ops, d, shared):
+    """The same with 100000 FP16 keys, shared or own: cut sums 8 for 128 keys, 2^-25 each on the average, over at
+    most 32768 keys: 2^-14; the output's rounding: 2^-11. Together 2^-10.8."""
+    g = torch.Generator().manual_seed(d)
+    b, t, heads, kv, keys = 2, 1200, 16, 4, 100000
+    v = (torch.rand(b, kv, keys, d, generator=g) + 0.5).half()
+    mean = v.double().mean(2)
+    v = v.cuda()
+    none = torch.zeros(b, kv, 8, d, dtype=torch.float16, device="cuda")
+    q = torch.zeros(b, t, heads, d, dtype=torch.float16, device="cuda")
+    lengths = torch.zeros(b, dtype=torch.int32, device="cuda")
+    if shared:
+        out = ops.prefix_attention(q, none, none, lengths, prefix_k=v[0], prefix_v=v[0])
+        want = mean[:1].expand(b, kv, d)
+    else:
+        out = ops.prefix_attention(q, v, v, lengths + keys)[:, -1:]
+        want = mean
+    want = want.repeat_interleave(heads // kv, 1)[:, None]
+    off = (out.double().cpu() - want).abs() / want
+    assert float(off.max()) <= 2.0 ** -10.8, float(off.max())
+
+
 @pytest.mark.parametrize("t", (1, 40))
 def test_streams_and_graphs(ops, t):
     """Calls on a side stream, and two captured graphs replayed in turn with new inputs: each keeps its own
