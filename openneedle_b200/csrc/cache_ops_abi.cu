@@ -75,10 +75,11 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     const bool i8 = a.cache_type == kCacheI8;
     const int R = a.heads / a.kvheads, tile = i8 ? 8 : 16;
     const long long rows = (long long)a.batch * a.tokens * a.heads;
-    // Keys of a tile CTA: its products cut their sums to 24 bits towards zero, eight times
-    // 128 keys, by up to 2^-23 and 2^-25 on the average. So many keys stay within half a
-    // step of FP16.  (INT8's sums leave the accumulator long before.)
-    const long long kTileKeys = i8 ? 1LL << 40 : 32768;
+    // Keys of a range: products cut their sums to 24 bits towards zero, 16-bit caches' eight
+    // times 128 keys, INT8's 16 times, by 2^-25 of the end's on the average. So many keys
+    // stay well within half a step of FP16, and INT8's streaming within 2^-16 (65536 keys
+    // of one sign in a range: 2^-13.6); its tiles' sums leave the accumulator long before.
+    const long long tile_keys = i8 ? 1LL << 40 : 32768, stream_keys = i8 ? 4096 : 1 << 18;
     // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys.
     // Tiles or streaming by their times, fitted to measurements (us): a tile CTA has its
     // multiprocessor to itself and takes 9 beside 0.9 for 128 keys of one tile (1.8 of
@@ -92,11 +93,12 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
         const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
         const long long most = (keys + (t.alt ? 511 : 255)) / (t.alt ? 512 : 256);
-        t.ranges = (int)std::max((keys + kTileKeys - 1) / kTileKeys,
+        t.ranges = (int)std::max((keys + tile_keys - 1) / tile_keys,
                                  std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL})));
         const long long units = groups * ((group_rows + tile - 1) / tile);
         const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
-        s.ranges = (int)std::max(1LL, std::min({want, (keys + 255) / 256, 64LL}));
+        s.ranges = (int)std::max((keys + stream_keys - 1) / stream_keys,
+                                 std::max(1LL, std::min({want, (keys + 255) / 256, 64LL})));
         if (group_rows <= tile) return s;
         const double waves = std::max(1.0, (double)tiles * t.ranges / sms);
         const double by_tiles = waves * (9.0 + (t.alt ? 7e-3 : 14e-3) * (double)keys / t.ranges);
@@ -115,7 +117,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     // tiles of the sequences' own rows that fill the machine take the prefix first, in
     // the same accumulators: no partial results
     p.joint_tiles = a.prefix && p.own.tiles && p.prefix.tiles && p.own.ranges == 1 &&
-                    (i8 || a.prefix + (long long)span <= kTileKeys) &&
+                    (i8 || a.prefix + (long long)span <= tile_keys) &&
                     (long long)a.batch * a.kvheads * ((a.tokens * R + 255) / 256) * 5 >= 4LL * sms;
     if (p.joint_tiles) p.prefix = PrefixSplit{};
     if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros

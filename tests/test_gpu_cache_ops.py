@@ -553,6 +553,23 @@ def test_long_sums_keep_their_bits(ops, d):
 
 
 @pytest.mark.parametrize("d", (64, 128))
+def test_long_sums_of_single_tokens(ops, d):
+    """The same for single tokens of sequences that fill the machine: 512 cut sums of pairs in 4096 keys, 2^-25
+    each on the average (2^-16), and as much again for the merge and the rest."""
+    b, kv, keys = 150, 4, 40000
+    g = torch.Generator(device="cuda").manual_seed(d)
+    v = torch.randint(1, 128, (b, kv, keys, d), generator=g, dtype=torch.int8, device="cuda")
+    scales = torch.rand(b, kv, keys, generator=g, device="cuda") + 0.5
+    out = ops.prefix_attention(torch.zeros(b, kv, d, device="cuda"), v, v,
+                               torch.full((b,), keys, dtype=torch.int32, device="cuda"), k_scales=scales,
+                               v_scales=scales)
+    for i in (0, 70, 149):
+        want = (v[i].double() * scales[i].double()[..., None]).mean(1)
+        off = (out[i].double() - want).abs() / want
+        assert float(off.max()) <= 2.0 ** -15, float(off.max())
+
+
+@pytest.mark.parametrize("d", (64, 128))
 @pytest.mark.parametrize("shared", (True, False))
 def test_long_sums_in_sixteen_bits(ops, d, shared):
     """The same with 100000 FP16 keys, shared or own: cut sums 8 for 128 keys, 2^-25 each on the average, over at
