@@ -51,13 +51,19 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
 }
 
 constexpr int kJointKeys = 512;
-constexpr long long kMaxLogits = 1LL << 26;   // kept for the weights
+constexpr long long kMaxLogits = 1LL << 27;   // kept for the weights
 
 struct Plan {
     PrefixSplit prefix, own;
     bool joint, joint_tiles, logits, neg_lse, weight_tiles;
     long long part_o, part_lse, neg_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
+
+// Whether the weights may come from the logits that the streaming kernel keeps.
+bool keeps_logits(const needle2_prefix_attention_args &a) {
+    return a.tokens > 0 && (long long)a.tokens * (a.heads / a.kvheads) <= kMaxLogitRows &&
+           (long long)a.batch * a.tokens * a.heads * a.capacity <= kMaxLogits;
+}
 
 int sm_count() {
     static int count[64] = {};
@@ -82,12 +88,15 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     const long long tile_keys = i8 ? 1LL << 40 : 32768, stream_keys = i8 ? 4096 : 1 << 18;
     // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys.
     // Tiles or streaming by their times, fitted to measurements (us): a tile CTA has its
-    // multiprocessor to itself and takes 9 beside 0.9 for 128 keys of one tile (1.8 of
-    // two), a streaming unit 1.2 of one beside its keys, of which the 16-bit caches'
-    // 128 dimensions take longest.  (358 sequences of 16 rows and 88 INT8 keys: 500 by
-    // tiles, 100 streaming; two prompts of 4096 tokens: 5100 streaming, 340 by tiles.)
+    // multiprocessor to itself and takes 9 beside its keys, whose conversion INT8 waits for,
+    // a streaming unit 1.2 beside its keys, of which the 16-bit caches' 128 dimensions take
+    // longest.  (358 sequences of 16 rows and 88 INT8 keys: 500 by tiles, 100 streaming; 600
+    // KV heads x 24 FP16 rows x 3436 keys: 212, 174; 800 x 10 INT8 rows x 2000: 404, 197;
+    // two prompts of 4096 tokens: 340, 5100.)
+    // Weights of the own keys: behind tiles a CTA of 256 keys takes the product again;
+    // streaming keeps the logits of few rows.  (600 x 24 rows x 3436: 319 and 58.)
     const double key = (i8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
-    auto split = [&](long long groups, long long group_rows, long long keys) {
+    auto split = [&](long long groups, long long group_rows, long long keys, bool weights) {
         PrefixSplit s, t;
         t.tiles = true;
         t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
@@ -101,13 +110,22 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
                                  std::max(1LL, std::min({want, (keys + 255) / 256, 64LL})));
         if (group_rows <= tile) return s;
         const double waves = std::max(1.0, (double)tiles * t.ranges / sms);
-        const double by_tiles = waves * (9.0 + (t.alt ? 7e-3 : 14e-3) * (double)keys / t.ranges);
-        const double streaming = 4.0 + units * (1.2 + key * (double)keys) / sms;
+        const double tile_key =
+            i8 ? (a.head_dim == 128 ? 33e-3 : 29e-3) : (t.alt ? 11e-3 : 14.5e-3) * (a.head_dim == 128 ? 1.3 : 1.0);
+        double by_tiles = waves * (9.0 + tile_key * (double)keys / t.ranges);
+        double streaming = 4.0 + units * (1.2 + key * (double)keys) / sms;
+        if (weights) {
+            const double ctas = std::max(1.0, (double)groups * ((a.capacity + 255) / 256) / sms);
+            const double again = 5.0 + ctas * (a.head_dim == 128 ? 7.5 : 5.7);
+            by_tiles += again;
+            streaming += keeps_logits(a) ? 3.0 + std::max(0.3 * group_rows, groups * group_rows * 1.1e-6 * a.capacity)
+                                         : again;
+        }
         return by_tiles < streaming ? t : s;
     };
     const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
-    if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span);
-    if (a.prefix) p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix);
+    if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span, a.weights != nullptr);
+    if (a.prefix) p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix, false);
     // few rows and keys: one kernel whose units take both key sets one after the other
     p.joint = a.prefix && a.capacity && !p.own.tiles && !p.prefix.tiles && a.prefix + (long long)span <= kJointKeys;
     if (p.joint) {
@@ -124,8 +142,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.own = PrefixSplit{};
         p.own.ranges = 1;
     }
-    p.logits = a.weights && a.tokens > 0 && !p.own.tiles && a.tokens * R <= kMaxLogitRows &&
-               (long long)a.batch * a.kvheads * a.tokens * R * a.capacity <= kMaxLogits;
+    p.logits = a.weights && !p.own.tiles && keeps_logits(a);
     p.neg_lse = a.weights != nullptr;
     p.weight_tiles = a.weights && !p.logits && a.tokens > 0 && R <= 128;
     long long at = 0;
