@@ -330,10 +330,12 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
     if (p.logits && seq >= 0)
         logits = p.logits + ((long long)(seq * p.kvheads + g) * TR + (m0 - seq * TR)) * p.capacity;
 
+    bool then_prefix = seq >= 0 && grid.joint;
     for (int i = 0;; ++i) {
         if (i == mine) {
-            if (seq < 0 || !grid.joint || s.k == (const char *)p.pk + g * p.pks[0] * G::kSize) break;
+            if (!then_prefix) break;
             // then the prefix, on the same state; every query sees all of it
+            then_prefix = false;
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
             s = prefix_set<TYPE, HD>(p, g);

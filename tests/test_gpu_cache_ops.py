@@ -636,3 +636,22 @@ def test_streams_and_graphs(ops, t):
             assert torch.equal(results[i][0], plain[j][0]) and torch.equal(results[i][1], plain[j][1])
             for x, y in zip(results[i][2], eager[j]):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("t,s", [(1, 30), (1, 64), (3, 300), (40, 64)])
+def test_prefix_that_is_a_view_of_the_cache(ops, cache, t, s):
+    """The shared prompt kept in the first slots of sequence 0: its prefix and its own keys start at one address.
+    Prefixes in a pass with the own keys (one and four warps a unit) and apart; the same as with copies."""
+    c = R.make_inputs(cache, 3, t, 8, 4, 64, 0, s, [0 if t == 1 else s, s // 2 + 1, s], seed=60 + t)
+    d = cuda(c)
+    scales = {n: d[n] for n in ("k_scales", "v_scales")}
+
+    def run(change):
+        prefix = {"prefix_" + n: None if d[n] is None else change(d[n][0, :, :20]) for n in ("k", "v", *scales)}
+        out, lse = ops.prefix_attention(d["q"], d["k"], d["v"], d["lengths"], return_lse=True, **scales, **prefix)
+        return (out, lse) + ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], **scales,
+                                                     **prefix)
+
+    for x, y in zip(run(lambda x: x), run(lambda x: x.clone())):
+        assert torch.equal(x, y)
