@@ -65,6 +65,18 @@ bool keeps_logits(const needle2_prefix_attention_args &a) {
            (long long)a.batch * a.tokens * a.heads * a.capacity <= kMaxLogits;
 }
 
+// The copy engine's maps take strides above zero and below 2^40 bytes; an axis of heads
+// or sequences may also stand still (the maps leave it out). Keys of other strides (one
+// row expanded along the axis) are streamed, whose loads take any address.
+bool can_map(long long stride, long long n, int size) {
+    return n <= 1 || (stride > 0 && stride < (1LL << 40) / size);
+}
+bool can_map_cache(long long key, long long keys, long long head, long long heads, long long seq, long long seqs,
+                   int size) {
+    return can_map(key, keys, size) && (head == 0 || can_map(head, heads, size)) &&
+           (seq == 0 || can_map(seq, seqs, size));
+}
+
 int sm_count() {
     static int count[64] = {};
     int dev = 0;
@@ -96,7 +108,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     // Weights of the own keys: behind tiles a CTA of 256 keys takes the product again;
     // streaming keeps the logits of few rows.  (600 x 24 rows x 3436: 319 and 58.)
     const double key = (i8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
-    auto split = [&](long long groups, long long group_rows, long long keys, bool weights) {
+    auto split = [&](long long groups, long long group_rows, long long keys, bool weights, bool mapped) {
         PrefixSplit s, t;
         t.tiles = true;
         t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
@@ -108,7 +120,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
         s.ranges = (int)std::max((keys + stream_keys - 1) / stream_keys,
                                  std::max(1LL, std::min({want, (keys + 255) / 256, 64LL})));
-        if (group_rows <= tile) return s;
+        if (group_rows <= tile || !mapped) return s;
         const double waves = std::max(1.0, (double)tiles * t.ranges / sms);
         const double tile_key =
             i8 ? (a.head_dim == 128 ? 33e-3 : 29e-3) : (t.alt ? 11e-3 : 14.5e-3) * (a.head_dim == 128 ? 1.3 : 1.0);
@@ -124,8 +136,20 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         return by_tiles < streaming ? t : s;
     };
     const int span = a.window ? (int)std::min<long long>(a.capacity, (long long)a.window + a.tokens) : a.capacity;
-    if (a.capacity || !a.prefix) p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span, a.weights != nullptr);
-    if (a.prefix) p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix, false);
+    const int size = i8 ? 1 : 2;
+    const long long seqs = a.cache_rows ? 2 : a.batch;      // (of the cache: known to the caller only)
+    auto own_mapped = [&](const long long (&s)[3]) {
+        return can_map_cache(s[2], a.capacity, s[1], a.kvheads, s[0], seqs, size);
+    };
+    auto prefix_mapped = [&](const long long (&s)[2]) {
+        return can_map_cache(s[1], a.prefix, s[0], a.kvheads, 0, 1, size);
+    };
+    if (a.capacity || !a.prefix)
+        p.own = split((long long)a.batch * a.kvheads, (long long)a.tokens * R, span, a.weights != nullptr,
+                      own_mapped(a.k_stride) && own_mapped(a.v_stride));
+    if (a.prefix)
+        p.prefix = split(a.kvheads, (long long)a.batch * a.tokens * R, a.prefix, false,
+                         prefix_mapped(a.prefix_k_stride) && prefix_mapped(a.prefix_v_stride));
     // few rows and keys: one kernel whose units take both key sets one after the other
     p.joint = a.prefix && a.capacity && !p.own.tiles && !p.prefix.tiles && a.prefix + (long long)span <= kJointKeys;
     if (p.joint) {
@@ -144,7 +168,10 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     }
     p.logits = a.weights && !p.own.tiles && keeps_logits(a);
     p.neg_lse = a.weights != nullptr;
-    p.weight_tiles = a.weights && !p.logits && a.tokens > 0 && R <= 128;
+    // (INT8's queries are split into the workspace first, whatever their strides)
+    const bool q_mapped = i8 || (can_map(a.q_stride[0], a.batch, 2) && can_map(a.q_stride[1], a.tokens, 2) &&
+                                 can_map(a.q_stride[2], a.heads, 2));
+    p.weight_tiles = a.weights && !p.logits && a.tokens > 0 && R <= 128 && q_mapped;
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long r = at;

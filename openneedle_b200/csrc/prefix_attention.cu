@@ -753,7 +753,8 @@ __global__ __launch_bounds__(128) void prefix_finish_kernel(const PrefixAttn p, 
 // and walks the sequence's query rows, eight columns at a time, adding
 // 2^(z - L_row) of the rows that see the key.  Only for more query heads a KV head
 // than a tile of the tensor-core kernel has rows (it took 3200 us for two prompts
-// of 4096 tokens, the tiles take 182), and to copy the weights of calls without
+// of 4096 tokens, the tiles take 182), for 16-bit queries of strides that the copy
+// engine does not take (expanded ones), and to copy the weights of calls without
 // tokens.
 
 template <int TYPE, int HD>

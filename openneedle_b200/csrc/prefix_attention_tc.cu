@@ -1047,8 +1047,7 @@ bool cache_map(CUtensorMap *map, const void *base, int type, int hd, long long k
     *seq_flag = seq_stride != 0 && seqs > 1;
     if (!*head_flag) heads = 1;
     if (!*seq_flag) seqs = 1;
-    const long long ks = keys > 1 && key_stride ? key_stride * size : row;
-    if (keys > 1 && !key_stride) keys = 1;       // refused by the caller
+    const long long ks = keys > 1 ? key_stride * size : row;     // (above zero: keys of stride 0 are streamed)
     const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)keys, (cuuint64_t)heads, (cuuint64_t)seqs};
     const cuuint64_t strides[3] = {(cuuint64_t)ks, (cuuint64_t)(*head_flag ? head_stride * size : row),
                                    (cuuint64_t)(*seq_flag ? seq_stride * size : row)};

@@ -157,3 +157,17 @@ def test_c_abi_refuses_evictions(change, message):
     assert lib.needle2_evict_device(sizes + attention._EVICT_POINTERS.pack(*p.values()), None) == -1
     assert message in attention.last_error()
     assert lib.needle2_evict_device(None, None) == -1
+
+
+def test_keys_that_the_copy_engine_cannot_walk_are_streamed():
+    """200 tokens of 8 sequences against 4096 shared keys: tiles split the prefix into few ranges, streaming into
+    others, which the workspace shows; a stride of 0 along the keys is planned as streaming."""
+    lib = attention._bind_operators()[0]
+    sizes = {}
+    for stride in (64, 0):
+        args = bytearray(pack(batch=8, tokens=200, prefix=4096))
+        at = attention._ATTENTION_SIZES.size - 8 * (32 - 18 - 1)       # prefix_k_stride[1]
+        assert int.from_bytes(args[at:at + 8], "little") == 64
+        args[at:at + 8] = stride.to_bytes(8, "little")
+        sizes[stride] = lib.needle2_prefix_attention_workspace(bytes(args))
+    assert 0 < sizes[64] != sizes[0] > 0

@@ -655,3 +655,74 @@ def test_prefix_that_is_a_view_of_the_cache(ops, cache, t, s):
 
     for x, y in zip(run(lambda x: x), run(lambda x: x.clone())):
         assert torch.equal(x, y)
+
+
+def dense_reference(c):
+    """cache_ops_reference.attention on the GPU, all sequences at once (a prefix, lengths of at least the tokens)."""
+    g = cuda(c)
+    b, t, heads, d = c["q"].shape
+    kv, s = c["k"].shape[1:3]
+    p, r = c["prefix_k"].shape[1], heads // kv
+    wide = lambda x, sc: x.double() if sc is None else x.double() * sc.double().unsqueeze(-1)   # noqa: E731
+    k, v = (torch.cat((wide(g["prefix_" + n], g[f"prefix_{n}_scales"]).expand(b, -1, -1, -1),
+                       wide(g[n], g[n + "_scales"])), 2) for n in ("k", "v"))
+    q = g["q"].double().view(b, t, kv, r, d).permute(0, 2, 1, 3, 4)                 # [B, KV, T, R, D]
+    at = (g["lengths"].view(b, 1) - t + torch.arange(t, device="cuda")).view(b, 1, t, 1, 1)
+    seen = torch.arange(-p, s, device="cuda") <= at
+    z = (torch.einsum("bgtrd,bgkd->bgtrk", q, k) * d ** -0.5).masked_fill(~seen, -math.inf)
+    size = (torch.einsum("bgtrd,bgkd->bgtrk", q.abs(), k.abs()) * d ** -0.5).masked_fill(~seen, 0)
+    soft = torch.softmax(z, -1)
+    back = lambda x: x.permute(0, 2, 1, 3, *range(4, x.dim())).reshape(b, t, heads, *x.shape[4:]).cpu()   # noqa: E731
+    gained = soft[..., p:].sum((2, 3)).cpu()
+    most = torch.zeros_like(z[..., 0])
+    if g["v_scales"] is not None:
+        scales = torch.cat((g["prefix_v_scales"].expand(b, -1, -1), g["v_scales"]), 2).double()
+        most = 127 * seen.expand_as(z).sum(-1) * scales.abs().amax(-1).view(b, kv, 1, 1)
+    return {"out": back(torch.einsum("bgtrk,bgkd->bgtrd", soft, v)), "lse": back(torch.logsumexp(z, -1)),
+            "weights": c["weights"].double() + gained, "gained": gained, "most_v": back(most),
+            "mix": back(torch.einsum("bgtrk,bgkd->bgtrd", soft, v.abs())), "dz": back(size.amax(-1)),
+            "total_v": back(torch.einsum("bgtrk,bgkd->bgtrd", seen.expand_as(z).double(), v.abs()))}
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("b,t", [(1, 1), (24, 1), (6, 200)])
+@pytest.mark.parametrize("expanded", [("k", "v"), ("prefix_k", "prefix_v"), ("k",), ("prefix_v",)])
+def test_keys_expanded_along_their_axis(ops, cache, b, t, expanded):
+    """One key's row standing for all of them (a stride of 0), at sizes that stream and that would take tiles."""
+    heads, kv, p, s = 16, 4, 450, 210
+    c = R.make_inputs(cache, b, t, heads, kv, 64, p, s, [s - 3 - i % 5 for i in range(b)], seed=70 + t)
+    for n in expanded:
+        c[n] = c[n][..., :1, :].expand_as(c[n])
+    ref = dense_reference(c)
+    bound = R.bounds(c, ref)
+    d = {n: None if x is None else x.cuda() for n, x in c.items()}
+    for n in expanded:
+        d[n] = d[n][..., :1, :].contiguous().expand_as(d[n])
+        assert d[n].stride(-2) == 0
+    args = {n: d[n] for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales", "prefix_v_scales")
+            if n in d}
+    out, lse = ops.prefix_attention(d["q"], d["k"], d["v"], d["lengths"], return_lse=True, **args)
+    R.check(out, ref["out"], bound["out"], "out")
+    R.check(lse, ref["lse"], bound["lse"], "lse")
+    out, weights = ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], **args)
+    R.check(out, ref["out"], bound["out"], "out of accumulate_attention")
+    R.check(weights, ref["weights"], bound["weights"], "weights")
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("b,t,axis", [(6, 200, 0), (6, 200, 1), (6, 200, 2), (3, 1, 0), (3, 1, 2)])
+def test_queries_expanded_along_an_axis(ops, cache, b, t, axis):
+    """The same query for every sequence, token or head, as a stride of 0."""
+    c = R.make_inputs(cache, b, t, 16, 4, 64, 450, 210, [207 - i for i in range(b)], seed=80 + t)
+    c["q"] = c["q"].narrow(axis, 0, 1).expand_as(c["q"])
+    ref = dense_reference(c)
+    bound = R.bounds(c, ref)
+    d = cuda(c)
+    d["q"] = d["q"].narrow(axis, 0, 1).contiguous().expand_as(d["q"])
+    args = {n: d[n] for n in ("prefix_k", "prefix_v", "k_scales", "v_scales", "prefix_k_scales", "prefix_v_scales")}
+    out, lse = ops.prefix_attention(d["q"], d["k"], d["v"], d["lengths"], return_lse=True, **args)
+    R.check(out, ref["out"], bound["out"], "out")
+    R.check(lse, ref["lse"], bound["lse"], "lse")
+    out, weights = ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], **args)
+    R.check(out, ref["out"], bound["out"], "out of accumulate_attention")
+    R.check(weights, ref["weights"], bound["weights"], "weights")
