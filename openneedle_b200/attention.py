@@ -289,8 +289,14 @@ def _apart(outs, ins):
 
 
 def _no_gradients(torch, *tensors):
+    """Refuse tensors whose gradients or forward-mode tangents the call would drop (INT8 codes have none, their scales
+    may)."""
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
         raise ValueError("these operators have no gradients: detach the inputs or call them under torch.no_grad()")
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and any(        # (inside of a dual level only)
+            x is not None and forward.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError("these operators have no gradients: detach the inputs of their tangents")
 
 
 def _want_cache(torch, k, v, k_scales, v_scales, shape, name):
@@ -411,7 +417,8 @@ def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales
                                               prefix_v, k_scales, v_scales, prefix_k_scales, prefix_v_scales, tokens,
                                               window, scale, out))
     sizes, size, rows, weigh, extents = plan
-    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights)
+    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights, k_scales, v_scales, prefix_k_scales, prefix_v_scales,
+                  out, weights_out)
     device = k.device
     if extents is not None:
         same = weights_out is not None and weights_out.data_ptr() == weights.data_ptr() and \
@@ -506,7 +513,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
         plan = _remember(key, _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales,
                                           out, in_place))
     sizes, shape, (n_out, n_in) = plan
-    _no_gradients(torch, k, v, weights)
+    _no_gradients(torch, k, v, weights, k_scales, v_scales, *(() if out is None else out))
     device = k.device
     context = _on_stream(torch, device, stream)
     if context is not None:

@@ -171,3 +171,48 @@ def test_keys_that_the_copy_engine_cannot_walk_are_streamed():
         args[at:at + 8] = stride.to_bytes(8, "little")
         sizes[stride] = lib.needle2_prefix_attention_workspace(bytes(args))
     assert 0 < sizes[64] != sizes[0] > 0
+
+
+@pytest.mark.parametrize("name", ("q", "weights", "k_scales", "v_scales", "prefix_k_scales", "prefix_v_scales", "out",
+                                  "weights_out"))
+@pytest.mark.parametrize("forward", (False, True))
+def test_attention_drops_no_gradient(name, forward):
+    """Of whatever floating tensor, backward or forward mode."""
+    from torch.autograd import forward_ad
+    c = inputs()
+    c.update(out=torch.zeros_like(c["q"]), weights_out=torch.zeros_like(c["weights"]))
+    more = {n: c[n] for n in ("out", "weights_out")}
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        attend(c, weigh=True, **more)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            attend(c, weigh=True, **more)
+        x = forward_ad.make_dual(c[name], torch.ones_like(c[name])) if forward else c[name].requires_grad_()
+        c[name] = x
+        if name in more:
+            more[name] = x
+        with pytest.raises(ValueError, match="no gradients"):
+            attend(c, weigh=True, **more)
+        with torch.no_grad(), pytest.raises(ValueError, match="no gradients" if forward else "CUDA tensors"):
+            attend(c, weigh=True, **more)
+
+
+@pytest.mark.parametrize("name", ("weights", "k_scales", "v_scales", "out"))
+@pytest.mark.parametrize("forward", (False, True))
+def test_evict_drops_no_gradient(name, forward):
+    from torch.autograd import forward_ad
+    c = inputs()
+    out = attention.Evicted(*(torch.zeros_like(c[n][:, :, :8]) for n in ("k", "v", "weights")),
+                            torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, 8, dtype=torch.int32),
+                            *(torch.zeros_like(c[n][:, :, :8]) for n in ("k_scales", "v_scales")))
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            evict(c, out=out)
+        x = out.v_scales if name == "out" else c[name]
+        x = forward_ad.make_dual(x, torch.ones_like(x)) if forward else x.requires_grad_()
+        if name == "out":
+            out = out._replace(v_scales=x)
+        else:
+            c[name] = x
+        with pytest.raises(ValueError, match="no gradients"):
+            evict(c, out=out)
