@@ -370,11 +370,10 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
             raise ValueError("tokens must be contiguous")
     if not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous")
-    window = int(window)
     if window < 0:
         raise ValueError("window must not be negative")
     window = 0 if window >= capacity else window
-    scale = head_dim ** -0.5 if scale is None else float(scale)
+    scale = head_dim ** -0.5 if scale is None else scale
     if weights is not None:
         _want(weights, "weights", (batch, kvheads, capacity), torch.float32, device, last=False)
     if out is not None:
@@ -408,6 +407,8 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
 def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
             prefix_v_scales, tokens, window, scale, out, return_lse, stream):
     lib, torch, types, raw_stream = _bind_operators()
+    # (numbers from here on: a plan is kept by its options' values, not by the objects that held them)
+    window, scale = int(window), None if scale is None else float(scale)
     key = (_layout(q), _layout(k), _layout(v), _layout(lengths), _layout(weights), _layout(weights_out),
            _layout(prefix_k), _layout(prefix_v), _layout(k_scales), _layout(v_scales), _layout(prefix_k_scales),
            _layout(prefix_v_scales), _layout(tokens), window, scale, _layout(out))
@@ -506,6 +507,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     to the inputs themselves (``in_place``; lengths and indices are new), or to
     new tensors of ``keep`` slots, zero behind the kept keys."""
     lib, torch, types, raw_stream = _bind_operators()
+    keep, first, recent, in_place = int(keep), int(first), int(recent), bool(in_place)   # (by value, as above)
     key = (_layout(k), _layout(v), _layout(weights), _layout(lengths), _layout(k_scales), _layout(v_scales), keep,
            first, recent, in_place, None if out is None else tuple(map(_layout, out)))
     plan = _plans.get(key)
@@ -549,7 +551,7 @@ def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_sca
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
-    device, keep, first, recent = k.device, int(keep), int(first), int(recent)
+    device = k.device
     if keep < 0 or first < 0 or recent < 0 or first + recent > keep:
         raise ValueError("first and recent must not be negative, nor exceed keep together")
     _want_cache(torch, k, v, k_scales, v_scales, (batch, kvheads, capacity, head_dim), "")

@@ -216,3 +216,26 @@ def test_evict_drops_no_gradient(name, forward):
             c[name] = x
         with pytest.raises(ValueError, match="no gradients"):
             evict(c, out=out)
+
+
+def test_options_in_tensors_are_taken_by_value(monkeypatch):
+    """A scale, a window or a count that is held in a tensor and changes in place: no plan of its earlier value."""
+    scale, window, keep = torch.tensor(0.125), torch.tensor(4), torch.tensor(8)
+    plans = {}
+    monkeypatch.setattr(attention, "_plans", plans)
+    for i in range(2):
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            attend(inputs(), scale=scale, window=window)
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            evict(inputs(), keep=keep, first=torch.tensor(1), recent=torch.tensor(2))
+        assert len(plans) == 2 * (i + 1)
+        scale *= 2
+        window += 1
+        keep += 1
+    packed = [p[0] for p in plans.values()]
+    at = attention.struct.calcsize("@9i")
+    assert [attention.struct.unpack_from("@f", x, at)[0] for x in packed[::2]] == [0.125, 0.25]
+    assert [attention.struct.unpack_from("@9i", x)[7] for x in packed[::2]] == [4, 5]
+    assert [attention.struct.unpack_from("@9i", x)[5] for x in packed[1::2]] == [8, 9]
+    with pytest.raises(ValueError, match="scale"):
+        attend(inputs(), scale=torch.tensor(0.0))
