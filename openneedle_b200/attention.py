@@ -9,6 +9,7 @@ CUDA tensors and do not synchronise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as ct
 import functools
 import struct
@@ -393,7 +394,9 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
         *_strides(3, k, v, k_scales, v_scales), *_strides(2, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales),
         *_strides(3, weights), *wide)
     one = 4096 if weigh else 0                             # (given or not: the pointers are not read)
-    size = lib.needle2_prefix_attention_workspace(sizes + _ATTENTION_POINTERS.pack(*[4096] * 14, one, one))
+    # the split goes by the multiprocessors of the current device, which has to be the tensors' then as in the call
+    with torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext():
+        size = lib.needle2_prefix_attention_workspace(sizes + _ATTENTION_POINTERS.pack(*[4096] * 14, one, one))
     if size < 0:
         raise ValueError(last_error())
     extents = None

@@ -239,3 +239,30 @@ def test_options_in_tensors_are_taken_by_value(monkeypatch):
     assert [attention.struct.unpack_from("@9i", x)[5] for x in packed[1::2]] == [8, 9]
     with pytest.raises(ValueError, match="scale"):
         attend(inputs(), scale=torch.tensor(0.0))
+
+
+def test_workspaces_are_sized_on_the_tensors_device(monkeypatch):
+    """The plan of tensors of device 1, made while another device is current: the library is asked under device 1."""
+    import contextlib
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d.index
+        yield
+        current[0] = before
+
+    class Library:
+        def needle2_prefix_attention_workspace(self, args):
+            asked.append(current[0])
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    types = attention._bind_operators()[2]
+    with FakeTensorMode():
+        q, k = (torch.empty(2, n, 5, 64, dtype=torch.bfloat16, device="cuda:1") for n in (8, 4))
+        lengths = torch.empty(2, dtype=torch.int32, device="cuda:1")
+        attention._plan_attention(Library(), torch, types, q.transpose(1, 2), k, k, lengths, None, None, None, None,
+                                  None, None, None, None, None, 0, None, None)
+    assert asked == [1] and current == [0]
