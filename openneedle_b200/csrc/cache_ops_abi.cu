@@ -17,6 +17,10 @@ namespace nb200 {
 namespace {
 
 constexpr long long kMaxUnits = 0x7fffffff;
+// Slots of a cache or prefix: indexes of keys are 32-bit, and the ends of key ranges (up to
+// 2^19, of a multiple of 32 keys each, or 2^16 of 128) and loops by a CTA's threads go
+// beyond the last one.
+constexpr long long kMaxKeys = 0x7e000000;
 
 bool refuse(const char *msg) {
     set_error(msg);
@@ -42,8 +46,10 @@ bool sizes_ok(const needle2_prefix_attention_args &a) {
     if (!(a.scale > 0.f) || !std::isfinite(a.scale))
         return refuse("prefix attention: scale must be positive and finite");
     const long long rows = (long long)a.batch * a.tokens;
-    // units of work and row numbers are 32-bit
-    if (a.capacity > 0x7fffff00 || a.prefix > 0x7fffff00 || rows * a.heads > kMaxUnits / 4 ||
+    // units of work, row numbers and the first key of a window (before a sequence's, where it is
+    // shorter) are 32-bit
+    if (a.capacity > kMaxKeys || a.prefix > kMaxKeys || rows * a.heads > kMaxUnits / 4 ||
+        (a.window < a.capacity && (long long)a.window + a.tokens > kMaxKeys) ||
         (long long)a.batch * a.kvheads > kMaxUnits / 64 ||
         (long long)a.batch * a.kvheads * (((long long)a.capacity + 63) / 64) > kMaxUnits)
         return refuse("prefix attention: the call is too large");
@@ -55,7 +61,7 @@ constexpr long long kMaxLogits = 1LL << 27;   // kept for the weights
 
 struct Plan {
     PrefixSplit prefix, own;
-    bool joint, joint_tiles, logits, neg_lse, weight_tiles;
+    bool joint, joint_tiles, logits, neg_lse, weight_tiles, fits;
     long long part_o, part_lse, neg_lse_at, logits_at, q16_at, q16_scale_at, bytes;
 };
 
@@ -190,7 +196,20 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
         p.q16_scale_at = take(rows * 4);
     }
     p.bytes = n > 1 ? at + 16 : at;              // partial rows lie on 32 bytes, the workspace on 16
+    // (more rows than a tile against keys that cannot be mapped, in many ranges)
+    auto units = [&](const PrefixSplit &s, long long groups, long long group_rows) {
+        const int unit_rows = s.tiles ? 128 : tile;
+        return groups * ((group_rows + unit_rows - 1) / unit_rows) * s.ranges;
+    };
+    p.fits = units(p.own, (long long)a.batch * a.kvheads, (long long)a.tokens * R) +
+                 units(p.prefix, a.kvheads, (long long)a.batch * a.tokens * R) <= kMaxUnits;
     return p;
+}
+
+bool plan_call(const needle2_prefix_attention_args &a, Plan &p) {
+    if (!sizes_ok(a)) return false;
+    p = plan_of(a);
+    return p.fits || refuse("prefix attention: the call is too large");
 }
 
 template <int N>
@@ -225,7 +244,8 @@ bool attention(const needle2_prefix_attention_args &a, void *workspace, long lon
     if (!a.lengths) return refuse("lengths is null");
     if ((a.weights != nullptr) != (a.weights_out != nullptr))
         return refuse("weights and weights_out go together");
-    const Plan plan = plan_of(a);
+    Plan plan;
+    if (!plan_call(a, plan)) return false;
     if (bytes < plan.bytes || (plan.bytes && (!workspace || !aligned16(workspace))))
         return refuse("prefix attention: the workspace is too small or not 16-byte aligned");
     PrefixAttn p{};
@@ -284,8 +304,8 @@ bool evict(const needle2_evict_args &a, cudaStream_t st) {
     if ((long long)a.first + a.recent > a.keep) return refuse("evict: first + recent must not exceed keep");
     if (a.out_capacity < a.keep) return refuse("evict: the output holds fewer than keep slots");
     if ((long long)a.batch * a.kvheads > kMaxUnits / 64 ||
-        (long long)a.batch * a.kvheads * ((a.keep + 15) / 16) > kMaxUnits || a.capacity > 0x7fffff00 ||
-        a.out_capacity > 0x7fffff00)
+        (long long)a.batch * a.kvheads * (((long long)a.keep + 15) / 16) > kMaxUnits || a.capacity > kMaxKeys ||
+        a.out_capacity > kMaxKeys)
         return refuse("evict: the call is too large");
     if (a.batch == 0) return true;
     const int size = a.cache_type == kCacheI8 ? 1 : 2;
@@ -342,7 +362,8 @@ bool evict(const needle2_evict_args &a, cudaStream_t st) {
 }  // namespace
 
 long long prefix_attention_workspace(const needle2_prefix_attention_args &a) {
-    return sizes_ok(a) ? plan_of(a).bytes : -1;
+    Plan plan;
+    return plan_call(a, plan) ? plan.bytes : -1;
 }
 bool prefix_attention(const needle2_prefix_attention_args &a, void *workspace, long long bytes, cudaStream_t st) {
     return attention(a, workspace, bytes, st);

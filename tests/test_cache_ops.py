@@ -266,3 +266,38 @@ def test_workspaces_are_sized_on_the_tensors_device(monkeypatch):
         attention._plan_attention(Library(), torch, types, q.transpose(1, 2), k, k, lengths, None, None, None, None,
                                   None, None, None, None, None, 0, None, None)
     assert asked == [1] and current == [0]
+
+
+def expanded(**change):
+    """`pack` with keys of stride 0, which take no memory, whatever their number."""
+    args = bytearray(pack(kstride=0, **change))
+    at = attention.struct.calcsize("@9if") + (-attention.struct.calcsize("@9if") % 8)
+    for i in (11, 18, 19, 20, 21):                          # v's, and those of the prefix
+        args[at + 8 * i:at + 8 * i + 8] = bytes(8)
+    return bytes(args)
+
+
+@pytest.mark.parametrize("change", [
+    {"capacity": 0x7f000000}, {"prefix": 0x7f000000},        # ends of key ranges
+    {"capacity": 0x7d800000, "window": 0x7d700000, "tokens": 1 << 24},       # the start of a window
+    {"batch": 1, "kvheads": 1, "heads": 1, "capacity": 1 << 27, "tokens": 1 << 20}])     # units of streamed keys
+def test_calls_beyond_32_bit_numbers_are_refused(change):
+    lib = attention._bind_operators()[0]
+    assert lib.needle2_prefix_attention_workspace(expanded(**change)) == -1
+    assert "too large" in attention.last_error()
+    args = expanded(**change, weights=4096, weights_out=4096)
+    assert lib.needle2_prefix_attention_device(args, 4096, 1 << 60, None) == -1
+    assert "too large" in attention.last_error()
+
+
+@pytest.mark.parametrize("change", [{"capacity": 0x7f000000}, {"out_capacity": 0x7f000000}])
+def test_evictions_beyond_32_bit_indexes_are_refused(change):
+    """Loops in steps of a CTA's threads would pass the largest index and never end."""
+    lib = attention._bind_operators()[0]
+    sizes = dict(batch=1, kvheads=1, head_dim=64, capacity=64, out_capacity=64, keep=8, first=2, recent=2,
+                 cache_type=0)
+    sizes.update(change)
+    args = attention._EVICT_SIZES.pack(*sizes.values(), *[0] * 30) + attention._EVICT_POINTERS.pack(
+        *[4096] * 5, 8192, *[16384] * 6, 65536)
+    assert lib.needle2_evict_device(args, None) == -1
+    assert "too large" in attention.last_error()
