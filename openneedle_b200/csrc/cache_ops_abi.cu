@@ -93,18 +93,41 @@ int sm_count() {
     return count[dev];
 }
 
+// Keys of a range: products cut their sums to 24 bits towards zero, 16-bit caches' eight
+// times 128 keys, INT8's 16 times, by 2^-25 of the end's on the average. So many keys
+// stay well within half a step of FP16, and INT8's streaming within 2^-16 (65536 keys
+// of one sign in a range: 2^-13.6); its tiles' sums leave the accumulator long before.
+constexpr long long kTileKeysI8 = 1LL << 40, kTileKeys16 = 32768, kStreamKeysI8 = 4096, kStreamKeys16 = 1 << 18;
+
+// Query rows of a streaming unit.
+int stream_rows(const needle2_prefix_attention_args &a) { return a.cache_type == kCacheI8 ? 8 : 16; }
+
+// `group_rows` query rows in each of `groups` row groups, against up to `keys` keys: in how
+// many key ranges streaming (s) and tiles (t) take them. More for more keys.
+void ranges_of(const needle2_prefix_attention_args &a, int sms, long long groups, long long group_rows, long long keys,
+               PrefixSplit &s, PrefixSplit &t) {
+    const bool i8 = a.cache_type == kCacheI8;
+    const long long tile_keys = i8 ? kTileKeysI8 : kTileKeys16, stream_keys = i8 ? kStreamKeysI8 : kStreamKeys16;
+    t.tiles = true;
+    t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
+    const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
+    const long long most = (keys + (t.alt ? 511 : 255)) / (t.alt ? 512 : 256);
+    t.ranges = (int)std::max((keys + tile_keys - 1) / tile_keys,
+                             std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL})));
+    const long long units = groups * ((group_rows + stream_rows(a) - 1) / stream_rows(a));
+    const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
+    s.ranges = (int)std::max((keys + stream_keys - 1) / stream_keys,
+                             std::max(1LL, std::min({want, (keys + 255) / 256, 64LL})));
+}
+
+long long padded(long long bytes) { return (bytes + 255) / 256 * 256; }
+
 Plan plan_of(const needle2_prefix_attention_args &a) {
     Plan p{};
     const int sms = sm_count();
     const bool i8 = a.cache_type == kCacheI8;
-    const int R = a.heads / a.kvheads, tile = i8 ? 8 : 16;
+    const int R = a.heads / a.kvheads, tile = stream_rows(a);
     const long long rows = (long long)a.batch * a.tokens * a.heads;
-    // Keys of a range: products cut their sums to 24 bits towards zero, 16-bit caches' eight
-    // times 128 keys, INT8's 16 times, by 2^-25 of the end's on the average. So many keys
-    // stay well within half a step of FP16, and INT8's streaming within 2^-16 (65536 keys
-    // of one sign in a range: 2^-13.6); its tiles' sums leave the accumulator long before.
-    const long long tile_keys = i8 ? 1LL << 40 : 32768, stream_keys = i8 ? 4096 : 1 << 18;
-    // `group_rows` query rows in each of `groups` row groups, against up to `keys` keys.
     // Tiles or streaming by their times, fitted to measurements (us): a tile CTA has its
     // multiprocessor to itself and takes 9 beside its keys, whose conversion INT8 waits for,
     // a streaming unit 1.2 beside its keys, of which the 16-bit caches' 128 dimensions take
@@ -116,17 +139,10 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     const double key = (i8 ? 4.3e-3 : 6e-3) * (a.head_dim == 128 ? 1.7 : 1.0);
     auto split = [&](long long groups, long long group_rows, long long keys, bool weights, bool mapped) {
         PrefixSplit s, t;
-        t.tiles = true;
-        t.alt = group_rows <= 128 || (i8 && a.head_dim == 128);
-        const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
-        const long long most = (keys + (t.alt ? 511 : 255)) / (t.alt ? 512 : 256);
-        t.ranges = (int)std::max((keys + tile_keys - 1) / tile_keys,
-                                 std::max(1LL, std::min({sms / std::max(1LL, tiles), most, 32LL})));
-        const long long units = groups * ((group_rows + tile - 1) / tile);
-        const long long want = (4LL * sms + units - 1) / std::max(1LL, units);
-        s.ranges = (int)std::max((keys + stream_keys - 1) / stream_keys,
-                                 std::max(1LL, std::min({want, (keys + 255) / 256, 64LL})));
+        ranges_of(a, sms, groups, group_rows, keys, s, t);
         if (group_rows <= tile || !mapped) return s;
+        const long long tiles = groups * ((group_rows + (t.alt ? 127 : 255)) / (t.alt ? 128 : 256));
+        const long long units = groups * ((group_rows + tile - 1) / tile);
         const double waves = std::max(1.0, (double)tiles * t.ranges / sms);
         const double tile_key =
             i8 ? (a.head_dim == 128 ? 33e-3 : 29e-3) : (t.alt ? 11e-3 : 14.5e-3) * (a.head_dim == 128 ? 1.3 : 1.0);
@@ -165,7 +181,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     // tiles of the sequences' own rows that fill the machine take the prefix first, in
     // the same accumulators: no partial results
     p.joint_tiles = a.prefix && p.own.tiles && p.prefix.tiles && p.own.ranges == 1 &&
-                    (i8 || a.prefix + (long long)span <= tile_keys) &&
+                    (i8 || a.prefix + (long long)span <= kTileKeys16) &&
                     (long long)a.batch * a.kvheads * ((a.tokens * R + 255) / 256) * 5 >= 4LL * sms;
     if (p.joint_tiles) p.prefix = PrefixSplit{};
     if (!a.capacity && p.own.ranges) {               // no key at all: the streaming kernel writes the zeros
@@ -181,7 +197,7 @@ Plan plan_of(const needle2_prefix_attention_args &a) {
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long r = at;
-        at += (bytes + 255) / 256 * 256;
+        at += padded(bytes);
         return r;
     };
     const int n = p.own.slots() + p.prefix.slots();
@@ -364,6 +380,23 @@ bool evict(const needle2_evict_args &a, cudaStream_t st) {
 long long prefix_attention_workspace(const needle2_prefix_attention_args &a) {
     Plan plan;
     return plan_call(a, plan) ? plan.bytes : -1;
+}
+long long prefix_attention_workspace_most(const needle2_prefix_attention_args &a) {
+    if (!sizes_ok(a)) return -1;
+    const int sms = sm_count();
+    const int R = a.heads / a.kvheads;
+    long long most = 0;
+    for (long long batch = 1; batch <= a.batch; ++batch) {
+        auto slots = [&](long long groups, long long group_rows, long long keys) {
+            PrefixSplit s, t;
+            ranges_of(a, sms, groups, group_rows, keys, s, t);
+            return (long long)(group_rows <= stream_rows(a) ? s.slots() : std::max(s.slots(), t.slots()));
+        };
+        const long long rows = batch * a.heads, n = slots(batch * a.kvheads, R, a.capacity) +
+                                                    (a.prefix ? slots(a.kvheads, batch * R, a.prefix) : 0);
+        if (n > 1) most = std::max(most, padded(rows * n * a.head_dim * 4) + padded(rows * n * 4) + 16);
+    }
+    return most;
 }
 bool prefix_attention(const needle2_prefix_attention_args &a, void *workspace, long long bytes, cudaStream_t st) {
     return attention(a, workspace, bytes, st);

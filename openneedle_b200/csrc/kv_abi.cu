@@ -126,7 +126,9 @@ __global__ void index_upload_kernel(const __grid_constant__ IndexArgs a, int *id
 }
 
 bool upload_index(KVPool &kv, const int *session_ids, const int *positions, int count, cudaStream_t st) {
-    if (!kv.ids.reserve(count) || !kv.pos.reserve(count)) return false;
+    // (room for all sessions at once: a captured call keeps the addresses)
+    const size_t most = std::max(count, kv.sessions);
+    if (!kv.ids.reserve(most) || !kv.pos.reserve(most)) return false;
     if (count <= kIndexArgMax) {
         IndexArgs a;
         a.count = count;
@@ -242,7 +244,6 @@ bool query_shared(KVPool &kv, const int *session_ids, const int *positions, int 
     needle2_prefix_attention_args a{};
     a.batch = count; a.tokens = 1; a.heads = kv.heads; a.kvheads = kv.kvheads; a.head_dim = kv.hd;
     a.prefix = kv.prefix;
-    a.capacity = most;                           // the longest entry decides how the keys are split
     a.cache_type = 0;
     a.scale = 1 / std::sqrt((float)kv.hd);
     const long long width = (long long)kv.heads * kv.hd, row = kv.hd;
@@ -263,9 +264,17 @@ bool query_shared(KVPool &kv, const int *session_ids, const int *positions, int 
     a.prefix_k = kv.pk.ptr; a.prefix_v = kv.pv.ptr; a.prefix_k_scales = kv.pks.ptr; a.prefix_v_scales = kv.pvs.ptr;
     a.lengths = kv.pos.ptr;
     a.cache_rows = kv.ids.ptr;
-    const long long bytes = prefix_attention_workspace(a);
-    if (bytes < 0 || !kv.shared_ws.reserve((size_t)bytes)) return false;
-    return prefix_attention(a, kv.shared_ws.ptr, bytes, st);
+    // the workspace is that of the largest call the pool can take, once: generation does not
+    // allocate, and a captured call keeps its address
+    if (!kv.shared_ws.cap) {
+        a.batch = kv.sessions;
+        a.capacity = kv.cs;
+        const long long bytes = prefix_attention_workspace_most(a);
+        if (bytes < 0 || !kv.shared_ws.reserve((size_t)std::max(bytes, 16LL))) return false;
+        a.batch = count;
+    }
+    a.capacity = most;                           // the longest entry decides how the keys are split
+    return prefix_attention(a, kv.shared_ws.ptr, (long long)kv.shared_ws.cap, st);
 }
 
 }  // namespace

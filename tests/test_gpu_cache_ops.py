@@ -726,3 +726,44 @@ def test_queries_expanded_along_an_axis(ops, cache, b, t, axis):
     out, weights = ops.accumulate_attention(d["q"], d["k"], d["v"], d["lengths"], d["weights"], **args)
     R.check(out, ref["out"], bound["out"], "out of accumulate_attention")
     R.check(weights, ref["weights"], bound["weights"], "weights")
+
+
+def test_pool_query_shared_allocates_once(ops):
+    """The pool's workspace does not grow with the positions."""
+    import numpy as np
+    kv = ops.KVCache(64, 8, 1, 128, 8192, 0, 0)
+    ids = list(range(64))
+    q = np.ones((64, 8 * 128), np.float32)
+    kv.store(ids, [0] * 64, *(np.ones((64, 128), np.float32) for _ in range(2)))
+    free = []
+    for at in (0, 700, 8191):
+        kv.query_shared(ids, [at] * 64, q)
+        free.append(torch.cuda.mem_get_info()[0])
+    assert free[0] == free[1] == free[2]
+
+
+def test_pool_query_shared_in_a_graph(ops):
+    """A captured call stays good when later calls are longer and of more sessions."""
+    import numpy as np
+    rng = np.random.default_rng(3)
+    kv = ops.KVCache(64, 8, 1, 128, 4000, 0, 500)
+    kv.set_prefix(*(rng.normal(size=(500, 128)).astype(np.float32) for _ in range(2)))
+    for at in range(500, 4000):
+        kv.store(list(range(64)), [at] * 64, *(rng.normal(size=(64, 128)).astype(np.float32) for _ in range(2)))
+    q = torch.from_numpy(rng.normal(size=(64, 1024)).astype(np.float32)).cuda()
+    out, want = torch.zeros(3, 1024, device="cuda"), torch.zeros(3, 1024, device="cuda")
+    few = ([5, 0, 9], [610, 619, 604])
+    kv.query_shared_device(*few, q, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.query_shared_device(*few, q, out, stream=torch.cuda.current_stream())
+    every = torch.zeros(64, 1024, device="cuda")
+    kv.query_shared_device(list(range(64)), [3999] * 64, q, every)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    again = torch.zeros(64, 1024, device="cuda")
+    kv.query_shared_device(list(range(64)), [3999] * 64, q, again)
+    assert torch.equal(again, every)
