@@ -39,6 +39,7 @@ struct Buf {
         cap = n;
         return true;
     }
+    bool clear(cudaStream_t st) { return !ptr || cudaMemsetAsync(ptr, 0, sizeof(T) * cap, st) == cudaSuccess; }
     void release() {
         if (ptr) cudaFree(ptr);
         ptr = nullptr;
@@ -311,6 +312,11 @@ KVPool *kv_pool_new(int sessions, int heads, int kvheads, int head_dim, int max_
         ok = ok && kv->sk.reserve(srow * head_dim) && kv->sv.reserve(srow * head_dim) && kv->sks.reserve(srow) &&
              kv->svs.reserve(srow);
     }
+    // slots that nothing was stored in are zeros, as in the reference's own cache
+    for (auto *b : {&kv->pk, &kv->pv, &kv->sk, &kv->sv}) ok = ok && b->clear(kv->stream);
+    for (auto *b : {&kv->pks, &kv->pvs, &kv->sks, &kv->svs, &kv->pkf, &kv->pvf, &kv->skf, &kv->svf})
+        ok = ok && b->clear(kv->stream);
+    ok = ok && cudaStreamSynchronize(kv->stream) == cudaSuccess;
     if (!ok) {
         if (last_error()[0] == 0) set_error("KV pool creation failed");
         delete kv;

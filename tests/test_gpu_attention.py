@@ -187,3 +187,20 @@ def test_validation_errors(attention):
         kv.store([0, 0], [4, 5], np.zeros((2, 256), np.float32), np.zeros((2, 256), np.float32))
     with pytest.raises(MemoryError, match="multiple of kvheads|at most 8"):
         attention.KVCache(1, 18, 2, 64, 8)
+
+
+def test_new_pools_are_empty(attention):
+    """A pool in memory that others left, beside some that live, holds zeros wherever nothing was stored."""
+    ones, alive = np.ones((4, 128), np.float32), []
+    for step in range(8):
+        pools = [attention.KVCache(4, 4, 2, 64, 64, 0, 0) for _ in range(6)]
+        for kv in pools:
+            for session in range(4):
+                for n, x in kv.export(session).items():
+                    assert not x.any(), (step, n)
+        for kv in pools:
+            for at in range(64):
+                kv.store([0, 1, 2, 3], [at] * 4, ones, ones)
+            assert kv.export(3)["keys_i8"].all()
+        alive.append(pools[step % 6])
+        del kv, pools
