@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
     char *ring = smem + G::kRing;
     float *scales = (float *)(smem + G::kScaleAt);               // [kScaleRing][K, V][kStep]
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], raw_full[4], raw_empty[4];
-    __shared__ __align__(8) uint64_t s_full[3], p_full[3][2], o_done[2], o_full[2], q_full;
+    __shared__ __align__(8) uint64_t s_full[3], p_full[3][2], o_done[2], o_full[2], q_full, drained;
     __shared__ float qscale[I8 ? 256 : 1];
     __shared__ float vmost[G::kScaleRing][2];
     __shared__ const char *qrow[256];
@@ -221,6 +221,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             mbar_init(&o_full[i], 1);
         }
         mbar_init(&q_full, 32 * kMathWarps);
+        mbar_init(&drained, 1);
         abort_at = 0;
         fence_barrier_init();
     }
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             constexpr uint32_t ids = idesc(BF, false, kStep), ido = idesc(BF, true, HD);
             auto step_of = [&](int k) { return each == 2 ? k >> 1 : k; };
             auto tile_of = [&](int k) { return alt || each == 2 ? k & 1 : 0; };
-            auto have = [&](int i) { return wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
+            auto have = [&](int i) { wait_phase(&full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag); };
             auto logits = [&](int k, int buffer) {        // S_k = Q K^T
                 const int i = 2 * step_of(k), w = tile_of(k);
                 const uint32_t kt = r0 + (i % kStages) * G::kKVBytes;
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                 __syncwarp();
             };
             auto have_v = [&](int j) {
-                if (!have(2 * j + 1)) return false;
+                have(2 * j + 1);
                 const int valid = j < before ? p.prefix - j * kStep : hi - lo - (j - before) * kStep;
                 if (!I8 && valid < kStep) {               // rows behind the range: whatever they hold, zeros
                     char *v = ring + ((2 * j + 1) % kStages) * G::kKVBytes;
@@ -333,31 +334,33 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                     fence_proxy_async();
                 }
                 __syncwarp();
-                return true;
             };
-            bool ok = n > 0 && wait_phase(&q_full, 0, abort_flag);
-            for (int k = 0; ok && k < min(items, ahead); ++k) {
-                ok = have(2 * step_of(k));
-                if (ok) logits(k, k);
+            if (n > 0) wait_phase(&q_full, 0, abort_flag);
+            for (int k = 0; k < min(items, ahead); ++k) {
+                have(2 * step_of(k));
+                logits(k, k);
             }
             Turn turn;
-            for (int k = 0; ok && k < items; ++k) {
+            for (int k = 0; k < items; ++k) {
                 const bool more = k + ahead < items;
-                ok = ((each == 2 && (k & 1)) || have_v(step_of(k))) &&
-                     (!G::kEarly || !more || have(2 * step_of(k + ahead))) &&
-                     wait_phase(&p_full[turn.buffer][0], turn.phase, abort_flag);
-                if (!ok) break;
+                if (each == 1 || !(k & 1)) have_v(step_of(k));
+                if (G::kEarly && more) have(2 * step_of(k + ahead));
+                wait_phase(&p_full[turn.buffer][0], turn.phase, abort_flag);
                 values(k, turn.buffer, 0);
-                ok = wait_phase(&p_full[turn.buffer][1], turn.phase, abort_flag);
-                if (!ok) break;
+                wait_phase(&p_full[turn.buffer][1], turn.phase, abort_flag);
                 values(k, turn.buffer, 1);
                 if (more) {
-                    ok = G::kEarly || have(2 * step_of(k + ahead));
-                    if (ok) logits(k + ahead, turn.buffer);
+                    if (!G::kEarly) have(2 * step_of(k + ahead));
+                    logits(k + ahead, turn.buffer);
                 }
                 turn.on(1, ahead);
             }
             __syncwarp();
+            if (__any_sync(0xffffffffu, *abort_flag)) {   // no product is in flight when TMEM is freed
+                if (elect_one()) tc::commit(&drained);
+                mbar_wait(&drained, 0);
+                __syncwarp();
+            }
         } else if (warp >= kConvertWarp) {
             // ---- INT8 tiles to FP16, exactly
             if constexpr (I8) {
@@ -385,17 +388,17 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
                         }
 #pragma unroll
                         for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                        if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) break;
+                        if (i >= kStages) wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag);
     #pragma unroll
                         for (int e = 0; e < kStep / kN; ++e) {
                             sk[me + e * kN] = kx[e];
                             sk[kStep + me + e * kN] = vx[e];
                         }
                         if (lane == 0) vmost[j % G::kScaleRing][warp - kConvertWarp] = most;
-                    } else if (i >= kStages && !wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag)) {
-                        break;
+                    } else if (i >= kStages) {
+                        wait_phase(&empty[s], (uint32_t)(i / kStages - 1) & 1, abort_flag);
                     }
-                    if (!wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag)) break;
+                    wait_phase(&raw_full[rs], (uint32_t)(i / G::kRaw) & 1, abort_flag);
                     const char *src = smem + G::kRawAt + rs * G::kRawBytes;
                     char *dst = ring + s * G::kKVBytes;
     #pragma unroll 4
@@ -496,19 +499,17 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
         // INT8: O leaves for these sums every kHold steps, held * hold + O is the whole
         // (see kHold)
         float held[HD], hold = 0.f;
-        bool ok = true;
         Turn turn;
         turn.on(w, ahead);
         for (int i = 0; i < mine; ++i, turn.on(each == 2 || alt ? 2 : 1, ahead)) {
             const int j = alt ? 2 * i + w : i;
             const int j0 = j < before ? j * kStep : lo + (j - before) * kStep;
             const int from = j < before ? 0 : first, to = j < before ? p.prefix - 1 : last;   // keys the row sees
-            ok = wait_phase(&s_full[turn.buffer], turn.phase, abort_flag);
+            wait_phase(&s_full[turn.buffer], turn.phase, abort_flag);
             if (I8) {
                 const int v = 2 * j + 1;                  // (and the step's scales)
-                ok = ok && wait_phase(&full[v % kStages], (uint32_t)(v / kStages) & 1, abort_flag);
+                wait_phase(&full[v % kStages], (uint32_t)(v / kStages) & 1, abort_flag);
             }
-            if (!ok) break;
             tc::fence_after();
             const uint32_t ts = s0 + turn.buffer * kStep;
             const float *sk = scales + (j % G::kScaleRing) * 2 * kStep;
@@ -572,7 +573,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             if (leave || (i > 0 && __any_sync(0xffffffffu, keep != 1.f))) {
                 // O holds the steps before: the last one's product has to end first (the
                 // ones before that had ended when these logits were computed)
-                ok = wait_phase(&o_done[w], (uint32_t)(i - 1) & 1, abort_flag);
+                wait_phase(&o_done[w], (uint32_t)(i - 1) & 1, abort_flag);
                 tc::fence_after();
                 hold *= keep;
                 if (leave) {
@@ -640,9 +641,10 @@ __global__ __launch_bounds__(kTileThreads, 1) void prefix_tile_kernel(
             part[0] = add2(part[0], part[1]);
             sum += part[0].x + part[0].y;
         }
-        if (mine > 0) ok = ok && wait_phase(&o_full[w], 0, abort_flag);
+        if (mine > 0) wait_phase(&o_full[w], 0, abort_flag);
         tc::fence_after();
-        if (ok && (alt || w < tiles)) {
+        if (*abort_flag) sum = __int_as_float(0x7fffffff);   // NaN in out, lse and the weights that follow from it
+        if (alt || w < tiles) {
             const float inv = sum == 0.f ? 0.f : (I8 ? vnorm * (1.f / 64.f) : 1.f) / sum;
             const float lse = sum == 0.f ? kNegInf : (top == kNegInf ? 0.f : top) + log2f(sum);
             const long long nrows = (long long)p.batch * p.tokens * p.heads;
@@ -773,7 +775,7 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
     constexpr int kStages = G::kStages;
     extern __shared__ __align__(16) char smem_raw[];
     char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2][2], s_free[2][2];
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2][2], s_free[2][2], drained;
     __shared__ __align__(16) float lse[kStages][I8 ? 2 : 1][kTile];   // minus the rows' lse, INT8: their factors
     __shared__ uint32_t tmem_at;
     __shared__ int abort_at;
@@ -799,6 +801,7 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
             mbar_init(&s_full[i >> 1][i & 1], 1);
             mbar_init(&s_free[i >> 1][i & 1], 2 * kTile);
         }
+        mbar_init(&drained, 1);
         abort_at = 0;
         fence_barrier_init();
     }
@@ -901,13 +904,11 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
             // ---- products
             constexpr uint32_t ids = idesc(BF, false, kTile);
             const uint32_t k0 = smem_addr(smem), q0 = smem_addr(smem) + G::kRing;
-            bool ok = true;
-            for (int i = 0; ok && i < n; ++i) {
+            for (int i = 0; i < n; ++i) {
                 const int s = i % kStages;
-                ok = wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag);
-                for (int w = 0; ok && w < 2; ++w) {
-                    if (i >= 2) ok = wait_phase(&s_free[w][i & 1], (uint32_t)(i / 2 - 1) & 1, abort_flag);
-                    if (!ok) break;
+                wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag);
+                for (int w = 0; w < 2; ++w) {
+                    if (i >= 2) wait_phase(&s_free[w][i & 1], (uint32_t)(i / 2 - 1) & 1, abort_flag);
                     __syncwarp();
                     if (elect_one()) {
                         tc::fence_after();
@@ -925,6 +926,11 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
                     }
                     __syncwarp();
                 }
+            }
+            if (__any_sync(0xffffffffu, *abort_flag)) {   // no product is in flight when TMEM is freed
+                if (elect_one()) tc::commit(&drained);
+                mbar_wait(&drained, 0);
+                __syncwarp();
             }
         }
         __syncwarp();
@@ -947,9 +953,9 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
         const float2 k2 = make_float2(ks, ks);
         for (int i = 0; i < n; ++i) {
             const int s = i % kStages;
-            if (!wait_phase(&s_full[w][i & 1], (uint32_t)(i / 2) & 1, abort_flag)) break;
+            wait_phase(&s_full[w][i & 1], (uint32_t)(i / 2) & 1, abort_flag);
             // (the rows' lse: written before the products' wait for the same phase)
-            if (!wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag)) break;
+            wait_phase(&full[s], (uint32_t)(i / kStages) & 1, abort_flag);
             tc::fence_after();
             const uint32_t ts = tmem + (2 * w + (i & 1)) * kTile + half * kCols + lanes;
             uint32_t raw[2][32];
@@ -999,6 +1005,7 @@ __global__ __launch_bounds__(kWeightThreads, 1) void weight_tile_kernel(const Pr
             part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
             total += part[0].x + part[0].y;
         }
+        if (*abort_flag) total = __int_as_float(0x7fffffff);   // (NaN)
         float *halves = &lse[0][0][0];                 // (free once every thread is past its rows)
         static_assert(kStages >= 2, "room for the sums");
         asm volatile("bar.sync 1, 512;" ::: "memory");

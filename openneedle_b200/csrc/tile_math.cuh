@@ -155,8 +155,10 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
         : "memory");
 }
 
-// Bounded wait; on its end the CTA's warps give up (and the kernel raises its
-// fault flag).
+// Bounded wait.  Where one runs out (never in working order) the CTA gives up: its
+// copying threads stop, its other warps, whose lanes have to stay together for the
+// warp-wide instructions, run on without waiting and write NaN, and the kernel
+// raises its fault flag.
 constexpr uint32_t kWaitLimit = 1u << 16;
 __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t a = smem_addr(bar);
@@ -171,6 +173,7 @@ __device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, volat
         : "r"(a), "r"(parity)
         : "memory");
     if (done) return true;
+    if (*abort_flag) return false;
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         asm volatile(
             "{\n\t.reg .pred p;\n\t"

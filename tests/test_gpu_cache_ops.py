@@ -767,3 +767,24 @@ def test_pool_query_shared_in_a_graph(ops):
     again = torch.zeros(64, 1024, device="cuda")
     kv.query_shared_device(list(range(64)), [3999] * 64, q, again)
     assert torch.equal(again, every)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_calls_repeat_themselves(ops, cache):
+    """Bit for bit: no atomics and no order of arrival in out, lse, weights or an eviction."""
+    for t, s in ((1, 900), (70, 300)):
+        c = R.make_inputs(cache, 20, t, 8, 4, 64, 700, s, [t + (37 * i) % (s - t) for i in range(20)], seed=90 + t)
+        first = call(ops, c) + call(ops, c, weigh=True)
+        e = evicted(ops, {**c, "weights": first[3].cpu()}, 60, 2, 5)[0]
+        for _ in range(5):
+            got = call(ops, c) + call(ops, c, weigh=True)
+            again = evicted(ops, {**c, "weights": got[3].cpu()}, 60, 2, 5)[0]
+            for x, y in zip(first + tuple(e), got + tuple(again)):
+                assert x is y is None or torch.equal(x, y)
+
+
+def test_no_wait_ran_out(ops):
+    """None of the calls above has raised the flag that a bounded wait of the tiles sets on its end."""
+    from openneedle_b200 import native
+    torch.cuda.synchronize()
+    assert native.device_fault() == 0
