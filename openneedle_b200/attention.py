@@ -239,7 +239,8 @@ def _bind_operators():
     def current_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 
-    return lib, torch, types, getattr(torch._C, "_cuda_getCurrentRawStream", current_stream)
+    return (lib, torch, types, getattr(torch._C, "_cuda_getCurrentRawStream", current_stream),
+            torch.autograd.forward_ad)
 
 
 def _on_stream(torch, device, stream):
@@ -289,14 +290,17 @@ def _apart(outs, ins):
             end_out = max(end_out, start + n)
 
 
-def _no_gradients(torch, *tensors):
+def _require(*tensors):
+    """Whether any of the tensors requires gradients (a plan's answer: it is kept by their layouts, see _layout)."""
+    return any(x is not None and x.requires_grad for x in tensors)
+
+
+def _no_gradients(torch, forward, require, *tensors):
     """Refuse tensors whose gradients or forward-mode tangents the call would drop (INT8 codes have none, their scales
     may)."""
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+    if require and torch.is_grad_enabled():
         raise ValueError("these operators have no gradients: detach the inputs or call them under torch.no_grad()")
-    forward = torch.autograd.forward_ad
-    if getattr(forward, "_current_level", 0) >= 0 and any(        # (inside of a dual level only)
-            x is not None and forward.unpack_dual(x).tangent is not None for x in tensors):
+    if any(x is not None and forward.unpack_dual(x).tangent is not None for x in tensors):
         raise ValueError("these operators have no gradients: detach the inputs of their tangents")
 
 
@@ -319,7 +323,7 @@ def _strides(axes, *tensors):
 
 
 def _layout(x):
-    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device(), x.requires_grad)
 
 
 def _pointer(x):
@@ -404,12 +408,14 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
         extents = ([_extent(out, "out"), _extent(weights_out, "weights_out")],
                    [_extent(x) for x in (q, k, v, prefix_k, prefix_v, lengths, tokens, k_scales, v_scales,
                                          prefix_k_scales, prefix_v_scales, weights)])
-    return sizes, size, (batch, count, heads), weigh, extents
+    require = _require(q, k, v, prefix_k, prefix_v, weights, k_scales, v_scales, prefix_k_scales, prefix_v_scales, out,
+                       weights_out)
+    return sizes, size, (batch, count, heads), weigh, extents, require
 
 
 def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
             prefix_v_scales, tokens, window, scale, out, return_lse, stream):
-    lib, torch, types, raw_stream = _bind_operators()
+    lib, torch, types, raw_stream, forward = _bind_operators()
     # (numbers from here on: a plan is kept by its options' values, not by the objects that held them)
     window, scale = int(window), None if scale is None else float(scale)
     key = (_layout(q), _layout(k), _layout(v), _layout(lengths), _layout(weights), _layout(weights_out),
@@ -420,9 +426,10 @@ def _attend(q, k, v, lengths, weights, weights_out, prefix_k, prefix_v, k_scales
         plan = _remember(key, _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, prefix_k,
                                               prefix_v, k_scales, v_scales, prefix_k_scales, prefix_v_scales, tokens,
                                               window, scale, out))
-    sizes, size, rows, weigh, extents = plan
-    _no_gradients(torch, q, k, v, prefix_k, prefix_v, weights, k_scales, v_scales, prefix_k_scales, prefix_v_scales,
-                  out, weights_out)
+    sizes, size, rows, weigh, extents, require = plan
+    if require or getattr(forward, "_current_level", 0) >= 0:    # (inside of a dual level)
+        _no_gradients(torch, forward, require, q, k, v, prefix_k, prefix_v, weights, k_scales, v_scales,
+                      prefix_k_scales, prefix_v_scales, out, weights_out)
     device = k.device
     if extents is not None:
         same = weights_out is not None and weights_out.data_ptr() == weights.data_ptr() and \
@@ -509,7 +516,7 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     The result goes to ``out`` (an ``Evicted`` of tensors with n >= keep slots),
     to the inputs themselves (``in_place``; lengths and indices are new), or to
     new tensors of ``keep`` slots, zero behind the kept keys."""
-    lib, torch, types, raw_stream = _bind_operators()
+    lib, torch, types, raw_stream, forward = _bind_operators()
     keep, first, recent, in_place = int(keep), int(first), int(recent), bool(in_place)   # (by value, as above)
     key = (_layout(k), _layout(v), _layout(weights), _layout(lengths), _layout(k_scales), _layout(v_scales), keep,
            first, recent, in_place, None if out is None else tuple(map(_layout, out)))
@@ -517,8 +524,9 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     if plan is None:
         plan = _remember(key, _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales,
                                           out, in_place))
-    sizes, shape, (n_out, n_in) = plan
-    _no_gradients(torch, k, v, weights, k_scales, v_scales, *(() if out is None else out))
+    sizes, shape, (n_out, n_in), require = plan
+    if require or getattr(forward, "_current_level", 0) >= 0:
+        _no_gradients(torch, forward, require, k, v, weights, k_scales, v_scales, *(() if out is None else out))
     device = k.device
     context = _on_stream(torch, device, stream)
     if context is not None:
@@ -550,7 +558,8 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
 
 
 def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_scales, v_scales, out, in_place):
-    """Check an eviction; its packed sizes, [batch, kvheads, keep], and the tensors' extents in bytes."""
+    """Check an eviction; its packed sizes, [batch, kvheads, keep], the tensors' extents in bytes, and whether any of
+    them requires gradients."""
     if k.dim() != 4 or k.dtype not in types:
         raise ValueError("k and v must be [batch, kvheads, capacity, head_dim] of int8, bfloat16 or float16")
     batch, kvheads, capacity, head_dim = k.shape
@@ -590,4 +599,5 @@ def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_sca
         extents = ([_extent(x, "out") for x in out],
                    [_extent(x) for x in (k, v, weights, lengths, k_scales, v_scales)])
     return _EVICT_SIZES.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
-                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep), extents
+                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep), extents, \
+        _require(k, v, weights, k_scales, v_scales, *(() if out is None else out))
