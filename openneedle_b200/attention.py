@@ -280,14 +280,62 @@ def _extent(x, name=None):
 
 def _apart(outs, ins):
     """Refuse outputs that share memory with an input or with one another; (tensor, bytes, name) and (tensor, bytes)."""
+    ins = list(ins)
     spans = sorted([(x.data_ptr(), n, name) for x, n, name in outs if n] + [(x.data_ptr(), n, "") for x, n in ins if n])
     end = end_out = 0                                      # of all spans, of the outputs' so far
     for start, n, name in spans:
         if start < (end if name else end_out):
-            raise ValueError(f"{name or 'an output'} overlaps an input or another output")
+            break
         end = max(end, start + n)
         if name:
             end_out = max(end_out, start + n)
+    else:
+        return
+    # address ranges meet: those of rows that lie between one another's (K and V of one tensor) may share nothing
+    for i, (x, n, name) in enumerate(outs):
+        for y, m in [o[:2] for o in outs[i + 1:]] + ins:
+            if n and m and x.data_ptr() < y.data_ptr() + m and y.data_ptr() < x.data_ptr() + n and _share(x, y):
+                raise ValueError(f"{name} overlaps an input or another output")
+
+
+def _axes(x):
+    """A tensor's axes as [(stride, elements)] in bytes, and the bytes that are contiguous at each of their points."""
+    width = x.element_size()
+    axes = sorted((s * width, n) for n, s in zip(x.shape, x.stride()) if n > 1)
+    while axes and axes[0][0] <= width:                    # (0: expanded)
+        s, n = axes.pop(0)
+        width += (n - 1) * s
+    return axes, width
+
+
+def _share(x, y):
+    """Whether any byte belongs to both tensors (or may, where their strides are too involved to tell)."""
+    (xa, xw), (ya, yw) = _axes(x), _axes(y)
+    steps = {}                                             # stride: the range of the difference of x's and y's index
+    for s, n in xa:
+        lo, hi = steps.get(s, (0, 0))
+        steps[s] = lo, hi + n - 1
+    for s, n in ya:
+        lo, hi = steps.get(s, (0, 0))
+        steps[s] = lo - n + 1, hi
+    steps = sorted(steps.items(), reverse=True)
+    budget = 1000
+
+    def meets(i, low, high):                               # a sum of the steps from i on in [low, high]
+        nonlocal budget
+        budget -= 1
+        if budget < 0:
+            return True
+        if i == len(steps):
+            return low <= 0 <= high
+        s, (lo, hi) = steps[i]
+        least, most = (sum(r[e] * t for t, r in steps[i + 1:]) for e in (0, 1))
+        first, last = max(lo, -((most - low) // s)), min(hi, (high - least) // s)
+        return any(meets(i + 1, low - d * s, high - d * s) for d in range(first, last + 1))
+
+    # x's byte minus y's: x.ptr + steps - y.ptr, within (-xw, yw)
+    offset = x.data_ptr() - y.data_ptr()
+    return meets(0, 1 - xw - offset, yw - 1 - offset)
 
 
 def _require(*tensors):
@@ -527,6 +575,10 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
     sizes, shape, (n_out, n_in), require = plan
     if require or getattr(forward, "_current_level", 0) >= 0:
         _no_gradients(torch, forward, require, k, v, weights, k_scales, v_scales, *(() if out is None else out))
+    if in_place:
+        _apart([(x, n, "the cache") for x, n in zip((k, v, weights, k_scales, v_scales), n_out)], [(lengths, n_in[0])])
+    elif out is not None:
+        _apart([(x, n, "out") for x, n in zip(out, n_out)], zip((k, v, weights, lengths, k_scales, v_scales), n_in))
     device = k.device
     context = _on_stream(torch, device, stream)
     if context is not None:
@@ -534,7 +586,6 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
             return evict(k, v, weights, lengths, keep, first=first, recent=recent, k_scales=k_scales, v_scales=v_scales,
                          out=out, in_place=in_place)
     if in_place:
-        _apart([(x, n, "the cache") for x, n in zip((k, v, weights, k_scales, v_scales), n_out)], [(lengths, n_in[0])])
         out = Evicted(k, v, weights, torch.empty(shape[:1], dtype=torch.int32, device=device),
                       torch.empty(shape, dtype=torch.int32, device=device), k_scales, v_scales)
     elif out is None:
@@ -547,7 +598,6 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
                       None if v_scales is None else torch.zeros(shape, **f32))
     else:
         out = Evicted(*out)
-        _apart([(x, n, "out") for x, n in zip(out, n_out)], zip((k, v, weights, lengths, k_scales, v_scales), n_in))
     args = sizes + _EVICT_POINTERS.pack(
         k.data_ptr(), v.data_ptr(), _pointer(k_scales), _pointer(v_scales), weights.data_ptr(), lengths.data_ptr(),
         out.k.data_ptr(), out.v.data_ptr(), _pointer(out.k_scales), _pointer(out.v_scales), out.weights.data_ptr(),

@@ -301,3 +301,51 @@ def test_evictions_beyond_32_bit_indexes_are_refused(change):
         *[4096] * 5, 8192, *[16384] * 6, 65536)
     assert lib.needle2_evict_device(args, None) == -1
     assert "too large" in attention.last_error()
+
+
+def test_interleaved_tensors_share_nothing():
+    """Rows between one another's: K and V of one tensor, an output in a fused projection beside its queries."""
+    c = inputs("bf16")
+    both = torch.zeros(2, 4, 30, 2, 64, dtype=torch.bfloat16)
+    per = torch.zeros(2, 2, 4, 30, 64, dtype=torch.bfloat16)
+    for k, v in ((both[:, :, :, 0], both[:, :, :, 1]), (per[:, 0], per[:, 1])):
+        c["k"], c["v"] = k, v
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            evict(c, in_place=True)
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            attend(c, out=torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16))
+    c["v"] = both.flatten(3)[:, :, :, 63:127]                # one value of each row is K's
+    c["k"] = both[:, :, :, 0]
+    with pytest.raises(ValueError, match="overlaps"):
+        evict(c, in_place=True)
+    fused = torch.zeros(2, 1, 24, 64, dtype=torch.bfloat16)
+    c["q"] = fused[:, :, :8]
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        attend(c, out=fused[:, :, 16:])
+    with pytest.raises(ValueError, match="out overlaps"):
+        attend(c, out=fused[:, :, 7:15])
+
+
+def test_shared_bytes_against_a_count():
+    """Whether two strided tensors share memory, against the bytes themselves."""
+    import random
+    rng = random.Random(5)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        flat = torch.zeros(4000, dtype=torch.uint8)
+        pair = []
+        for size in rng.choices((1, 2, 4), k=2):
+            shape = [rng.randint(1, 4) for _ in range(rng.randint(0, 3))] + [rng.choice((1, 4, 6))]
+            strides = [rng.choice((0, 1, 2, 4, 6, 8, 12, 24, 40, 7, 13)) for _ in shape[:-1]] + [1]
+            start = rng.randint(0, 30) * 4
+            base = flat if size == 1 else flat.view(torch.int16 if size == 2 else torch.int32)
+            x = base.as_strided(shape, strides, start // size)
+            points = [start]
+            for n, s in zip(shape, strides):
+                points = [p + i * s * size for p in points for i in range(n)]
+            pair.append((x, {p + i for p in points for i in range(size)}))
+        (x, a), (y, b) = pair
+        got = attention._share(x, y)
+        seen[got] += 1
+        assert got == bool(a & b), (x.shape, x.stride(), y.shape, y.stride())
+    assert min(seen.values()) > 300

@@ -788,3 +788,28 @@ def test_no_wait_ran_out(ops):
     from openneedle_b200 import native
     torch.cuda.synchronize()
     assert native.device_fault() == 0
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("layout", ("key", "sequence"))
+def test_keys_and_values_of_one_tensor(ops, cache, layout):
+    """K and V rows side by side, or a sequence's behind one another: attended and thinned out in place."""
+    b, kv, s, d = 3, 4, 300, 64
+    c = R.make_inputs(cache, b, 1, 8, kv, d, 0, s, [300, 120, 77], seed=95)
+    plain = call(ops, c, weigh=True)
+    e, _ = evicted(ops, c, 90, 3, 10)
+    dev = cuda(c)
+    shape = (b, kv, s, 2, d) if layout == "key" else (b, 2, kv, s, d)
+    whole = torch.zeros(shape, dtype=c["k"].dtype, device="cuda")
+    k, v = (whole[:, :, :, i] if layout == "key" else whole[:, i] for i in (0, 1))
+    k.copy_(dev["k"])
+    v.copy_(dev["v"])
+    scales = {n: dev[n] for n in ("k_scales", "v_scales")}
+    got = ops.accumulate_attention(dev["q"], k, v, dev["lengths"], dev["weights"], **scales)
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+    i = ops.evict(k, v, dev["weights"], dev["lengths"], 90, first=3, recent=10, in_place=True, **scales)
+    assert torch.equal(i.indices, e.indices) and torch.equal(i.lengths, e.lengths)
+    for j, n in enumerate(e.lengths.tolist()):
+        for x, y in ((k, e.k), (v, e.v), (dev["weights"], e.weights)):
+            assert torch.equal(x[j, :, :n], y[j, :, :n])
+        assert torch.equal(k[j, :, n:], c["k"][j, :, n:].cuda()) and torch.equal(v[j, :, n:], c["v"][j, :, n:].cuda())
