@@ -769,6 +769,23 @@ def test_pool_query_shared_in_a_graph(ops):
     assert torch.equal(again, every)
 
 
+@pytest.mark.parametrize("cache", ("bf16", "f16"))
+@pytest.mark.parametrize("d", (64, 128))
+def test_long_sums_of_single_tokens_in_sixteen_bits(ops, cache, d):
+    """Single tokens of sequences that fill the machine over 262144 keys of one sign, the longest range that streams:
+    a warp takes a quarter of it, 4096 cut sums of 16 keys, 2^-25 each on the average: 2^-13; the output's rounding:
+    2^-11 or 2^-8; and a twentieth for the weights' sums and the merge."""
+    b, kv, keys = 150, 4, 1 << 18
+    g = torch.Generator(device="cuda").manual_seed(d)
+    v = (torch.rand(1, kv, keys, d, generator=g, device="cuda") + 0.5).to(R.TYPES[cache])
+    own = v.expand(b, -1, -1, -1)                            # the sequences' own keys: one cache for all
+    q = torch.zeros(b, kv, d, dtype=v.dtype, device="cuda")
+    out = ops.prefix_attention(q, own, own, torch.full((b,), keys, dtype=torch.int32, device="cuda"))
+    want = v[0].double().mean(1)
+    off = ((out.double() - want) / want).abs()
+    assert float(off.max()) <= 1.05 * (2.0 ** -13 + torch.finfo(v.dtype).eps / 2), float(off.max())
+
+
 @pytest.mark.parametrize("cache", CACHES)
 def test_calls_repeat_themselves(ops, cache):
     """Bit for bit: no atomics and no order of arrival in out, lse, weights or an eviction."""
@@ -781,13 +798,6 @@ def test_calls_repeat_themselves(ops, cache):
             again = evicted(ops, {**c, "weights": got[3].cpu()}, 60, 2, 5)[0]
             for x, y in zip(first + tuple(e), got + tuple(again)):
                 assert x is y is None or torch.equal(x, y)
-
-
-def test_no_wait_ran_out(ops):
-    """None of the calls above has raised the flag that a bounded wait of the tiles sets on its end."""
-    from openneedle_b200 import native
-    torch.cuda.synchronize()
-    assert native.device_fault() == 0
 
 
 @pytest.mark.parametrize("cache", CACHES)
@@ -813,3 +823,10 @@ def test_keys_and_values_of_one_tensor(ops, cache, layout):
         for x, y in ((k, e.k), (v, e.v), (dev["weights"], e.weights)):
             assert torch.equal(x[j, :, :n], y[j, :, :n])
         assert torch.equal(k[j, :, n:], c["k"][j, :, n:].cuda()) and torch.equal(v[j, :, n:], c["v"][j, :, n:].cuda())
+
+
+def test_no_wait_ran_out(ops):
+    """None of the calls above has raised the flag that a bounded wait of the tiles sets on its end."""
+    from openneedle_b200 import native
+    torch.cuda.synchronize()
+    assert native.device_fault() == 0
