@@ -370,6 +370,13 @@ def _strides(axes, *tensors):
     return [n for x in tensors for n in ((0,) * axes if x is None else x.stride()[:axes])]
 
 
+def _pack(sizes, *numbers):
+    try:
+        return sizes.pack(*numbers)
+    except struct.error:
+        raise ValueError("the call is too large: its sizes do not fit the library's numbers") from None
+
+
 def _layout(x):
     return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device(), x.requires_grad)
 
@@ -441,9 +448,9 @@ def _plan_attention(lib, torch, types, q, k, v, lengths, weights, weights_out, p
         return [x.stride(0), 0, x.stride(1)] if single else list(x.stride()[:3])
 
     wide = [kvheads * capacity, capacity, 1] if weights_out is None else list(weights_out.stride())
-    sizes = _ATTENTION_SIZES.pack(
-        batch, count, heads, kvheads, head_dim, prefix, capacity, window, cache_type, scale, *rows(q), *rows(out),
-        *_strides(3, k, v, k_scales, v_scales), *_strides(2, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales),
+    sizes = _pack(
+        _ATTENTION_SIZES, batch, count, heads, kvheads, head_dim, prefix, capacity, window, cache_type, scale, *rows(q),
+        *rows(out), *_strides(3, k, v, k_scales, v_scales), *_strides(2, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales),
         *_strides(3, weights), *wide)
     one = 4096 if weigh else 0                             # (given or not: the pointers are not read)
     # the split goes by the multiprocessors of the current device, which has to be the tensors' then as in the call
@@ -648,6 +655,7 @@ def _plan_evict(torch, types, k, v, weights, lengths, keep, first, recent, k_sca
     elif out is not None:
         extents = ([_extent(x, "out") for x in out],
                    [_extent(x) for x in (k, v, weights, lengths, k_scales, v_scales)])
-    return _EVICT_SIZES.pack(batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
-                             *_strides(3, k, v, k_scales, v_scales, weights), *to), (batch, kvheads, keep), extents, \
-        _require(k, v, weights, k_scales, v_scales, *(() if out is None else out))
+    sizes = _pack(_EVICT_SIZES, batch, kvheads, head_dim, capacity, slots, keep, first, recent, types[k.dtype][0],
+                  *_strides(3, k, v, k_scales, v_scales, weights), *to)
+    require = _require(k, v, weights, k_scales, v_scales, *(() if out is None else out))
+    return sizes, (batch, kvheads, keep), extents, require

@@ -349,3 +349,19 @@ def test_shared_bytes_against_a_count():
         seen[got] += 1
         assert got == bool(a & b), (x.shape, x.stride(), y.shape, y.stride())
     assert min(seen.values()) > 300
+
+
+def test_sizes_beyond_the_librarys_numbers():
+    c = inputs("bf16")
+    with pytest.raises(ValueError, match="too large"):
+        evict(c, keep=1 << 31)
+    for scale in (1e39, 1e-50):                              # infinity and zero in 32 bits
+        with pytest.raises(ValueError, match="scale must be positive and finite"):
+            attend(c, scale=scale)
+    for n in ("k", "v"):
+        c[n] = c[n][:, :, :1].expand(2, 4, 1 << 31, 64)
+    with pytest.raises(ValueError, match="too large"):
+        attend(c)
+    c["weights"] = c["weights"][:, :, :1].expand(2, 4, 1 << 31)
+    with pytest.raises(ValueError, match="too large"):
+        evict(c)
