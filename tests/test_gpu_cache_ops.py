@@ -825,6 +825,51 @@ def test_keys_and_values_of_one_tensor(ops, cache, layout):
         assert torch.equal(k[j, :, n:], c["k"][j, :, n:].cuda()) and torch.equal(v[j, :, n:], c["v"][j, :, n:].cuda())
 
 
+@pytest.mark.parametrize("in_place", (False, True))
+def test_evict_beyond_32_bit_offsets(ops, in_place):
+    """The last keys of a cache of 34 million INT8 rows (2.2 GB) have the weights."""
+    s, n, keep, first, recent = 34_000_000, 34_000_000 - 3, 700, 10, 20
+    g = torch.Generator("cuda").manual_seed(2)
+    k = torch.zeros(1, 1, s, 64, dtype=torch.int8, device="cuda")
+    k[:, :, -2000:] = torch.randint(-127, 128, (1, 1, 2000, 64), generator=g, device="cuda", dtype=torch.int8)
+    k[:, :, :first] = 7
+    v = -k
+    scales = torch.rand(1, 1, s, generator=g, device="cuda")
+    w = torch.zeros(1, 1, s, device="cuda")
+    w[:, :, -1500:] = torch.rand(1, 1, 1500, generator=g, device="cuda") + 0.5
+    x = w[0, 0, :n].clone()
+    x[:first] = x[n - recent:] = 2.0
+    at = torch.sort(x, descending=True, stable=True).indices[:keep].sort().values
+    want = [y[0, 0][at] for y in (k, v, w, scales)]
+    e = ops.evict(k, v, w, torch.tensor([n], dtype=torch.int32, device="cuda"), keep, first=first, recent=recent,
+                  k_scales=scales, v_scales=scales.clone(), in_place=in_place)
+    assert torch.equal(e.indices[0, 0], at.int()) and int(e.lengths) == keep
+    for x, y in zip((e.k, e.v, e.weights, e.k_scales), want):
+        assert torch.equal(x[0, 0, :keep], y)
+    assert not e.weights[0, 0, keep:].any()
+
+
+@pytest.mark.parametrize("t", (1, 100))
+def test_weights_beyond_32_bit_offsets(ops, t):
+    """The weights of the last keys of the same cache, and the others' as they were."""
+    s, n = 34_000_000, 34_000_000 - 3
+    g = torch.Generator("cuda").manual_seed(3)
+    k = torch.zeros(1, 1, s, 64, dtype=torch.int8, device="cuda")
+    k[:, :, -400:] = torch.randint(-127, 128, (1, 1, 400, 64), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.full((1, 1, s), 0.01, device="cuda")
+    q = torch.randn(1, t, 2, 64, generator=g, device="cuda")
+    w = torch.rand(1, 1, s, generator=g, device="cuda")
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    _, got = ops.accumulate_attention(q, k, k, lengths, w, k_scales=scales, v_scales=scales, window=64)
+    tail = slice(s - 400, s)
+    _, want = ops.accumulate_attention(q, k[:, :, tail].clone(), k[:, :, tail].clone(), lengths - (s - 400),
+                                       w[:, :, tail].clone(), k_scales=scales[:, :, tail].clone(),
+                                       v_scales=scales[:, :, tail].clone(), window=64)
+    # the same keys from the front of a small cache: only the order of the sums may differ
+    assert (got[:, :, tail] - want).abs().max() <= 1e-5 * want.max()
+    assert torch.equal(got[:, :, :s - 400], w[:, :, :s - 400])
+
+
 def test_no_wait_ran_out(ops):
     """None of the calls above has raised the flag that a bounded wait of the tiles sets on its end."""
     from openneedle_b200 import native
