@@ -255,10 +255,16 @@ int needle2_kv_export(void *kv, int session, int8_t *keys, int8_t *values, float
  * weight is copied).  Rows of out and lse for t >= tokens[b] are left as they were.
  *
  * Strides are in elements; the last axis of q, out, k, v and the prefix is
- * contiguous, and their pointers and strides are multiples of 16 bytes.
+ * contiguous, and their pointers and strides are multiples of 16 bytes.  Inputs
+ * may be expanded (strides of 0) and may be views of one another: a prefix kept in
+ * a cache's first slots.  Up to 0x7e000000 slots and prefix keys.
  * Lengths are clamped to [0, capacity], token counts to [0, tokens].  Own keys at
  * and behind the length are never used, whatever they hold; every key that any
  * query of its sequence sees must be finite.
+ *
+ * needle2_b200_device_fault() tells whether a bounded wait of the tile kernels has
+ * run out, which no working order brings about: the call's outputs that depend on
+ * it, accumulated weights among them, are NaN then.
  */
 typedef struct {
     int batch, tokens, heads, kvheads, head_dim;   /* head_dim 64 or 128; heads a multiple of kvheads */
@@ -273,7 +279,7 @@ typedef struct {
     long long prefix_k_scale_stride[2], prefix_v_scale_stride[2];
     long long weights_stride[3], weights_out_stride[3];
     const void *q;                                 /* [batch][tokens][heads][head_dim] */
-    void *out;                                     /* like q; not overlapping the inputs */
+    void *out;                                     /* like q; sharing no byte with the inputs */
     const void *k, *v;                             /* [batch][kvheads][capacity][head_dim] */
     const float *k_scales, *v_scales;              /* [batch][kvheads][capacity], INT8 only */
     const void *prefix_k, *prefix_v;               /* [kvheads][prefix][head_dim] */

@@ -205,6 +205,9 @@ class KVCache:
 # (rows on 16-byte boundaries), run on torch's current stream or on `stream`
 # without synchronising, allocate through torch (results and workspace belong to
 # that stream, so captured graphs each keep their own) and have no gradients.
+# Inputs may be views of one another; outputs share no byte with them unless a call
+# says so. A bounded wait of a kernel that ran out, which no working order brings
+# about, leaves NaN in the call's outputs and sets native.device_fault().
 
 # needle2_prefix_attention_args and needle2_evict_args: sizes and strides, then the pointers
 _ATTENTION_SIZES = struct.Struct("@9if32q")
@@ -533,9 +536,10 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, *, k_scales
     Token t of sequence b stands at own index ``lengths[b] - tokens[b] + t`` and
     sees the whole prefix and its own keys up to there, the last ``window`` of
     them if window > 0.  ``tokens`` (int32 [batch]) says how many of q's tokens a
-    sequence has; rows behind them are left as they were in ``out``.  A query
-    that sees nothing gets zeros.  With ``return_lse`` also the natural logarithm
-    of the softmax's denominators, float32 [batch, tokens, heads]."""
+    sequence has; rows behind them are left as they were in ``out`` (in new
+    tensors, as in the returned lse, they hold anything).  A query that sees nothing
+    gets zeros.  With ``return_lse`` also the natural logarithm of the softmax's
+    denominators, float32 [batch, tokens, heads]."""
     out, lse, _ = _attend(q, k, v, lengths, None, None, prefix_k, prefix_v, k_scales, v_scales, prefix_k_scales,
                           prefix_v_scales, tokens, window, scale, out, return_lse, stream)
     return (out, lse) if return_lse else out
@@ -562,8 +566,8 @@ def evict(k, v, weights, lengths, keep, *, first=0, recent=0, k_scales=None, v_s
 
     Of a sequence's ``lengths[b]`` keys, ``keep`` stay per KV head where there
     are more: the first ``first``, the last ``recent`` and, of those between
-    them, the ones of the largest weight (the lower index of equal ones, NaN
-    last).  They are packed in their order into the front of the result, an
+    them, the ones of the largest weight (the lower index of equal ones, NaN as
+    -inf).  They are packed in their order into the front of the result, an
     ``Evicted`` of k, v, weights [batch, kvheads, n, ..], lengths, indices
     [batch, kvheads, keep] (-1 behind the kept) and an INT8 cache's scales.
     Slots behind the kept keys have weight 0 and otherwise stay as they were.

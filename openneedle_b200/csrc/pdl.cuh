@@ -7,14 +7,19 @@
 namespace nb200 {
 
 // kernel<<<grid, block, smem, st>>>(args...) that may begin while the previous
-// kernel in the stream drains (programmatic stream serialisation).  Every
-// kernel launched this way executes griddepcontrol.wait before it reads or
-// writes memory that earlier kernels use.  The kernels do not trigger their
-// successors early (griddepcontrol.launch_dependents): on the decode step a
-// successor released at the start of its predecessor occupies SM slots while
-// it waits and was measured slower (2.34 ms per config-5 step) than leaving
+// kernel in the stream drains (programmatic stream serialisation).  A kernel
+// launched this way executes griddepcontrol.wait before it reads or writes
+// memory that the previous kernel writes or uses, and in every CTA, so that it
+// ends after the previous kernel has.  With one exception the kernels do not
+// trigger their successors early (griddepcontrol.launch_dependents): on the decode
+// step a successor released at the start of its predecessor occupies SM slots
+// while it waits and was measured slower (2.34 ms per config-5 step) than leaving
 // the release to the predecessor's exit (2.21 ms) or not using programmatic
-// launches at all (2.25 ms).
+// launches at all (2.25 ms).  The exception: prefix_tile_kernel, itself launched
+// after everything before it has ended, triggers at its start where
+// prefix_stream_kernel of the same call follows; the two write apart from one
+// another, and the streaming kernel waits at its end instead of its start, so that
+// what follows it follows both.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                        Args &&...args) {

@@ -505,8 +505,10 @@ __device__ __forceinline__ void stream_unit(const PrefixAttn &p, const StreamGri
                     mma16816<false>(o[4 * x + 3], a, i8x2_to_f16<0x4342>(h01), i8x2_to_f16<0x4342>(h23));
                 }
             } else {
-                // the softmax weights are rounded to the cache's type for the product;
-                // their sum keeps 32 bits
+                // the softmax weights are rounded to the cache's type for the product, off by
+                // half a step of each at most; their sum keeps 32 bits (two sequences of 200
+                // keys in bf16: 1.7e-3 from the definition, 1.6e-3 with 32-bit weights, the
+                // output's rounding the most of it)
                 a[0] = pack2<BF>(z[2 * k][0], z[2 * k][1]);
                 a[1] = pack2<BF>(z[2 * k][2], z[2 * k][3]);
                 a[2] = pack2<BF>(z[2 * k + 1][0], z[2 * k + 1][1]);

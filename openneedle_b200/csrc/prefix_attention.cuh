@@ -97,8 +97,8 @@ struct PrefixSplit {
 bool launch_prefix_finish(const PrefixAttn &p, cudaStream_t st);
 bool launch_key_weights(const PrefixAttn &p, cudaStream_t st);
 // Streaming kernel: `prefix` / `own` say which key sets it takes; after_tiles:
-// the tile kernel of the same call was launched before it with stream_next, runs
-// beside it, and has ended when it ends; joint: the own keys' units take the
+// the tile kernel of the same call was launched before it with stream_next, may
+// still run, and has ended when it ends; joint: the own keys' units take the
 // prefix too (prefix_slots 0).
 bool launch_prefix_stream(const PrefixAttn &p, bool prefix, bool own, bool joint, bool after_tiles, cudaStream_t st);
 // Tile kernel for the sets whose split says `tiles`; joint: the own keys' units
